@@ -51,7 +51,7 @@
 extern "C" {
 #endif
 
-#define KDA_ABI_VERSION 6
+#define KDA_ABI_VERSION 7
 
 enum kda_dtype { KDA_F32 = 0, KDA_BF16 = 1, KDA_F16 = 2 };
 
@@ -236,6 +236,61 @@ KDA_API int kda_bwd_noalloc(const KdaDesc *desc, const void *q, const void *k, c
                             const void *saved, const void *dO, const float *dstateT,
                             void *dq, void *dk, void *dv, float *dg, void *dbeta, float *dstate0,
                             void *stream);
+
+/* ---- AdamW over many tensors at once ----
+ * One tensor of the step.  p (updated) and g have dtype `dtype`, numel contiguous elements each.
+ * The states m, v: float32 [numel] (state_bits 32), or 8-bit codes [numel] with one exponent byte
+ * per 256 consecutive elements, m_exp, v_exp [ceil(numel / 256)] (state_bits 8; all zero bytes
+ * are the zero state).  ema: float32 [numel], read only where KdaAdamW.use_ema is set.  Every
+ * pointer needs its element's alignment only; 16 bytes (8 for codes) are faster.  The tensors of one call must not
+ * overlap. */
+typedef struct KdaAdamWTensor {
+  void *p;
+  const void *g;
+  void *m, *v;
+  uint8_t *m_exp, *v_exp;
+  float *ema;
+  int64_t numel;
+  int32_t dtype, reserved;
+} KdaAdamWTensor;
+
+typedef struct KdaAdamW {
+  double lr, beta1, beta2, eps, weight_decay;
+  double max_grad_norm;   /* clip the gradients' global 2-norm to this; 0: no clipping */
+  double ema_decay;
+  int64_t step;           /* this step's number, from 1 (unused with step_dev) */
+  uint32_t seed;          /* of the 8-bit states' stochastic rounding */
+  int32_t state_bits;     /* 32, or 8 (eps at least 1e-30: magnitudes below 2^-126 count as zero) */
+  int32_t bias_correction;
+  int32_t use_ema;
+  int32_t norm_given;     /* with clipping: grad_norm holds ||g|| already (kda_grad_norm), read instead
+                             of computed: how several calls clip by one norm */
+  int32_t reserved;
+} KdaAdamW;
+
+/* One AdamW step over `count` tensors (a host array, read before the call returns):
+ *   g <- g min(1, max_grad_norm / (||g|| + 1e-6));  m <- beta1 m + (1 - beta1) g;
+ *   v <- beta2 v + (1 - beta2) g^2;
+ *   p <- p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps);
+ *   ema <- ema_decay ema + (1 - ema_decay) p
+ * (without bias_correction both corrections are 1).  For capture into a graph, step_dev (a
+ * device counter, advanced by the call before it is used) and lr_dev (a device float) replace step
+ * and lr.  grad_norm (device float, may be NULL) receives ||g|| over all tensors before
+ * clipping.  The workspace (kda_adamw_workspace_bytes) is needed with clipping, grad_norm,
+ * step_dev or lr_dev.  Results do not depend on the order in which blocks run.
+ * Counterpart: the trainers' AdamW, gradient clipping and ModelEMA (train_mlx_k400.py:176-222,
+ * :379-408). */
+KDA_API size_t kda_adamw_workspace_bytes(int64_t count);
+KDA_API int kda_adamw_step(const KdaAdamW *args, const KdaAdamWTensor *tensors, int64_t count,
+                           int64_t *step_dev, const float *lr_dev, float *grad_norm, void *ws,
+                           size_t ws_bytes, void *stream);
+/* The global 2-norm of the tensors' g (the other pointers are not read), to a device float. */
+KDA_API int kda_grad_norm(const KdaAdamWTensor *tensors, int64_t count, float *norm, void *ws,
+                          size_t ws_bytes, void *stream);
+/* An 8-bit state's values as bf16 (exact): n codes and ceil(n / 256) exponent bytes; is_signed: m's
+ * format, else v's. */
+KDA_API int kda_decode_state8(int64_t n, int is_signed, const uint8_t *code, const uint8_t *exp,
+                              void *out, void *stream);
 
 #ifdef __cplusplus
 }

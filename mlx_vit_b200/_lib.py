@@ -12,7 +12,7 @@ import threading
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libkda_b200.so")
 
-KDA_ABI_VERSION = 6
+KDA_ABI_VERSION = 7
 KDA_F32, KDA_BF16, KDA_F16 = 0, 1, 2
 KDA_FLAG_FORCE_GENERIC = 0x1
 KDA_FLAG_DEBUG_WAIT_TIMEOUT = 0x2
@@ -30,7 +30,8 @@ EXPORTS = ("kda_abi_version", "kda_strerror", "kda_check_desc", "kda_workspace_b
            "kda_saved_bytes", "kda_launch_counter", "kda_device_status", "kda_fwd", "kda_bwd",
            "kda_bwd_noalloc", "kda_fwd_gated", "kda_bwd_gated", "kda_fwd_recurrent",
            "kda_l2norm_silu_fwd", "kda_l2norm_silu_bwd", "kda_gated_rmsnorm_fwd", "kda_gated_rmsnorm_bwd",
-           "kda_conv_silu_fwd", "kda_conv_silu_bwd")
+           "kda_conv_silu_fwd", "kda_conv_silu_bwd",
+           "kda_adamw_workspace_bytes", "kda_adamw_step", "kda_grad_norm", "kda_decode_state8")
 
 
 class KdaStrides(ctypes.Structure):
@@ -53,6 +54,16 @@ class KdaGate(ctypes.Structure):
                 ("b", ctypes.c_void_p), ("allow_neg_eigval", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
+class KdaAdamW(ctypes.Structure):
+    """The constants of one AdamW step (include/kda_b200.h, KdaAdamW)."""
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+                ("eps", ctypes.c_double), ("weight_decay", ctypes.c_double),
+                ("max_grad_norm", ctypes.c_double), ("ema_decay", ctypes.c_double),
+                ("step", ctypes.c_int64), ("seed", ctypes.c_uint32), ("state_bits", ctypes.c_int32),
+                ("bias_correction", ctypes.c_int32), ("use_ema", ctypes.c_int32),
+                ("norm_given", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
 class KdaError(RuntimeError):
     def __init__(self, status: int, msg: str, where: str):
         super().__init__(f"{where}: {STATUS.get(status, status)} ({msg})")
@@ -60,6 +71,7 @@ class KdaError(RuntimeError):
 
 
 _lib = None
+_tensors = None
 _lock = threading.Lock()
 
 
@@ -102,6 +114,14 @@ def _declare(L):
                  ("kda_conv_silu_bwd", [i64, i64, I, I, P, P, P, P, P, P, P, I, f32, P, P])):
         getattr(L, n).restype = I
         getattr(L, n).argtypes = a
+    # the tensor table (KdaAdamWTensor) is passed as an array of 9 int64 per tensor
+    L.kda_adamw_workspace_bytes.restype = S
+    L.kda_adamw_workspace_bytes.argtypes = [i64]
+    for n, a in (("kda_adamw_step", [ctypes.POINTER(KdaAdamW), P, i64, P, P, P, P, S, P]),
+                 ("kda_grad_norm", [P, i64, P, P, S, P]),
+                 ("kda_decode_state8", [i64, I, P, P, P, P])):
+        getattr(L, n).restype = I
+        getattr(L, n).argtypes = a
 
 
 def lib(path: str | None = None):
@@ -127,6 +147,20 @@ def lib(path: str | None = None):
         if path is None:
             _lib = L
         return L
+
+
+def tensors():
+    """The host module that reads lists of torch tensors (csrc/tensors_module.cpp); raises if it is
+    not built."""
+    global _tensors
+    if _tensors is None:
+        try:
+            from . import _tensors as module
+        except ImportError as e:
+            raise RuntimeError("mlx_vit_b200/_tensors.so not built or not loadable: run "
+                               "`python -m mlx_vit_b200.build`") from e
+        _tensors = module
+    return _tensors
 
 
 def check(status: int, where: str):

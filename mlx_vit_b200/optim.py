@@ -1,0 +1,249 @@
+"""AdamW over a model's tensors in one kernel launch, with float32 or 8-bit states.
+
+``AdamW`` is a ``torch.optim.Optimizer`` for the training step around the KDA layers; the
+reference trainers' optimizer, gradient clipping and shadow average (train_mlx_k400.py:176-222,
+:379-408) are one pass here:
+
+    g   <- g min(1, max_grad_norm / (||g|| + 1e-6))
+    m   <- beta1 m + (1 - beta1) g
+    v   <- beta2 v + (1 - beta2) g^2
+    p   <- p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
+    ema <- ema_decay ema + (1 - ema_decay) p
+
+``adamw_step`` is the same step on lists of tensors, ``grad_norm`` the global gradient norm alone.
+All launches go on the current torch CUDA stream; there is no CPU path.
+
+With ``state_bits=8`` m and v are held as one byte an element plus one exponent byte per
+``STATE_BLOCK`` consecutive elements: e is float32's exponent field of the block's largest
+magnitude plus one, and a code's magnitude 8 k + f stands for (1 + f / 8) 2^(k - L + e - 127),
+zero for zero; m has a sign in bit 7 and L = 15, v has L = 31.  Values are rounded to their three
+bits of mantissa stochastically (to nearest, v could never decay by beta2 = 0.999 a step), by bits
+that a hash of (seed, step, tensor, element) gives: the same call gives the same states.  Magnitudes
+below the least code become it or zero for m, unbiased, and the least code for v.  A block that
+holds a value that is not finite reads back as NaN.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _lib
+
+STATE_BLOCK = 256
+
+State8 = Tuple[torch.Tensor, torch.Tensor]
+
+
+def zeros_state8(p: torch.Tensor) -> State8:
+    """The zero 8-bit state of a tensor: (codes, exponents)."""
+    n = p.numel()
+    return (torch.zeros(n, dtype=torch.uint8, device=p.device),
+            torch.zeros(-(-n // STATE_BLOCK), dtype=torch.uint8, device=p.device))
+
+
+def decode_state8(codes: torch.Tensor, exps: torch.Tensor, signed: bool) -> torch.Tensor:
+    """The values of an 8-bit state as bf16, which holds them exactly, in the codes' shape."""
+    _need(codes.is_cuda and exps.is_cuda and codes.device == exps.device, "an 8-bit state lies on one CUDA device")
+    _need(codes.dtype == torch.uint8 and exps.dtype == torch.uint8, "codes and exponents are uint8")
+    _need(codes.is_contiguous() and exps.is_contiguous(), "codes and exponents must be contiguous")
+    n = codes.numel()
+    _need(exps.numel() == -(-n // STATE_BLOCK), f"{n} codes take {-(-n // STATE_BLOCK)} exponents, got {exps.numel()}")
+    out = torch.empty(codes.shape, dtype=torch.bfloat16, device=codes.device)
+    with torch.cuda.device(codes.device):
+        _lib.check(_lib.lib().kda_decode_state8(n, int(signed), codes.data_ptr(), exps.data_ptr(), out.data_ptr(),
+                                                torch.cuda.current_stream().cuda_stream), "kda_decode_state8")
+    return out
+
+
+def _need(ok, msg):
+    if not ok:
+        raise ValueError(msg)
+
+
+def _workspace(count, dev):
+    n = _lib.lib().kda_adamw_workspace_bytes(count)
+    return torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", dev)), n
+
+
+@torch.no_grad()
+def grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
+    """The 2-norm of all gradients together, a float32 scalar on their device (sums in 64 bits)."""
+    grads = list(grads)
+    rows, dev = _lib.tensors().grad_table(grads)
+    with torch.cuda.device(dev):
+        out = torch.empty((), dtype=torch.float32, device=grads[0].device)
+        ws, nws = _workspace(len(grads), dev)
+        _lib.check(_lib.lib().kda_grad_norm(rows, len(grads), out.data_ptr(), ws.data_ptr(), nws,
+                                            torch.cuda.current_stream().cuda_stream), "kda_grad_norm")
+    return out
+
+
+@torch.no_grad()
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
+               exp_avgs: Sequence[Union[torch.Tensor, State8]], exp_avg_sqs: Sequence[Union[torch.Tensor, State8]], *,
+               step: Union[int, torch.Tensor], lr: Union[float, torch.Tensor], betas=(0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float = 1e-2, bias_correction: bool = True, max_grad_norm: Optional[float] = None,
+               emas: Optional[Sequence[torch.Tensor]] = None, ema_decay: Optional[float] = None, seed: int = 0,
+               norm: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """One AdamW step over lists of CUDA tensors, in place.
+
+    ``params`` and ``grads`` are float32, bfloat16 or float16, dense in memory and each pair laid
+    out alike.  The states are contiguous float32 tensors, or (codes, exponents) pairs
+    (``zeros_state8``) for 8 bits, in the parameter's order in memory.  ``step`` is this
+    step's number from 1, or an int64 CUDA scalar that the call advances; ``lr`` a number or a
+    float32 CUDA scalar.  A captured graph needs both as tensors: numbers would be frozen in it.
+    With ``max_grad_norm`` the gradients are scaled as they are read (``grads`` keep their values)
+    by their global norm, or by ``norm``, a float32 CUDA scalar, where that is given.  ``emas``
+    (float32) follow the parameters with ``ema_decay``.  Tensors must not overlap one another.
+    Returns the gradients' norm (float32 scalar) with ``max_grad_norm``, else None.
+    """
+    params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
+    bits = 8 if exp_avgs and isinstance(exp_avgs[0], (tuple, list)) else 32
+    _need((emas is None) == (ema_decay is None), "emas and ema_decay go together")
+    _need(ema_decay is None or 0.0 <= ema_decay <= 1.0, f"ema_decay must lie in [0, 1], got {ema_decay}")
+    _need(0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0, f"betas must lie in [0, 1), got {betas}")
+    _need(eps >= 0.0, f"eps must not be negative, got {eps}")
+    _need(bits == 32 or eps >= 1e-30, f"8-bit states need an eps of at least 1e-30, got {eps}")
+    _need(max_grad_norm is None or max_grad_norm > 0.0, f"max_grad_norm must be positive, got {max_grad_norm}")
+    _need(norm is None or max_grad_norm is not None, "norm is used with max_grad_norm only")
+    rows, dev = _lib.tensors().adamw_table(params, grads, exp_avgs, exp_avg_sqs, None if emas is None else list(emas),
+                                           bits)
+    step_t = step if isinstance(step, torch.Tensor) else None
+    lr_t = lr if isinstance(lr, torch.Tensor) else None
+    for n, t, dt in (("step", step_t, torch.int64), ("lr", lr_t, torch.float32), ("norm", norm, torch.float32)):
+        _need(t is None or (t.get_device() == dev and t.dtype == dt and t.numel() == 1),
+              f"{n} as a tensor must be one {dt} value on the parameters' device")
+    if step_t is None:
+        _need(step >= 1, f"step counts from 1, got {step}")
+    with torch.cuda.device(dev):
+        if (step_t is None or lr_t is None) and torch.cuda.is_current_stream_capturing():
+            raise ValueError("adamw_step: step and lr must be CUDA tensors while a graph is captured")
+        out = norm
+        ws, nws = None, 0
+        if max_grad_norm is not None or step_t is not None or lr_t is not None:
+            ws, nws = _workspace(len(params), dev)
+            if max_grad_norm is not None and norm is None:
+                out = torch.empty((), dtype=torch.float32, device=params[0].device)
+        args = _lib.KdaAdamW(0.0 if lr_t is not None else float(lr), betas[0], betas[1], eps, weight_decay,
+                             max_grad_norm or 0.0, ema_decay or 0.0, 0 if step_t is not None else step,
+                             seed & 0xFFFFFFFF, bits, bool(bias_correction), emas is not None, norm is not None, 0)
+        _lib.check(_lib.lib().kda_adamw_step(
+            ctypes.byref(args), rows, len(params), None if step_t is None else step_t.data_ptr(),
+            None if lr_t is None else lr_t.data_ptr(), None if out is None else out.data_ptr(),
+            None if ws is None else ws.data_ptr(), nws, torch.cuda.current_stream().cuda_stream), "kda_adamw_step")
+    return out
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) with every tensor of a group updated by one launch.
+
+    ``state_bits`` 32 or 8; ``max_grad_norm`` clips the global norm over all groups (the last
+    step's norm is ``self.grad_norm``); ``ema_decay`` keeps a float32 shadow of every parameter
+    (``ema_of``), started at the parameter's first step.  ``capturable`` keeps the step's number
+    and the learning rate on the device, so that ``step`` can be captured into a CUDA graph
+    after one eager step; the parameters of a group then share one step number and all need
+    gradients, and ``lr`` is the tensor ``group["lr"]`` (fill it to change it).
+    """
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
+                 bias_correction: bool = True, state_bits: int = 32, max_grad_norm: Optional[float] = None,
+                 ema_decay: Optional[float] = None, seed: int = 0, capturable: bool = False):
+        _need(state_bits in (8, 32), f"state_bits must be 8 or 32, got {state_bits}")
+        _need(max_grad_norm is None or max_grad_norm > 0.0, f"max_grad_norm must be positive, got {max_grad_norm}")
+        _need(ema_decay is None or 0.0 <= ema_decay <= 1.0, f"ema_decay must lie in [0, 1], got {ema_decay}")
+        self.state_bits, self.max_grad_norm, self.ema_decay = state_bits, max_grad_norm, ema_decay
+        self.seed, self.capturable = int(seed), bool(capturable)
+        self.grad_norm = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
+                                      bias_correction=bias_correction))
+
+    def __getstate__(self):
+        names = ("state_bits", "max_grad_norm", "ema_decay", "seed", "capturable", "grad_norm")
+        return {**super().__getstate__(), **{n: getattr(self, n) for n in names}}
+
+    def ema_of(self, p: torch.Tensor) -> torch.Tensor:
+        """The shadow average of a parameter, in its shape (float32)."""
+        return self.state[p]["ema"].as_strided(p.shape, p.stride())
+
+    def _init_state(self, p):
+        st = self.state[p]
+        if not self.capturable:
+            st["step"] = 0
+        for name in ("exp_avg", "exp_avg_sq"):
+            if self.state_bits == 8:
+                st[name], st[name + "_exp"] = zeros_state8(p)
+            else:
+                st[name] = torch.zeros(p.numel(), dtype=torch.float32, device=p.device)
+        if self.ema_decay is not None:  # in the parameter's order in memory, as every state
+            st["ema"] = p.detach().as_strided((p.numel(),), (1,)).float().clone()
+        return st
+
+    def _states(self, ps, name):
+        if self.state_bits == 8:
+            return [(self.state[p][name], self.state[p][name + "_exp"]) for p in ps]
+        return [self.state[p][name] for p in ps]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        calls = []  # (group, parameters, gradients in memory order, step number)
+        for group in self.param_groups:
+            live = [p for p in group["params"] if p.grad is not None]
+            if not live:
+                continue
+            capturing = live[0].is_cuda and torch.cuda.is_current_stream_capturing()
+            for p in live:
+                if not self.state[p]:
+                    if capturing:
+                        raise ValueError("AdamW: take one step before a step is captured into a graph")
+                    self._init_state(p)
+            grads = [p.grad for p in live]
+            for i in _lib.tensors().unlike(live, grads):
+                grads[i] = torch.empty_like(live[i]).copy_(grads[i])
+            if self.capturable:
+                _need(len(live) == len(group["params"]), "a capturable AdamW needs every parameter's gradient")
+                dev = live[0].device
+                for name, dt in (("step", torch.int64), ("lr", torch.float32)):
+                    t = group.get(name, 0)
+                    if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != dt:
+                        if capturing:
+                            raise ValueError("AdamW: take one step before a step is captured into a graph")
+                        group[name] = torch.as_tensor(t, dtype=dt, device=dev).clone()
+                calls.append((group, live, grads, group["step"]))
+            else:
+                by_step = {}
+                for p, g in zip(live, grads):
+                    at = by_step.setdefault(self.state[p]["step"] + 1, ([], []))
+                    at[0].append(p)
+                    at[1].append(g)
+                calls += [(group, ps, gs, n) for n, (ps, gs) in by_step.items()]
+        norm = None
+        if self.max_grad_norm is not None and len(calls) > 1:
+            norm = grad_norm([g for c in calls for g in c[2]])
+        for group, ps, gs, n in calls:
+            out = adamw_step(ps, gs, self._states(ps, "exp_avg"),
+                             self._states(ps, "exp_avg_sq"), step=n,
+                             lr=group["lr"] if self.capturable else float(group["lr"]), betas=group["betas"],
+                             eps=group["eps"], weight_decay=group["weight_decay"],
+                             bias_correction=group["bias_correction"], max_grad_norm=self.max_grad_norm,
+                             emas=None if self.ema_decay is None else [self.state[p]["ema"] for p in ps],
+                             ema_decay=self.ema_decay, seed=self.seed, norm=norm)
+            self.grad_norm = out
+            if not self.capturable:
+                for p in ps:
+                    self.state[p]["step"] = n
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """As torch's, but the states keep their own dtypes (torch casts them to the parameters')."""
+        super().load_state_dict(state_dict)
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
+            if i in state_dict["state"]:
+                self.state[p] = {k: v.to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
+                                 for k, v in state_dict["state"][i].items()}

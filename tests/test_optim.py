@@ -1,0 +1,102 @@
+"""CPU: the optimizer's argument checks and its 8-bit state format (restated)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from mlx_vit_b200 import _lib, optim
+from optim_testutil import decode, encode, mix
+
+
+def test_cpu_tensors_are_refused():
+    p, g, m, v = (torch.zeros(4) for _ in range(4))
+    with pytest.raises(ValueError, match="no CPU path"):
+        optim.adamw_step([p], [g], [m], [v], step=1, lr=1e-3)
+    with pytest.raises(ValueError, match="no CPU path"):
+        optim.grad_norm([g])
+    with pytest.raises(ValueError, match="CUDA"):
+        optim.decode_state8(torch.zeros(4, dtype=torch.uint8), torch.zeros(1, dtype=torch.uint8), True)
+    w = torch.nn.Parameter(torch.zeros(4))
+    w.grad = torch.zeros(4)
+    with pytest.raises(ValueError, match="no CPU path"):
+        optim.AdamW([w]).step()
+
+
+@pytest.mark.parametrize("kw", [dict(state_bits=4), dict(max_grad_norm=0.0), dict(ema_decay=1.5)])
+def test_bad_options_are_refused(kw):
+    with pytest.raises(ValueError):
+        optim.AdamW([torch.nn.Parameter(torch.zeros(4))], **kw)
+
+
+@pytest.mark.parametrize("kw", [dict(betas=(1.0, 0.9)), dict(eps=-1.0), dict(max_grad_norm=-1.0), dict(ema_decay=0.5)])
+def test_bad_step_arguments_are_refused(kw):
+    p, g, m, v = (torch.zeros(4) for _ in range(4))
+    with pytest.raises(ValueError):
+        optim.adamw_step([p], [g], [m], [v], step=1, lr=1e-3, **kw)
+
+
+def call(rows=(), count=None, step_dev=None, ws=None, nws=0, norm=None, **kw):
+    a = dict(lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.0, max_grad_norm=0.0, ema_decay=0.0, step=1,
+             seed=0, state_bits=32, bias_correction=1, use_ema=0, norm_given=0, reserved=0)
+    a.update(kw)
+    table = (ctypes.c_int64 * max(1, 9 * len(rows)))(*[x for r in rows for x in r])
+    return _lib.STATUS[_lib.lib().kda_adamw_step(ctypes.byref(_lib.KdaAdamW(**a)), table,
+                                                 len(rows) if count is None else count, step_dev, None, norm, ws, nws,
+                                                 None)]
+
+
+def test_c_entry_refuses_bad_arguments_before_any_launch():
+    a = 1 << 20
+    good = (a, a, a, a, 0, 0, 0, 16, _lib.KDA_F32)
+
+    def row(**kw):
+        names = ("p", "g", "m", "v", "me", "ve", "ema", "n", "dtype")
+        return tuple(kw.get(n, x) for n, x in zip(names, good))
+
+    assert _lib.STATUS[_lib.lib().kda_adamw_step(None, None, 0, None, None, None, None, 0, None)] == "KDA_ERR_INVALID_ARG"
+    assert call([row(p=0)]) == "KDA_ERR_INVALID_ARG"
+    assert call([row(g=0)]) == "KDA_ERR_INVALID_ARG"
+    assert call([row(n=-1)]) == "KDA_ERR_INVALID_ARG"
+    assert call([row(dtype=9)]) == "KDA_ERR_DTYPE"
+    assert call([row(m=a + 2)]) == "KDA_ERR_MISALIGNED"
+    assert call([row(g=a + 1)]) == "KDA_ERR_MISALIGNED"
+    assert call([row()], state_bits=16) == "KDA_ERR_UNSUPPORTED"
+    assert call([row()], state_bits=8) == "KDA_ERR_INVALID_ARG"  # no exponent bytes
+    assert call([row()], use_ema=1) == "KDA_ERR_INVALID_ARG"
+    assert call([row()], step=0) == "KDA_ERR_INVALID_ARG"
+    assert call([row()], beta2=1.0) == "KDA_ERR_INVALID_ARG"
+    assert call([row()], eps=float("nan")) == "KDA_ERR_INVALID_ARG"
+    assert call([row()], lr=float("inf")) == "KDA_ERR_INVALID_ARG"
+    assert call([row()], count=-1) == "KDA_ERR_INVALID_ARG"
+    assert call([row()], max_grad_norm=1.0, norm_given=1) == "KDA_ERR_INVALID_ARG"
+    assert call([]) == "KDA_OK"
+    L = _lib.lib()
+    assert _lib.STATUS[L.kda_decode_state8(4, 1, None, None, None, None)] == "KDA_ERR_INVALID_ARG"
+    assert L.kda_decode_state8(0, 1, None, None, None, None) == 0
+    assert L.kda_adamw_workspace_bytes(0) == 0 and L.kda_adamw_workspace_bytes(1) > 256
+
+
+@pytest.mark.parametrize("low,signed", [(15, True), (31, False)])
+def test_format_round_trip_and_bracket(low, signed):
+    """Every value a code stands for is kept by any random bits, and a rounded value is one of its
+    two neighbours: at most one eighth of its binade away."""
+    rng = np.random.default_rng(low)
+    code = np.arange(256, dtype=np.uint8)
+    code = code[(code & (127 if signed else 255)) <= 8 * low - 1]
+    code = np.concatenate([code, np.zeros(256 - code.size, np.uint8)])
+    exp = np.array([130], np.uint8)
+    x = decode(code, exp, low, signed)
+    c2, e2 = encode(x.astype(np.float32), rng.integers(0, 65536, 256), low, signed)
+    assert e2[0] == 130 and np.array_equal(decode(c2, e2, low, signed), x)
+    y = (rng.standard_normal(4096) * np.exp2(rng.uniform(-12, 0, 4096))).astype(np.float32)
+    y = y if signed else np.abs(y)
+    c, e = encode(y, rng.integers(0, 65536, 4096), low, signed)
+    d = decode(c, e, low, signed)
+    assert (np.abs(d - y) <= np.maximum(np.abs(y) / 8, 1.125 * np.exp2(np.repeat(e, 256) - 127.0 - low))).all()
+
+
+def test_hash_spreads():
+    h = mix(np.arange(1 << 16, dtype=np.uint64))
+    assert len(set(h.tolist())) == 1 << 16
+    assert abs((h & np.uint64(0xFFFF)).mean() / 65535 - 0.5) < 0.01
