@@ -237,6 +237,36 @@ KDA_API int kda_bwd_noalloc(const KdaDesc *desc, const void *q, const void *k, c
                             void *dq, void *dk, void *dv, float *dg, void *dbeta, float *dstate0,
                             void *stream);
 
+/* ---- linear products with a fused epilogue (16-bit operands, float32 accumulation) ----
+ * dtype is KDA_BF16 or KDA_F16 for every matrix.  Matrices are row-major with ld* elements from row
+ * to row; x, w, dz, z (where the call writes it) need 16-byte aligned bases and row pitches
+ * (KDA_ERR_MISALIGNED), the others their element's alignment only (aligned ones are faster).
+ * Sizes up to 2^30 each.
+ *   kda_linear_fwd:    y [M][N] = act(x [M][K] w [N][K]^T + bias [N]) + residual [M][N];
+ *                      z [M][N] (may be NULL) receives x w^T + bias, rounded, for the backward
+ *   kda_act_grad:      dz = dy act'(z) over [rows][cols]; with KDA_ACT_NONE a copy (z may be NULL),
+ *                      which also brings a matrix into the alignment the others need
+ *   kda_linear_dgrad:  dx [M][K] = dz [M][N] w [N][K]; with an activation times act'(z [M][K]), the
+ *                      saved input of the activation that x came from
+ *   kda_linear_wgrad:  dw [N][K] = dz^T x, db [N] = column sums of dz (db may be NULL, then no
+ *                      workspace is needed)
+ * bias, residual and db may be NULL.  Counterpart: the nn.Linear layers of the reference's
+ * blocks and their MLP (HybridBlock, nope_gdn_mlx.py:4009-4090). */
+enum kda_act { KDA_ACT_NONE = 0, KDA_ACT_RELU = 1, KDA_ACT_SILU = 2, KDA_ACT_GELU = 3, KDA_ACT_GELU_TANH = 4 };
+
+KDA_API int kda_linear_fwd(int dtype, int act, int64_t M, int64_t N, int64_t K, const void *x, int64_t ldx,
+                           const void *w, int64_t ldw, const void *bias, const void *residual, int64_t ldr,
+                           void *y, int64_t ldy, void *z, int64_t ldz, void *stream);
+KDA_API int kda_linear_dgrad(int dtype, int act, int64_t M, int64_t N, int64_t K, const void *dz, int64_t ldd,
+                             const void *w, int64_t ldw, const void *z, int64_t ldz, void *dx, int64_t ldx,
+                             void *stream);
+KDA_API size_t kda_linear_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K);
+KDA_API int kda_linear_wgrad(int dtype, int64_t M, int64_t N, int64_t K, const void *dz, int64_t ldd,
+                             const void *x, int64_t ldx, void *dw, int64_t ldw, void *db, void *ws,
+                             size_t ws_bytes, void *stream);
+KDA_API int kda_act_grad(int dtype, int act, int64_t rows, int64_t cols, const void *dy, int64_t ldy,
+                         const void *z, int64_t ldz, void *dz, int64_t ldd, void *stream);
+
 /* ---- AdamW over many tensors at once ----
  * One tensor of the step.  p (updated) and g have dtype `dtype`, numel contiguous elements each.
  * The states m, v: float32 [numel] (state_bits 32), or 8-bit codes [numel] with one exponent byte

@@ -25,6 +25,7 @@ int recurrent_fwd(const Params &p, int dq, int db, cudaStream_t st);
 size_t tc128_workspace_bytes(const KdaDesc *d);
 int tc128_fwd(const Params &p, int dtype_beta, cudaStream_t st);
 int tc128_fwd_device_status(bool reset);
+int linear_device_status(bool reset);
 static std::atomic<uint64_t> g_launches{0};
 void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 }  // namespace kda
@@ -70,7 +71,8 @@ int kda_device_status(int reset) {
   const int f = kda::tc_fwd_device_status(reset != 0);
   const int b = kda::tc_bwd_device_status(reset != 0);
   const int f128 = kda::tc128_fwd_device_status(reset != 0);
-  return f ? f : b ? b : f128;
+  const int lin = kda::linear_device_status(reset != 0);
+  return f ? f : b ? b : f128 ? f128 : lin;
 }
 
 uint64_t kda_launch_counter(void) { return kda::g_launches.load(std::memory_order_relaxed); }

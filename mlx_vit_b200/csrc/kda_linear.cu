@@ -1,0 +1,671 @@
+// Linear products with a fused epilogue, on the 5th-generation tensor cores (16-bit operands,
+// float32 accumulation in tensor memory):
+//
+//   forward   y  = act(x W^T + bias) + residual, and z = x W^T + bias kept for the backward
+//   dgrad     dx = dz W,  or  (dz W) * act'(z) where an activation lies below
+//   wgrad     dW = dz^T x,  db = the column sums of dz
+//
+// One kernel: C[m][n] = sum_k A[m][k] B[n][k] over tiles of 128 CG x BN, where each operand lies in
+// memory k-contiguous ("K-major") or m- / n-contiguous ("MN-major": the transposes are read in
+// place).  Each persistent CTA (or pair of CTAs, CG = 2, whose tensor cores work on one tile and read
+// half of B each) walks its tiles with one thread copying operand blocks of 64 k by TMA into a
+// ring of stages, one thread issuing the products, and eight warps taking finished accumulators
+// from tensor memory through the epilogue while the next tile's products run (two accumulators).
+// Rows, columns and k past the end are TMA's zero fill and clipped stores.
+#include <initializer_list>
+
+#include "kda_act.cuh"
+#include "kda_common.cuh"
+#include "kda_mma.cuh"
+#include "kda_tc05.cuh"
+#include "kda_tma.cuh"
+
+namespace kda {
+namespace linear {
+
+// set to a KDA_ERR_* code by a bounded wait that gave up (read by kda_device_status)
+static __device__ int g_linear_status;
+
+constexpr int kThreads = 384;     // producer, issuer, allocator, idle, 8 epilogue warps
+constexpr int kEpiWarp = 4, kEpiWarps = 8;
+constexpr int kBlockK = 64;       // k per stage: 128 bytes, the swizzle's width
+constexpr int kStageA = 128 * 128;
+constexpr int kStaging = kEpiWarps * 2 * 4096;  // two 32 x 64 tiles a warp
+constexpr int kOnesN = 32;        // columns of the product with ones that sums dz's columns
+constexpr int kSmemMax = 232448;
+constexpr int kPolls = 1 << 20;   // bound of a wait: some tens of milliseconds and more, against microseconds of work
+
+enum { kInNone = 0, kInAdd = 1, kInActGrad = 2 };
+
+struct alignas(64) Args {
+  CUtensorMap a, b, out, in, z;
+  int64_t ldo, ldi;
+  const void *bias, *in_ptr;
+  void *out_ptr;
+  float *sums;          // ONES: [tiles_n][m] partial column sums of A
+  int m, n, k, tiles_m, tiles_n;
+  uint32_t idesc, idesc_ones;
+  int act, in_kind, out_tma, in_tma, save_z;
+};
+
+template <int CG, int BN, bool ONES>
+struct Shape {
+  static constexpr int kStageB = BN / CG * 128;
+  static constexpr int kStage = kStageA + kStageB;
+  static constexpr int kOnes = ONES ? kOnesN / CG * 128 : 0;
+  static constexpr int kFixed = kStaging + kOnes + kEpiWarps * 256 + 512;
+  static constexpr int kStages = (kSmemMax - kFixed) / kStage < 8 ? (kSmemMax - kFixed) / kStage : 8;
+  static constexpr int kAcc = BN + (ONES ? kOnesN : 0);   // tensor-memory columns of one accumulator
+  static constexpr int kBufs = 2 * kAcc <= 512 ? 2 : 1;
+  static constexpr int kCols = kBufs * kAcc <= 128 ? 128 : kBufs * kAcc <= 256 ? 256 : 512;
+  static constexpr int kSmem = kStages * kStage + kFixed;
+};
+
+// ---- what pairs of CTAs need ----
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t saddr, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(saddr), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t addr) {  // addr: a shared::cluster address
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" :: "r"(addr) : "memory");
+}
+__device__ __forceinline__ bool wait_cluster(uint32_t mbar, uint32_t parity) {  // bounded, as mbar_wait
+  for (int i = 0; i < kPolls; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok) : "r"(mbar), "r"(parity) : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+
+template <int CG>
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t mbar) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n"
+        :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(mbar) : "memory");
+  else  // the barrier is the pair's first CTA's
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n"
+        :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(mbar) : "memory");
+}
+__device__ __forceinline__ void store_box(const CUtensorMap *map, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];\n"
+               :: "l"(map), "r"(src), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;\n" :: "n"(N) : "memory"); }
+
+template <int CG>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CG == 1) tc_mma(d, a, b, idesc, accumulate);
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+        :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t mbar) {  // to the barrier at this offset in every CTA of the pair
+  if constexpr (CG == 1) tc_commit(mbar);
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
+        :: "r"(mbar), "h"((uint16_t)3) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void alloc(uint32_t dst, uint32_t cols) {
+  if constexpr (CG == 1) {
+    tmem_alloc(dst, cols);
+    tmem_relinquish();
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" :: "r"(dst), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void dealloc(uint32_t taddr, uint32_t cols) {
+  if constexpr (CG == 1) tmem_dealloc(taddr, cols);
+  else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" :: "r"(taddr), "r"(cols) : "memory");
+}
+
+// byte offset of 16-byte chunk c of row r in a tile of 128-byte rows with the 128-byte swizzle
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+
+template <typename T> struct Pair;
+template <> struct Pair<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const type v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+  }
+};
+template <> struct Pair<__half> {
+  using type = __half2;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const type v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<const type *>(&u)); }
+};
+
+// A 32 x 64 tile between global memory and a warp's staging rows where no TMA map can describe the
+// matrix (a row pitch or a base that 16 bytes do not divide): coalesced 2-byte accesses.
+template <typename T>
+__device__ __forceinline__ void tile_in(uint8_t *st, const T *p, int64_t ld, int rows, int cols, int lane) {
+  for (int r = 0; r < 32; ++r) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = lane + 32 * h;
+      const T v = r < rows && c < cols ? p[r * ld + c] : T(0.f);
+      *reinterpret_cast<T *>(st + chunk_at(r, c >> 3) + (c & 7) * 2) = v;
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void tile_out(const uint8_t *st, T *p, int64_t ld, int rows, int cols, int lane) {
+  for (int r = 0; r < rows; ++r) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = lane + 32 * h;
+      if (c < cols) p[r * ld + c] = *reinterpret_cast<const T *>(st + chunk_at(r, c >> 3) + (c & 7) * 2);
+    }
+  }
+}
+
+template <typename T, int CG, int BN, bool A_MN, bool B_MN, bool ONES>
+__global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ Args g) {
+  using S = Shape<CG, BN, ONES>;
+  using P = Pair<T>;
+  extern __shared__ __align__(1024) uint8_t sm[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0;
+  const uint32_t base = smem_u32(sm);
+  if (base & 1023) {  // the swizzled tiles need a 1024-byte aligned base (every CTA has the same)
+    if (tid == 0) atomicExch(&g_linear_status, KDA_ERR_MISALIGNED);
+    return;
+  }
+  uint8_t *staging = sm + S::kStages * S::kStage, *ones = staging + kStaging;
+  float *bias_sm = reinterpret_cast<float *>(ones + S::kOnes);
+  // barriers: full[stages], empty[stages], acc_full[2], acc_empty[2], in[8 warps]; then tensor memory's address
+  const uint32_t bars = smem_u32(bias_sm) + kEpiWarps * 256;
+  const uint32_t full = bars, empty = full + 8 * S::kStages, acc_full = empty + 8 * S::kStages,
+                 acc_empty = acc_full + 16, in_bar = acc_empty + 16, tmem_at = in_bar + 8 * kEpiWarps;
+  const int kblocks = (g.k + kBlockK - 1) / kBlockK;
+  const int tiles = g.tiles_m * g.tiles_n, first = blockIdx.x / CG, step = gridDim.x / CG;
+
+  if (tid == 0) {
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(full + 8 * s, 1);
+      mbar_init(empty + 8 * s, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full + 8 * i, 1);
+      mbar_init(acc_empty + 8 * i, kEpiWarps * CG);
+    }
+    for (int w = 0; w < kEpiWarps; ++w) mbar_init(in_bar + 8 * w, 1);
+    mbar_fence_init();
+  }
+  if (ONES)
+    for (int i = tid; i < S::kOnes / 4; i += kThreads) reinterpret_cast<uint32_t *>(ones)[i] = P::pack(1.f, 1.f);
+  if (warp == 2) alloc<CG>(tmem_at, S::kCols);
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(sm + (tmem_at - base));
+  bool ok = true;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---- operand copies; both CTAs' bytes of a stage arrive on the first CTA's barrier ----
+      const uint32_t full_lead = CG == 2 ? map_rank(full, 0) : full;
+      uint32_t it = 0;
+      for (int t = first; ok && t < tiles; t += step) {
+        const int m0 = (t / g.tiles_n) * 128 * CG + (int)rank * 128;
+        const int n0 = (t % g.tiles_n) * BN + (int)rank * (BN / CG);
+        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+          const uint32_t s = it % S::kStages, ph = (it / S::kStages) & 1;
+          if (!(ok = wait_cluster(empty + 8 * s, ph ^ 1))) break;
+          if (rank == 0) mbar_expect_tx(full + 8 * s, S::kStage * CG);
+          const uint32_t at = base + s * S::kStage, bt = at + kStageA, fb = full_lead + 8 * s;
+          if (A_MN) {
+            load_box<CG>(at, &g.a, m0, kb * kBlockK, fb);
+            load_box<CG>(at + 8192, &g.a, m0 + 64, kb * kBlockK, fb);
+          } else {
+            load_box<CG>(at, &g.a, kb * kBlockK, m0, fb);
+          }
+          if (B_MN) {
+#pragma unroll
+            for (int j = 0; j < BN / CG / 64; ++j)
+              load_box<CG>(bt + 8192 * j, &g.b, n0 + 64 * j, kb * kBlockK, fb);
+          } else {
+            load_box<CG>(bt, &g.b, kb * kBlockK, n0, fb);
+          }
+        }
+      }
+      if (!ok && rank == 0)  // gave up: let the copies in flight land before the CTA ends
+        for (uint32_t i = it > S::kStages ? it - S::kStages : 0; i < it; ++i)
+          mbar_wait(full + 8 * (i % S::kStages), (i / S::kStages) & 1, 1 << 16);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      // ---- products ----
+      uint32_t it = 0, n = 0;
+      for (int t = first; ok && t < tiles; t += step, ++n) {
+        const uint32_t buf = n % S::kBufs, use = n / S::kBufs;
+        const uint32_t d = tmem + buf * S::kAcc;
+        if (!(ok = wait_cluster(acc_empty + 8 * buf, (use & 1) ^ 1))) break;
+        tc_fence_after();
+        const int tn = t % g.tiles_n;
+        bool summed = false;
+        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+          const uint32_t s = it % S::kStages, ph = (it / S::kStages) & 1;
+          if (!(ok = wait_cluster(full + 8 * s, ph))) break;
+          tc_fence_after();
+          const uint32_t at = base + s * S::kStage, bt = at + kStageA;
+#pragma unroll
+          for (int k = 0; k < kBlockK / 16; ++k)
+            mma<CG>(d, A_MN ? desc_mn(at, k) : desc_k(at, k), B_MN ? desc_mn(bt, k) : desc_k(bt, k), g.idesc,
+                    kb > 0 || k > 0);
+          if (ONES && kb % g.tiles_n == tn) {  // the column sums' share of this column tile
+#pragma unroll
+            for (int k = 0; k < kBlockK / 16; ++k)
+              mma<CG>(d + BN, A_MN ? desc_mn(at, k) : desc_k(at, k), desc_k(smem_u32(ones), 0), g.idesc_ones,
+                      summed || k > 0);
+            summed = true;
+          }
+          commit<CG>(empty + 8 * s);
+        }
+        if (ok) commit<CG>(acc_full + 8 * buf);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= kEpiWarp) {
+    // ---- epilogue: warp (q, half) takes rows 32 q .. 32 q + 31 of every second 64-column chunk ----
+    const int e = warp - kEpiWarp, q = warp & 3, half = e >> 2;
+    uint8_t *st = staging + e * 8192;
+    const uint32_t st_at = smem_u32(st), my_in = in_bar + 8 * e;
+    float *bs = bias_sm + e * 64;
+    const uint32_t empty_lead = CG == 2 ? map_rank(acc_empty, 0) : acc_empty;
+    const T *bias = static_cast<const T *>(g.bias);
+    uint32_t n = 0, in_phase = 0, flip = 0;
+    for (int t = first; ok && t < tiles; t += step, ++n) {
+      const uint32_t buf = n % S::kBufs, use = n / S::kBufs;
+      const int tm = t / g.tiles_n, tn = t % g.tiles_n;
+      const int row0 = tm * 128 * CG + (int)rank * 128 + 32 * q;
+      ok = wait_cluster(acc_full + 8 * buf, use & 1);
+      if (!__all_sync(0xFFFFFFFFu, ok)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t acc = tmem + buf * S::kAcc + ((uint32_t)(32 * q) << 16);
+      if (ONES && half == 0) {
+        uint32_t v;
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n" : "=r"(v) : "r"(acc + BN));
+        tmem_wait_ld();
+        if (row0 + lane < g.m) g.sums[(int64_t)tn * g.m + row0 + lane] = tn < kblocks ? __uint_as_float(v) : 0.f;
+      }
+      for (int c = half; c < BN / 64; c += 2) {
+        const int col0 = tn * BN + 64 * c;
+        if (row0 >= g.m || col0 >= g.n) break;
+        const int rows = min(32, g.m - row0), cols = min(64, g.n - col0);
+        // this chunk's staging tile: with a z to save the second one is z's
+        const int b = g.save_z ? 0 : (flip++ & 1);
+        uint8_t *so = st + b * 4096;
+        const uint32_t so_at = st_at + b * 4096;
+        if (lane == 0) {  // its last store has been read (one newer one may still be)
+          if (g.save_z || !g.out_tma) store_wait_read<0>();
+          else store_wait_read<1>();
+        }
+        __syncwarp();
+        if (g.in_kind) {
+          if (g.in_tma) {
+            if (lane == 0) {
+              fence_proxy_async_smem();
+              mbar_expect_tx(my_in, 4096);
+              load_box<1>(so_at, &g.in, col0, row0, my_in);
+            }
+            ok = mbar_wait(my_in, in_phase, kPolls);
+            in_phase ^= 1;
+            if (!__all_sync(0xFFFFFFFFu, ok)) {
+              ok = false;
+              break;
+            }
+          } else {
+            tile_in<T>(so, static_cast<const T *>(g.in_ptr) + row0 * g.ldi + col0, g.ldi, rows, cols, lane);
+            __syncwarp();
+          }
+        }
+        if (bias) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int j = lane + 32 * h;
+            bs[j] = j < cols ? to_f<T>(bias[col0 + j]) : 0.f;
+          }
+          __syncwarp();
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t r[32];
+          tmem_ld32(acc + 64 * c + 32 * h, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {  // 8 columns: one 16-byte chunk of the row
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[8 * u + j]);
+            if (bias) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] += bs[32 * h + 8 * u + j];
+            }
+            const uint32_t at = chunk_at(lane, 4 * h + u);
+            uint4 *slot = reinterpret_cast<uint4 *>(so + at);
+            if (g.save_z)
+              *reinterpret_cast<uint4 *>(st + 4096 + at) =
+                  make_uint4(P::pack(v[0], v[1]), P::pack(v[2], v[3]), P::pack(v[4], v[5]), P::pack(v[6], v[7]));
+            if (g.in_kind == kInActGrad) {
+              const uint4 zi = *slot;
+              const uint32_t w[4] = {zi.x, zi.y, zi.z, zi.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float2 z = P::unpack(w[j]);
+                v[2 * j] *= activate_grad(g.act, z.x);
+                v[2 * j + 1] *= activate_grad(g.act, z.y);
+              }
+            } else {
+              if (g.act != KDA_ACT_NONE) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = activate(g.act, v[j]);
+              }
+              if (g.in_kind == kInAdd) {
+                const uint4 ri = *slot;
+                const uint32_t w[4] = {ri.x, ri.y, ri.z, ri.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const float2 x = P::unpack(w[j]);
+                  v[2 * j] += x.x;
+                  v[2 * j + 1] += x.y;
+                }
+              }
+            }
+            *slot = make_uint4(P::pack(v[0], v[1]), P::pack(v[2], v[3]), P::pack(v[4], v[5]), P::pack(v[6], v[7]));
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (!g.out_tma)
+          tile_out<T>(so, static_cast<T *>(g.out_ptr) + row0 * g.ldo + col0, g.ldo, rows, cols, lane);
+        if (lane == 0) {
+          if (g.out_tma) store_box(&g.out, so_at, col0, row0);
+          if (g.save_z) store_box(&g.z, st_at + 4096, col0, row0);
+          store_commit();
+        }
+        __syncwarp();
+      }
+      if (!ok) break;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (CG == 2) arrive_cluster(empty_lead + 8 * buf);
+        else mbar_arrive(acc_empty + 8 * buf);
+      }
+    }
+    if (lane == 0) store_wait_read<0>();
+    __syncwarp();
+  }
+  if (!ok) atomicExch(&g_linear_status, KDA_ERR_TIMEOUT);
+  tc_fence_before();
+  __syncthreads();
+  if (CG == 2) cluster_sync();  // neither CTA ends while the other's products or copies may touch it
+  tc_fence_after();
+  if (warp == 2) dealloc<CG>(tmem, S::kCols);
+}
+
+// db[j] = sum over the partials, in their order
+template <typename T>
+__global__ void __launch_bounds__(256) sums_kernel(const float *part, int parts, int m, T *db) {
+  const int j = blockIdx.x * 256 + threadIdx.x;
+  if (j >= m) return;
+  float s = 0.f;
+  for (int i = 0; i < parts; ++i) s += part[(int64_t)i * m + j];
+  db[j] = from_f<T>(s);
+}
+
+// dz = dy act'(z) over a [rows][cols] matrix (z null: a copy), any strides and alignments
+template <typename T>
+__global__ void __launch_bounds__(256) act_grad_kernel(int act, int64_t rows, int cols, const T *dy, int64_t ldy, const T *z,
+                                                       int64_t ldz, T *dz, int64_t ldd) {
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    for (int c = blockIdx.x * 256 + threadIdx.x; c < cols; c += gridDim.x * 256) {
+      float v = to_f<T>(dy[r * ldy + c]);
+      if (z) v *= activate_grad(act, to_f<T>(z[r * ldz + c]));
+      dz[r * ldd + c] = from_f<T>(v);
+    }
+  }
+}
+
+// ---- host side ----
+static bool tma_able(const void *p, int64_t ld) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0; }
+
+static int device_sms() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  static int known[64];  // written once with the same value by whoever comes first
+  if (dev < 64 && known[dev]) return known[dev];
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  if (dev < 64) known[dev] = n;
+  return n;
+}
+
+template <typename T, int CG, int BN, bool A_MN, bool B_MN, bool ONES>
+static int launch(Args &g, int sms, cudaStream_t st) {
+  using S = Shape<CG, BN, ONES>;
+  auto kernel = gemm_kernel<T, CG, BN, A_MN, B_MN, ONES>;
+  g.tiles_m = (g.m + 128 * CG - 1) / (128 * CG);
+  g.tiles_n = (g.n + BN - 1) / BN;
+  constexpr uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+  auto idesc = [&](int n, bool b_mn) {
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)A_MN << 15) | ((uint32_t)b_mn << 16) |
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
+  };
+  g.idesc = idesc(BN, B_MN);
+  g.idesc_ones = idesc(kOnesN, false);
+  const cudaError_t a = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+  if (a != cudaSuccess) return KDA_ERR_CUDA;
+  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n, units = sms / CG;
+  if (tiles > (1ll << 30)) return KDA_ERR_UNSUPPORTED;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((tiles < units ? tiles : units) * CG));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = CG > 1 ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kernel, g) != cudaSuccess) return KDA_ERR_CUDA;
+  count_launch();
+  return KDA_OK;
+}
+
+// The tile shape.  A pair of CTAs on 256 x 256 reads the least shared memory per product and is
+// taken where its tiles fill the GPU; smaller products take smaller tiles so that more SMs work.
+template <int BN, int CG>
+static int64_t tiles_of(int64_t m, int64_t n) {
+  return ((m + 128 * CG - 1) / (128 * CG)) * ((n + BN - 1) / BN);
+}
+template <typename T, bool A_MN, bool B_MN, bool ONES>
+static int dispatch(Args &g, const void *a, int64_t lda, const void *b, int64_t ldb, cudaStream_t st) {
+  const int sms = device_sms();
+  if (!sms) return KDA_ERR_CUDA;
+  int cg = 1, bn = 64;
+  if (tiles_of<256, 2>(g.m, g.n) * 4 >= sms / 2 * 3) cg = 2, bn = 256;
+  else if (tiles_of<128, 1>(g.m, g.n) * 4 >= sms * 3) bn = 128;
+  int s;
+  if ((s = A_MN ? tma_map_rows16(&g.a, a, g.k, g.m, lda, 64) : tma_map_rows16(&g.a, a, g.m, g.k, lda, 128))) return s;
+  if ((s = B_MN ? tma_map_rows16(&g.b, b, g.k, g.n, ldb, 64) : tma_map_rows16(&g.b, b, g.n, g.k, ldb, bn / cg))) return s;
+  if (cg == 2) return launch<T, 2, 256, A_MN, B_MN, ONES>(g, sms, st);
+  if (bn == 128) return launch<T, 1, 128, A_MN, B_MN, ONES>(g, sms, st);
+  return launch<T, 1, 64, A_MN, B_MN, ONES>(g, sms, st);
+}
+
+static int set_out(Args &g, void *p, int64_t ld) {
+  g.out_ptr = p;
+  g.ldo = ld;
+  g.out_tma = tma_able(p, ld);
+  return g.out_tma ? tma_map_rows16(&g.out, p, g.m, g.n, ld, 32) : KDA_OK;
+}
+static int set_in(Args &g, int kind, const void *p, int64_t ld) {
+  g.in_kind = kind;
+  g.in_ptr = p;
+  g.ldi = ld;
+  g.in_tma = tma_able(p, ld);
+  return g.in_tma ? tma_map_rows16(&g.in, p, g.m, g.n, ld, 32) : KDA_OK;
+}
+
+static int check(int dtype, int act, int64_t m, int64_t n, int64_t k) {
+  if (dtype != KDA_BF16 && dtype != KDA_F16) return KDA_ERR_DTYPE;
+  if (act < KDA_ACT_NONE || act > KDA_ACT_GELU_TANH) return KDA_ERR_INVALID_ARG;
+  if (m <= 0 || n <= 0 || k <= 0) return KDA_ERR_INVALID_ARG;
+  if (m > (1ll << 30) || n > (1ll << 30) || k > (1ll << 30)) return KDA_ERR_UNSUPPORTED;
+  return KDA_OK;
+}
+static bool ld_ok(int64_t ld, int64_t cols) { return ld >= cols && ld <= (1ll << 38); }
+static bool even(std::initializer_list<const void *> ps) {
+  for (const void *p : ps)
+    if ((uintptr_t)p % 2) return false;
+  return true;
+}
+
+int device_status(bool reset) {
+  int v = 0;
+  const int zero = 0;
+  if (cudaDeviceSynchronize() != cudaSuccess) return KDA_ERR_CUDA;
+  if (cudaMemcpyFromSymbol(&v, g_linear_status, sizeof(v)) != cudaSuccess) return KDA_ERR_CUDA;
+  if (reset && v && cudaMemcpyToSymbol(g_linear_status, &zero, sizeof(zero)) != cudaSuccess) return KDA_ERR_CUDA;
+  return v;
+}
+
+}  // namespace linear
+int linear_device_status(bool reset) { return linear::device_status(reset); }
+}  // namespace kda
+
+using namespace kda::linear;
+
+extern "C" {
+
+int kda_linear_fwd(int dtype, int act, int64_t M, int64_t N, int64_t K, const void *x, int64_t ldx, const void *w,
+                   int64_t ldw, const void *bias, const void *residual, int64_t ldr, void *y, int64_t ldy, void *z,
+                   int64_t ldz, void *stream) {
+  int s = check(dtype, act, M, N, K);
+  if (s) return s;
+  if (!x || !w || !y || !ld_ok(ldx, K) || !ld_ok(ldw, K) || !ld_ok(ldy, N) || (residual && !ld_ok(ldr, N)) ||
+      (z && !ld_ok(ldz, N)))
+    return KDA_ERR_INVALID_ARG;
+  if (!tma_able(x, ldx) || !tma_able(w, ldw) || (z && !tma_able(z, ldz)) || !even({bias, residual, y}))
+    return KDA_ERR_MISALIGNED;
+  Args g = {};
+  g.m = (int)M; g.n = (int)N; g.k = (int)K; g.act = act; g.bias = bias;
+  if ((s = set_out(g, y, ldy))) return s;
+  if (residual && (s = set_in(g, kInAdd, residual, ldr))) return s;
+  if (z) {
+    g.save_z = 1;
+    if ((s = kda::tma_map_rows16(&g.z, z, M, N, ldz, 32))) return s;
+  }
+  cudaStream_t st = (cudaStream_t)stream;
+  return dtype == KDA_BF16 ? dispatch<__nv_bfloat16, false, false, false>(g, x, ldx, w, ldw, st)
+                           : dispatch<__half, false, false, false>(g, x, ldx, w, ldw, st);
+}
+
+int kda_linear_dgrad(int dtype, int act, int64_t M, int64_t N, int64_t K, const void *dz, int64_t ldd, const void *w,
+                     int64_t ldw, const void *z, int64_t ldz, void *dx, int64_t ldx, void *stream) {
+  int s = check(dtype, act, M, N, K);
+  if (s) return s;
+  if (!dz || !w || !dx || !ld_ok(ldd, N) || !ld_ok(ldw, K) || !ld_ok(ldx, K) || (z && !ld_ok(ldz, K)) ||
+      (act != KDA_ACT_NONE && !z))
+    return KDA_ERR_INVALID_ARG;
+  if (!tma_able(dz, ldd) || !tma_able(w, ldw) || !even({z, dx})) return KDA_ERR_MISALIGNED;
+  Args g = {};
+  g.m = (int)M; g.n = (int)K; g.k = (int)N; g.act = act;
+  if ((s = set_out(g, dx, ldx))) return s;
+  if (act != KDA_ACT_NONE && (s = set_in(g, kInActGrad, z, ldz))) return s;
+  cudaStream_t st = (cudaStream_t)stream;
+  return dtype == KDA_BF16 ? dispatch<__nv_bfloat16, false, true, false>(g, dz, ldd, w, ldw, st)
+                           : dispatch<__half, false, true, false>(g, dz, ldd, w, ldw, st);
+}
+
+size_t kda_linear_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (check(KDA_BF16, KDA_ACT_NONE, M, N, K)) return 0;
+  return (size_t)((K + 63) / 64) * N * sizeof(float);
+}
+
+int kda_linear_wgrad(int dtype, int64_t M, int64_t N, int64_t K, const void *dz, int64_t ldd, const void *x, int64_t ldx,
+                     void *dw, int64_t ldw, void *db, void *ws, size_t ws_bytes, void *stream) {
+  int s = check(dtype, KDA_ACT_NONE, M, N, K);
+  if (s) return s;
+  if (!dz || !x || !dw || !ld_ok(ldd, N) || !ld_ok(ldx, K) || !ld_ok(ldw, K)) return KDA_ERR_INVALID_ARG;
+  if (!tma_able(dz, ldd) || !tma_able(x, ldx) || !even({dw, db})) return KDA_ERR_MISALIGNED;
+  if (db && (!ws || (uintptr_t)ws % 16 || ws_bytes < kda_linear_wgrad_workspace_bytes(M, N, K))) return KDA_ERR_WORKSPACE;
+  Args g = {};
+  g.m = (int)N; g.n = (int)K; g.k = (int)M;
+  if ((s = set_out(g, dw, ldw))) return s;
+  cudaStream_t st = (cudaStream_t)stream;
+  g.sums = static_cast<float *>(ws);
+  if (!db)
+    return dtype == KDA_BF16 ? dispatch<__nv_bfloat16, true, true, false>(g, dz, ldd, x, ldx, st)
+                             : dispatch<__half, true, true, false>(g, dz, ldd, x, ldx, st);
+  s = dtype == KDA_BF16 ? dispatch<__nv_bfloat16, true, true, true>(g, dz, ldd, x, ldx, st)
+                        : dispatch<__half, true, true, true>(g, dz, ldd, x, ldx, st);
+  if (s) return s;
+  const unsigned grid = (unsigned)((N + 255) / 256);
+  if (dtype == KDA_BF16) sums_kernel<<<grid, 256, 0, st>>>(g.sums, g.tiles_n, (int)N, static_cast<__nv_bfloat16 *>(db));
+  else sums_kernel<<<grid, 256, 0, st>>>(g.sums, g.tiles_n, (int)N, static_cast<__half *>(db));
+  if (cudaGetLastError() != cudaSuccess) return KDA_ERR_CUDA;
+  kda::count_launch();
+  return KDA_OK;
+}
+
+int kda_act_grad(int dtype, int act, int64_t rows, int64_t cols, const void *dy, int64_t ldy, const void *z, int64_t ldz,
+                 void *dz, int64_t ldd, void *stream) {
+  int s = check(dtype, act, rows, cols, 1);
+  if (s) return s;
+  if (!dy || !dz || !ld_ok(ldy, cols) || !ld_ok(ldd, cols) || (z && !ld_ok(ldz, cols)) || (act != KDA_ACT_NONE && !z))
+    return KDA_ERR_INVALID_ARG;
+  if (!even({dy, z, dz})) return KDA_ERR_MISALIGNED;
+  const dim3 grid((unsigned)((cols + 255) / 256 < 64 ? (cols + 255) / 256 : 64), (unsigned)(rows < 4096 ? rows : 4096));
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == KDA_BF16)
+    act_grad_kernel<<<grid, 256, 0, st>>>(act, rows, (int)cols, static_cast<const __nv_bfloat16 *>(dy), ldy,
+                                          static_cast<const __nv_bfloat16 *>(act ? z : nullptr), ldz,
+                                          static_cast<__nv_bfloat16 *>(dz), ldd);
+  else
+    act_grad_kernel<<<grid, 256, 0, st>>>(act, rows, (int)cols, static_cast<const __half *>(dy), ldy,
+                                          static_cast<const __half *>(act ? z : nullptr), ldz, static_cast<__half *>(dz), ldd);
+  if (cudaGetLastError() != cudaSuccess) return KDA_ERR_CUDA;
+  kda::count_launch();
+  return KDA_OK;
+}
+
+}  // extern "C"

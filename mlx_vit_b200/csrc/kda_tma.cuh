@@ -26,6 +26,11 @@ struct alignas(64) TmaMaps {
 int tma_map_bthd(CUtensorMap *map, const void *base, int64_t B, int64_t T, int64_t H, int64_t D, bool fp32,
                  const Str *st = nullptr);
 
+// Encodes the map of a row-major matrix of 16-bit elements ([rows][cols], `ld` elements from row to
+// row) with a box of box_rows x 64 columns, 128-byte swizzle.  KDA_ERR_MISALIGNED unless base and
+// row pitch are multiples of 16 bytes.
+int tma_map_rows16(CUtensorMap *map, const void *base, int64_t rows, int64_t cols, int64_t ld, int box_rows);
+
 // x: first column of the box (a multiple of 64 for bf16, of 32 for fp32)
 __device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap *map, int h, int t0, int b,
                                               uint32_t mbar, int x = 0) {

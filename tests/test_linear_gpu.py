@@ -1,0 +1,384 @@
+"""GPU: the linear products against the formulas in 64 bits.
+
+Tolerances, with h = finfo.eps / 2 (half a step of the 16-bit type) and u = 2^-24.  A product of
+length K accumulates in float32 with an error of at most (K + 2) u sum |a||b| (operands are exact),
+far under h at these sizes but carried along.  y: that error times the activation's slope (at
+most 1.13), the activation's own error (9e-6 relative of the distribution function, a few u
+else), and h of the result.  z and the gradient at z are stored in 16 bits: h of each, through the
+second derivative (at most 0.8) and the next product."""
+import math
+
+import pytest
+import torch
+
+from mlx_vit_b200 import _lib
+from mlx_vit_b200.linear import ACTIVATIONS, linear_act, mlp
+
+pytestmark = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16}
+SLOPE = 1.13   # largest |act'|
+CURVE = 0.8    # largest |act''|
+U = 2.0 ** -24
+
+
+def act64(z, kind):
+    if kind == "relu":
+        return torch.relu(z)
+    if kind == "silu":
+        return z * torch.sigmoid(z)
+    if kind == "gelu":
+        return z * torch.special.ndtr(z)
+    if kind == "gelu_tanh":
+        return 0.5 * z * (1 + torch.tanh(math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)))
+    return z
+
+
+def grad64(z, kind):
+    z = z.detach().requires_grad_()
+    with torch.enable_grad():
+        act64(z, kind).sum().backward()
+    return z.grad
+
+
+def rnd(g, *s, dt, scale=1.0):
+    return (torch.randn(*s, generator=g, device="cuda") * scale).to(dt)
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def near(got, want, tol, name):
+    err = (got.double() - want).abs()
+    bad = ~(err <= tol)
+    assert not bad.any(), (name, int(bad.sum()), float(err[bad].max()), tuple(bad.nonzero()[0].tolist()))
+
+
+def product(a, b):
+    """a b^T in 64 bits and the bound of its float32 accumulation."""
+    return a @ b.t(), (a.shape[1] + 2) * U * (a.abs() @ b.abs().t())
+
+
+def check_linear(m, n, k, dtype, act, bias, residual, seed=0, pad=0, train=True):
+    dt, h = DT[dtype], torch.finfo(DT[dtype]).eps / 2
+    tiny = float(torch.finfo(dt).tiny) * torch.finfo(dt).eps  # half a subnormal step and more
+    g = gen(seed)
+    x = rnd(g, m, k + pad, dt=dt)[:, :k]
+    w = rnd(g, n, k, dt=dt, scale=k ** -0.5)
+    b = rnd(g, n, dt=dt, scale=0.5) if bias else None
+    r = rnd(g, m, n + pad, dt=dt)[:, pad:] if residual else None
+    dy = rnd(g, m, n, dt=dt)
+    leaves = [t for t in (x, w, b, r) if t is not None]
+    if train:
+        for t in leaves:
+            t.requires_grad_()
+    y = linear_act(x, w, b, act, r)
+    assert y.shape == (m, n) and y.dtype == dt
+    X, W, DY = x.detach().double(), w.detach().double(), dy.double()
+    z, ez = product(X, W)
+    if bias:
+        z = z + b.detach().double()
+        ez = ez + U * z.abs()
+    a = act64(z, act)
+    want = a + (r.detach().double() if residual else 0)
+    ea = SLOPE * ez + 1.2e-5 * a.abs() + 8 * U * z.abs()
+    near(y, want, ea + h * want.abs() * 1.01 + tiny, "y")
+    if not train:
+        return
+    grads = dict(zip([i for i, t in enumerate((x, w, b, r)) if t is not None], torch.autograd.grad(y, leaves, dy)))
+    s = grad64(z, act)
+    dz = DY * s
+    if act == "none":
+        edz = torch.zeros_like(dz)
+    elif act == "relu":  # the sign of z may differ where z is within its own error of zero
+        edz = h * dz.abs() + DY.abs() * (z.abs() <= ez + h * z.abs() + tiny)
+    else:
+        edz = DY.abs() * (CURVE * (ez + h * z.abs() * 1.01 + tiny) + 2e-5) + h * dz.abs() * 1.01
+    edz = edz + (0 if act == "none" else tiny)
+    dx, e = product(dz, W.t())
+    near(grads[0], dx, e * 1.01 + edz @ W.abs() + h * dx.abs() * 1.01 + tiny, "dx")
+    dw, e = product(dz.t(), X.t())
+    near(grads[1], dw, e * 1.01 + edz.t() @ X.abs() + h * dw.abs() * 1.01 + tiny, "dw")
+    if bias:
+        db = dz.sum(0)
+        near(grads[2], db, (m + 2) * U * dz.abs().sum(0) + edz.sum(0) + h * db.abs() * 1.01 + tiny, "db")
+    if residual:
+        assert torch.equal(grads[3], dy)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("m,n,k", [(1, 8, 8), (1, 1, 1), (3, 5, 7), (64, 64, 64), (128, 128, 64), (129, 65, 72), (31, 400, 768),
+                                   (257, 255, 129), (500, 1000, 520), (16, 2304, 200)])
+def test_shapes(cuda, dtype, m, n, k):
+    check_linear(m, n, k, dtype, "none", True, True)
+
+
+@pytest.mark.parametrize("m,n,k", [(2048, 2304, 768), (3000, 2560, 136), (1900, 4100, 60), (4096, 1024, 4096), (5001, 2111, 333)])
+def test_large_tiles(cuda, m, n, k):
+    """Enough tiles for pairs of CTAs, whole and ragged."""
+    check_linear(m, n, k, "bf16", "gelu", True, True)
+
+
+def test_wgrad_large_tiles(cuda):
+    check_linear(300, 2600, 4200, "bf16", "none", True, False)
+
+
+@pytest.mark.parametrize("act", list(ACTIVATIONS))
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("bias,residual", [(True, True), (False, False), (True, False), (False, True)])
+def test_epilogues(cuda, act, dtype, bias, residual):
+    check_linear(200, 136, 96, dtype, act, bias, residual, seed=1)
+
+
+@pytest.mark.parametrize("pad", [1, 3, 8])
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_strided_views(cuda, pad, act):
+    check_linear(77, 90, 101, "bf16", act, True, True, seed=2, pad=pad)
+
+
+@pytest.mark.parametrize("m", [1, 2, 4, 7, 8, 9, 15, 16, 17, 32, 33, 100])
+def test_few_rows(cuda, m):
+    check_linear(m, 1000, 2056, "bf16", "gelu", True, True, seed=m, train=False)
+    check_linear(m, 130, 4097, "fp16", "silu", True, True, seed=m, train=False)
+
+
+def check_mlp(m, k, n, out, dtype, act, bias, residual, seed=0):
+    dt, h = DT[dtype], torch.finfo(DT[dtype]).eps / 2
+    tiny = float(torch.finfo(dt).tiny) * torch.finfo(dt).eps
+    g = gen(seed)
+    x, w1, w2 = rnd(g, m, k, dt=dt), rnd(g, n, k, dt=dt, scale=k ** -0.5), rnd(g, out, n, dt=dt, scale=n ** -0.5)
+    b1 = rnd(g, n, dt=dt, scale=0.5) if bias else None
+    b2 = rnd(g, out, dt=dt, scale=0.5) if bias else None
+    r = rnd(g, m, out, dt=dt) if residual else None
+    dy = rnd(g, m, out, dt=dt)
+    leaves = [t.requires_grad_() for t in (x, w1, b1, w2, b2, r) if t is not None]
+    y = mlp(x, w1, b1, w2, b2, act, r)
+    got = list(torch.autograd.grad(y, leaves, dy))
+    X, W1, W2, DY = (t.detach().double() for t in (x, w1, w2, dy))
+    z, ez = product(X, W1)
+    if bias:
+        z = z + b1.detach().double()
+        ez = ez + U * z.abs()
+    a = act64(z, act)
+    ea = SLOPE * ez + 1.2e-5 * a.abs() + 8 * U * z.abs() + h * a.abs() * 1.01 + tiny  # h is stored in 16 bits
+    want, e = product(a, W2)
+    ey = e * 1.01 + ea @ W2.abs().t()
+    if bias:
+        want = want + b2.detach().double()
+    if residual:
+        want = want + r.detach().double()
+    near(y, want, ey + 2 * U * want.abs() + h * want.abs() * 1.01 + tiny, "y")
+    dh, e = product(DY, W2.t())
+    s = grad64(z, act)
+    dz = dh * s
+    es = (z.abs() <= ez + h * z.abs() + tiny).double() if act == "relu" else \
+        CURVE * (ez + h * z.abs() * 1.01 + tiny) + 2e-5 if act != "none" else torch.zeros_like(z)
+    edz = SLOPE * e + dh.abs() * es + h * dz.abs() * 1.02 + tiny
+    checks = []
+    dx, e = product(dz, W1.t())
+    checks.append((dx, e * 1.01 + edz @ W1.abs()))
+    dw1, e = product(dz.t(), X.t())
+    checks.append((dw1, e * 1.01 + edz.t() @ X.abs()))
+    if bias:
+        checks.append((dz.sum(0), (m + 2) * U * dz.abs().sum(0) + edz.sum(0)))
+    dw2, e = product(DY.t(), a.t())
+    checks.append((dw2, e * 1.01 + DY.abs().t() @ ea))
+    if bias:
+        checks.append((DY.sum(0), (m + 2) * U * DY.abs().sum(0)))
+    for i, (v, e) in enumerate(checks):
+        near(got[i], v, e + h * v.abs() * 1.01 + tiny, i)
+    if residual:
+        assert torch.equal(got[-1], dy)
+
+
+@pytest.mark.parametrize("act", list(ACTIVATIONS))
+@pytest.mark.parametrize("m,k,n,out", [(50, 72, 200, 72), (1, 64, 256, 64), (131, 33, 77, 21)])
+def test_mlp(cuda, act, m, k, n, out):
+    check_mlp(m, k, n, out, "bf16", act, True, True)
+
+
+@pytest.mark.parametrize("dtype,bias,residual", [("fp16", True, True), ("bf16", False, False), ("bf16", False, True)])
+def test_mlp_large(cuda, dtype, bias, residual):
+    check_mlp(1568, 512, 2048, 512, dtype, "gelu", bias, residual)
+
+
+def test_leading_dimensions_and_layouts(cuda):
+    """(B, T, K) inputs, transposed and expanded views, gradients for some operands only."""
+    g = gen(5)
+    x = rnd(g, 3, 7, 40, dt=torch.bfloat16)
+    w = rnd(g, 40, 24, dt=torch.bfloat16, scale=0.2).t()       # column-major weight
+    r = rnd(g, 24, dt=torch.bfloat16).expand(3, 7, 24)          # broadcast residual
+    y = linear_act(x.transpose(0, 1), w, None, "none", r.transpose(0, 1))
+    want = x.transpose(0, 1).double() @ w.double().t() + r.double().transpose(0, 1)
+    assert y.shape == (7, 3, 24)
+    near(y, want, 2.0 ** -8 * want.abs() * 1.01 + 50 * U * 40, "y")
+    row = rnd(g, 1, 40, dt=torch.bfloat16).expand(5, 40)
+    near(linear_act(row, w), row.double() @ w.double().t(), 2.0 ** -8 * (row.double() @ w.double().t()).abs() * 1.01 + 50 * U * 40, "e")
+    one = linear_act(x[0, 0], w)
+    assert one.shape == (24,) and torch.equal(one, linear_act(x[:1, :1], w)[0, 0])
+    b = rnd(g, 24, dt=torch.bfloat16).requires_grad_()
+    linear_act(x, w, b, "gelu").sum().backward()
+    assert b.grad is not None and w.grad is None
+    rr = torch.zeros(3, 7, 24, dtype=torch.bfloat16, device=cuda, requires_grad=True)
+    linear_act(x, w, None, "none", rr).sum().backward()
+    assert (rr.grad == 1).all()
+
+
+def test_broadcast_leaf_gradients(cuda):
+    """A residual and an input that broadcast: their gradients are summed by autograd."""
+    g = gen(6)
+    x0, r0 = rnd(g, 1, 64, dt=torch.bfloat16).requires_grad_(), rnd(g, 32, dt=torch.bfloat16).requires_grad_()
+    w = rnd(g, 32, 64, dt=torch.bfloat16, scale=0.125)
+    dy = rnd(g, 6, 32, dt=torch.bfloat16)
+    linear_act(x0.expand(6, 64), w, None, "none", r0.expand(6, 32)).backward(dy)
+    want = dy.double().sum(0)
+    near(r0.grad, want, 6 * 2.0 ** -8 * dy.double().abs().sum(0), "r")
+    want = (dy.double() @ w.double())
+    near(x0.grad[0], want.sum(0), 7 * 2.0 ** -8 * want.abs().sum(0) + 1e-5, "x")
+
+
+def test_no_rows(cuda):
+    w = torch.ones(8, 16, dtype=torch.bfloat16, device=cuda, requires_grad=True)
+    x = torch.empty(2, 0, 16, dtype=torch.bfloat16, device=cuda, requires_grad=True)
+    b = torch.ones(8, dtype=torch.bfloat16, device=cuda, requires_grad=True)
+    y = linear_act(x, w, b, "gelu")
+    y.sum().backward()
+    assert y.shape == (2, 0, 8) and (w.grad == 0).all() and (b.grad == 0).all() and x.grad.shape == x.shape
+    w2 = torch.ones(16, 8, dtype=torch.bfloat16, device=cuda, requires_grad=True)
+    w.grad = None
+    y = mlp(x, w, b, w2, None, "gelu", x)
+    y.sum().backward()
+    assert y.shape == x.shape and (w.grad == 0).all() and (w2.grad == 0).all()
+
+
+def test_values_that_are_not_finite_stay_in_their_rows(cuda):
+    g = gen(8)
+    x = rnd(g, 40, 72, dt=torch.bfloat16)
+    w = rnd(g, 24, 72, dt=torch.bfloat16)
+    clean = linear_act(x, w, None, "relu")
+    x[3, 5], x[9, 0] = float("nan"), float("inf")
+    y = linear_act(x, w, None, "relu")
+    keep = torch.ones(40, dtype=torch.bool, device=cuda)
+    keep[[3, 9]] = False
+    assert torch.equal(y[keep], clean[keep]) and torch.isnan(y[3]).all()
+    assert torch.equal(torch.isinf(y[9]), w[:, 0] > 0)
+
+
+def test_rows_behind_the_last_are_left_alone(cuda):
+    """Outputs written through TMA and element by element end where the matrix ends."""
+    g = gen(9)
+    for n in (72, 75):
+        x, w = rnd(g, 70, 64, dt=torch.bfloat16), rnd(g, n, 64, dt=torch.bfloat16)
+        buf = torch.full((80, n), 7.0, dtype=torch.bfloat16, device=cuda)
+        L = _lib.lib()
+        _lib.check(L.kda_linear_fwd(_lib.KDA_BF16, 0, 70, n, 64, x.data_ptr(), 64, w.data_ptr(), 64, None, None, 0,
+                                    buf.data_ptr(), n, None, 0, torch.cuda.current_stream().cuda_stream), "fwd")
+        assert (buf[70:] == 7).all() and torch.equal(buf[:70], linear_act(x, w))
+
+
+def test_refusals(cuda):
+    x, w = torch.zeros(4, 16, dtype=torch.bfloat16, device=cuda), torch.zeros(8, 16, dtype=torch.bfloat16, device=cuda)
+    b, r = torch.zeros(8, dtype=torch.bfloat16, device=cuda), torch.zeros(4, 8, dtype=torch.bfloat16, device=cuda)
+    for bad in ((x.float(), w.float()), (x, w.half()), (x, w[:, :8]), (x, w[0]), (x, w, b[:4]), (x, w, b.float()),
+                (x, w, b, "swish"), (x, w, b, "gelu", r[:3]), (x, w.cpu()), (x, w[:0])):
+        with pytest.raises(ValueError):
+            linear_act(*bad)
+    with pytest.raises(ValueError):
+        mlp(x, w, None, w, None)
+    y = linear_act(x.requires_grad_(), w, b, "gelu")
+    (gx,) = torch.autograd.grad(y.float().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        gx.sum().backward()
+
+
+def test_same_results_every_time(cuda):
+    g = gen(10)
+    x, w1, w2 = rnd(g, 900, 256, dt=torch.bfloat16), rnd(g, 1024, 256, dt=torch.bfloat16, scale=0.06), rnd(g, 256, 1024, dt=torch.bfloat16, scale=0.03)
+    b1, b2 = rnd(g, 1024, dt=torch.bfloat16), rnd(g, 256, dt=torch.bfloat16)
+    outs = []
+    for _ in range(3):
+        leaves = [t.detach().requires_grad_() for t in (x, w1, b1, w2, b2)]
+        y = mlp(*leaves, "gelu", x)
+        outs.append([y.detach(), *torch.autograd.grad(y, leaves, x)])
+    for o in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(outs[0], o))
+
+
+def test_capture_and_two_streams(cuda):
+    """A training step captured into a graph and replayed on new inputs, two graphs one after the other,
+    and two streams at once: the same as eager."""
+    g = gen(11)
+    w1, w2 = rnd(g, 512, 128, dt=torch.bfloat16, scale=0.09), rnd(g, 128, 512, dt=torch.bfloat16, scale=0.04)
+    b1 = rnd(g, 512, dt=torch.bfloat16)
+
+    def step(x):
+        leaves = [t.detach().requires_grad_() for t in (x, w1, b1, w2)]
+        y = mlp(leaves[0], leaves[1], leaves[2], leaves[3], None, "gelu", leaves[0])
+        return [y.detach(), *torch.autograd.grad(y, leaves, x)]
+
+    xs = [rnd(g, 300 + 20 * i, 128, dt=torch.bfloat16) for i in range(2)]
+    eager = [step(x) for x in xs]
+    graphs = []
+    for x in xs:
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            step(x)
+        torch.cuda.current_stream().wait_stream(s)
+        graph, buf = torch.cuda.CUDAGraph(), x.clone()
+        with torch.cuda.graph(graph):
+            out = step(buf)
+        graphs.append((graph, buf, out))
+    for _ in range(2):
+        for (graph, buf, out), x, want in zip(graphs, xs, eager):
+            buf.copy_(x)
+            graph.replay()
+        for (graph, buf, out), want in zip(graphs, eager):
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = []
+    for s, x in zip(streams, xs):
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        got = []
+        for s, x in zip(streams, xs):
+            with torch.cuda.stream(s):
+                got.append(step(x))
+    torch.cuda.synchronize()
+    for o, want in zip(got, eager):
+        assert all(torch.equal(a, b) for a, b in zip(o, want))
+    assert _lib.lib().kda_device_status(0) == 0
+
+
+def test_offsets_past_32_bits(cuda):
+    """More than 2^31 elements in x, y and dy: the last rows are those of a small product."""
+    m, k, n = (1 << 25) + 40, 64, 72
+    w = rnd(gen(12), n, k, dt=torch.bfloat16, scale=0.125)
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device=cuda)
+    x[-300:] = rnd(gen(13), 300, k, dt=torch.bfloat16)
+    y = linear_act(x, w, None, "none")
+    assert torch.equal(y[-300:], linear_act(x[-300:].contiguous(), w))
+    assert (y[:100] == 0).all()
+    leaf = w.clone().requires_grad_()
+    out = linear_act(x, leaf)
+    (dw,) = torch.autograd.grad(out, leaf, y)
+    X, Y = x[-300:].double(), y[-300:].double()
+    want = Y.t() @ X
+    near(dw, want, 2.0 ** -8 * want.abs() * 1.01 + 400 * U * (Y.abs().t() @ X.abs()), "dw")
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_gradient_against_differences(cuda, act):
+    """Central differences of the 64-bit formula along the returned gradient's direction."""
+    g = gen(14)
+    x, w = rnd(g, 20, 48, dt=torch.float16).requires_grad_(), rnd(g, 40, 48, dt=torch.float16, scale=0.15).requires_grad_()
+    dy = rnd(g, 20, 40, dt=torch.float16)
+    gx, gw = torch.autograd.grad(linear_act(x, w, None, act), (x, w), dy)
+    f = lambda a, b: float((act64(a @ b.t(), act) * dy.double()).sum())  # noqa: E731
+    X, W = x.detach().double(), w.detach().double()
+    for grad, move in ((gx, lambda e, d: f(X + e * d, W)), (gw, lambda e, d: f(X, W + e * d))):
+        d = grad.double() / grad.double().norm()
+        diff = (move(1e-4, d) - move(-1e-4, d)) / 2e-4
+        assert abs(diff - float((grad.double() * d).sum())) <= 4e-3 * abs(diff)
