@@ -248,8 +248,8 @@ KDA_API int kda_bwd_noalloc(const KdaDesc *desc, const void *q, const void *k, c
  *                      which also brings a matrix into the alignment the others need
  *   kda_linear_dgrad:  dx [M][K] = dz [M][N] w [N][K]; with an activation times act'(z [M][K]), the
  *                      saved input of the activation that x came from
- *   kda_linear_wgrad:  dw [N][K] = dz^T x, db [N] = column sums of dz (db may be NULL, then no
- *                      workspace is needed)
+ *   kda_linear_wgrad:  dw [N][K] = dz^T x, db [N] = column sums of dz (db may be NULL); its workspace
+ *                      is what kda_linear_wgrad_workspace_bytes asks for (0: none)
  * bias, residual and db may be NULL.  Counterpart: the nn.Linear layers of the reference's
  * blocks and their MLP (HybridBlock, nope_gdn_mlx.py:4009-4090). */
 enum kda_act { KDA_ACT_NONE = 0, KDA_ACT_RELU = 1, KDA_ACT_SILU = 2, KDA_ACT_GELU = 3, KDA_ACT_GELU_TANH = 4 };
@@ -260,7 +260,7 @@ KDA_API int kda_linear_fwd(int dtype, int act, int64_t M, int64_t N, int64_t K, 
 KDA_API int kda_linear_dgrad(int dtype, int act, int64_t M, int64_t N, int64_t K, const void *dz, int64_t ldd,
                              const void *w, int64_t ldw, const void *z, int64_t ldz, void *dx, int64_t ldx,
                              void *stream);
-KDA_API size_t kda_linear_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K);
+KDA_API size_t kda_linear_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, int with_db);
 KDA_API int kda_linear_wgrad(int dtype, int64_t M, int64_t N, int64_t K, const void *dz, int64_t ldd,
                              const void *x, int64_t ldx, void *dw, int64_t ldw, void *db, void *ws,
                              size_t ws_bytes, void *stream);

@@ -121,7 +121,7 @@ def _declare(L):
     L.kda_adamw_workspace_bytes.restype = S
     L.kda_adamw_workspace_bytes.argtypes = [i64]
     L.kda_linear_wgrad_workspace_bytes.restype = S
-    L.kda_linear_wgrad_workspace_bytes.argtypes = [i64, i64, i64]
+    L.kda_linear_wgrad_workspace_bytes.argtypes = [i64, i64, i64, I]
     for n, a in (("kda_adamw_step", [ctypes.POINTER(KdaAdamW), P, i64, P, P, P, P, S, P]),
                  ("kda_grad_norm", [P, i64, P, P, S, P]),
                  ("kda_decode_state8", [i64, I, P, P, P, P]),
@@ -159,8 +159,8 @@ def lib(path: str | None = None):
 
 
 def tensors():
-    """The host module that reads lists of torch tensors (csrc/tensors_module.cpp); raises if it is
-    not built."""
+    """The host module around tensor lists and linear products (csrc/tensors_module.cpp); raises if it
+    is not built."""
     global _tensors
     if _tensors is None:
         try:

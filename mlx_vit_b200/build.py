@@ -38,7 +38,7 @@ def _deps():
 
 
 def build_host(verbose: bool = False) -> str:
-    """The CPython module that reads lists of torch tensors."""
+    """The CPython module around the library's host-bound operators."""
     import sysconfig
 
     import torch
@@ -49,7 +49,9 @@ def build_host(verbose: bool = False) -> str:
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-isystem", sysconfig.get_paths()["include"], *(f for p in include_paths() for f in ("-isystem", p)),
-           HOST_SRC, "-o", HOST_OUT, *(f"-L{p}" for p in library_paths()), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+           "-isystem", os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include"),
+           HOST_SRC, "-o", HOST_OUT, *(f"-L{p}" for p in library_paths()), f"-L{PKG}", "-Wl,-rpath,$ORIGIN",
+           "-l:libkda_b200.so", "-ltorch_python", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
     if verbose:
         print(" ".join(cmd))
     subprocess.run(cmd, check=True)

@@ -616,8 +616,8 @@ int kda_linear_dgrad(int dtype, int act, int64_t M, int64_t N, int64_t K, const 
                            : dispatch<__half, false, true, false>(g, dz, ldd, w, ldw, st);
 }
 
-size_t kda_linear_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  if (check(KDA_BF16, KDA_ACT_NONE, M, N, K)) return 0;
+size_t kda_linear_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, int with_db) {
+  if (!with_db || check(KDA_BF16, KDA_ACT_NONE, M, N, K)) return 0;
   return (size_t)((K + 63) / 64) * N * sizeof(float);
 }
 
@@ -627,7 +627,8 @@ int kda_linear_wgrad(int dtype, int64_t M, int64_t N, int64_t K, const void *dz,
   if (s) return s;
   if (!dz || !x || !dw || !ld_ok(ldd, N) || !ld_ok(ldx, K) || !ld_ok(ldw, K)) return KDA_ERR_INVALID_ARG;
   if (!tma_able(dz, ldd) || !tma_able(x, ldx) || !even({dw, db})) return KDA_ERR_MISALIGNED;
-  if (db && (!ws || (uintptr_t)ws % 16 || ws_bytes < kda_linear_wgrad_workspace_bytes(M, N, K))) return KDA_ERR_WORKSPACE;
+  if (db && (!ws || (uintptr_t)ws % 16 || ws_bytes < kda_linear_wgrad_workspace_bytes(M, N, K, 1)))
+    return KDA_ERR_WORKSPACE;
   Args g = {};
   g.m = (int)N; g.n = (int)K; g.k = (int)M;
   if ((s = set_out(g, dw, ldw))) return s;

@@ -1,12 +1,20 @@
-// mlx_vit_b200._tensors: the host-side reading of lists of torch tensors, in C++.
+// mlx_vit_b200._tensors: the host side of the operators whose launches are shorter than Python's way
+// to them, in C++: the reading of a model's tensor lists for the optimizer, and the linear
+// products with their autograd functions.
 //
-// A step over a model's parameters looks at some hundred tensors five times (parameter,
+// An optimizer step over a model's parameters looks at some hundred tensors five times (parameter,
 // gradient, two states, shadow) before its one launch.  From Python that is about 0.1 us an
 // attribute and 2.5 us a tensor, longer than the kernel for all but the largest models; here it is some
 // ten nanoseconds a tensor.  Nothing is kept between calls.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <ATen/cuda/CUDAContextLight.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -57,6 +65,10 @@ PyObject *guarded(F f) {
     return f();
   } catch (const Refused &r) {
     PyErr_SetString(PyExc_ValueError, r.why.c_str());
+  } catch (python_error &e) {
+    e.restore();
+  } catch (const c10::Error &e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
   } catch (const std::exception &e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
   }
@@ -189,9 +201,288 @@ PyObject *unlike(PyObject *, PyObject *args) {
   });
 }
 
+// ---- linear products ----
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+
+void done(int status, const char *where) {
+  TORCH_CHECK(status == 0, where, ": ", kda_strerror(status));
+}
+void *stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
+int dtype_of(const Tensor &t) { return t.scalar_type() == at::kBFloat16 ? KDA_BF16 : KDA_F16; }
+void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+// elements from row to row of a matrix with contiguous rows
+int64_t pitch(const Tensor &t) {
+  return !t.defined() ? 0 : t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), t.size(1));
+}
+// a matrix that the products can read: a row pitch of whole 16-byte units
+Tensor matrix(int64_t rows, int64_t cols, const Tensor &like) {
+  const int64_t ld = (cols + 7) / 8 * 8;
+  Tensor t = at::empty({rows, ld}, like.options());
+  return ld == cols ? t : t.narrow(1, 0, cols);
+}
+// a tensor as a matrix with contiguous rows, in place where its strides allow it
+Tensor rows_of(const Tensor &x, int64_t cols) {
+  Tensor t = x.dim() == 2 ? x : x.reshape({x.numel() / cols, cols});
+  if ((cols > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < cols)) t = t.contiguous();
+  return t;
+}
+void act_grad(int act, const Tensor &dy, const Tensor &z, const Tensor &dz) {
+  done(kda_act_grad(dtype_of(dy), act, dy.size(0), dy.size(1), ptr(dy), pitch(dy), ptr(z), pitch(z), ptr(dz), pitch(dz),
+                    stream()),
+       "kda_act_grad");
+}
+// the matrix itself where the products can read it, else a copy with padded rows
+Tensor readable(const Tensor &t) {
+  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && pitch(t) % 8 == 0) return t;
+  Tensor out = matrix(t.size(0), t.size(1), t);
+  act_grad(KDA_ACT_NONE, t, Tensor(), out);
+  return out;
+}
+void product(int act, const Tensor &x, const Tensor &w, const Tensor &b, const Tensor &r, const Tensor &y, const Tensor &z) {
+  done(kda_linear_fwd(dtype_of(x), act, x.size(0), w.size(0), w.size(1), ptr(x), pitch(x), ptr(w), pitch(w), ptr(b),
+                      ptr(r), pitch(r), ptr(y), pitch(y), ptr(z), pitch(z), stream()),
+       "kda_linear_fwd");
+}
+void dgrad(int act, const Tensor &dz, const Tensor &w, const Tensor &z, const Tensor &dx) {
+  done(kda_linear_dgrad(dtype_of(dz), act, dz.size(0), w.size(0), w.size(1), ptr(dz), pitch(dz), ptr(w), pitch(w), ptr(z),
+                        pitch(z), ptr(dx), pitch(dx), stream()),
+       "kda_linear_dgrad");
+}
+void wgrad(const Tensor &dz, const Tensor &x, bool want_db, Tensor &dw, Tensor &db) {
+  const int64_t m = dz.size(0), n = dz.size(1), k = x.size(1);
+  dw = at::empty({n, k}, x.options());
+  if (want_db) db = at::empty({n}, x.options());
+  const size_t nws = kda_linear_wgrad_workspace_bytes(m, n, k, want_db);
+  Tensor ws;
+  if (nws) ws = at::empty({(int64_t)nws}, x.options().dtype(at::kByte));
+  done(kda_linear_wgrad(dtype_of(x), m, n, k, ptr(dz), pitch(dz), ptr(x), pitch(x), ptr(dw), k, ptr(db), ptr(ws), nws, stream()),
+       "kda_linear_wgrad");
+}
+std::vector<int64_t> with_last(const Tensor &x, int64_t n) {
+  std::vector<int64_t> s = x.sizes().vec();
+  s.back() = n;
+  return s;
+}
+// the results of a backward pass that has no derivative of its own
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list in;
+  for (Tensor &g : grads)
+    if (g.defined()) in.push_back(g = g.detach().requires_grad_());
+  variable_list out = torch::autograd::DelayedError("the linear products are differentiable once", (int)in.size())(variable_list(in));
+  size_t i = 0;
+  for (Tensor &g : grads)
+    if (g.defined()) g = out[i++];
+  return grads;
+}
+
+using Maybe = std::optional<Tensor>;
+Maybe maybe(const Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); }
+Tensor plain(const Maybe &t) { return t ? *t : Tensor(); }
+// which of the tensor arguments need a gradient; an absent one has no edge in the graph
+struct Needs {
+  const AutogradContext *ctx;
+  size_t edge = 0;
+  bool operator()(bool present) { return present && ctx->needs_input_grad(edge++); }
+};
+
+struct LinearAct : public torch::autograd::Function<LinearAct> {
+  static Tensor forward(AutogradContext *ctx, Tensor x, Tensor w, Maybe bias, Maybe residual, int64_t act, bool save) {
+    const int64_t n = w.size(0), k = w.size(1);
+    const Tensor b = plain(bias), r = plain(residual);
+    Tensor y = at::empty(with_last(x, n), x.options()), z;
+    if (x.numel()) {
+      const c10::cuda::CUDAGuard guard(x.device());
+      Tensor x2 = readable(rows_of(x, k)), w2 = readable(rows_of(w, k));
+      if (save && act) z = matrix(x2.size(0), n, x);
+      product((int)act, x2, w2, b.defined() ? b.contiguous() : b, r.defined() ? rows_of(r, n) : r, y.view({-1, n}), z);
+      if (save) ctx->save_for_backward({x2, w2, z});
+    } else if (save) {
+      ctx->save_for_backward({x, w, z});
+    }
+    if (save) {
+      ctx->saved_data["act"] = act;
+      ctx->saved_data["sizes"] = x.sizes().vec();
+      ctx->saved_data["bias"] = b.defined();
+      ctx->saved_data["residual"] = r.defined();
+    }
+    return y;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list dys) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor x = saved[0].detach(), w = saved[1].detach(), z = saved[2], dy = dys[0].detach();
+    const int64_t n = w.size(0), k = w.size(1);
+    const int act = (int)ctx->saved_data["act"].toInt();
+    const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
+    Needs needs{ctx};
+    const bool need_x = needs(true), need_w = needs(true), need_b = needs(ctx->saved_data["bias"].toBool());
+    variable_list g(6);
+    if (needs(ctx->saved_data["residual"].toBool())) g[3] = dy;
+    if (x.numel() == 0) {
+      if (need_x) g[0] = at::zeros(sizes, x.options());
+      if (need_w) g[1] = at::zeros_like(w);
+      if (need_b) g[2] = at::zeros({n}, w.options());
+    } else if (need_x || need_w || need_b) {
+      const c10::cuda::CUDAGuard guard(x.device());
+      Tensor dz = rows_of(dy, n);
+      if (act) {
+        const Tensor out = matrix(dz.size(0), n, dz);
+        act_grad(act, dz, z, out);
+        dz = out;
+      } else {
+        dz = readable(dz);
+      }
+      if (need_x) {
+        g[0] = at::empty(sizes, x.options());
+        dgrad(KDA_ACT_NONE, dz, w, Tensor(), g[0].view({-1, k}));
+      }
+      if (need_w || need_b) wgrad(dz, x, need_b, g[1], g[2]);
+      if (!need_w) g[1] = Tensor();
+    }
+    return once(g);
+  }
+};
+
+struct Mlp : public torch::autograd::Function<Mlp> {
+  static Tensor forward(AutogradContext *ctx, Tensor x, Tensor w1, Maybe bias1, Tensor w2, Maybe bias2, Maybe residual,
+                        int64_t act, bool save) {
+    const int64_t n = w1.size(0), k = w1.size(1), out = w2.size(0);
+    const Tensor b1 = plain(bias1), b2 = plain(bias2), r = plain(residual);
+    Tensor y = at::empty(with_last(x, out), x.options()), h, z;
+    if (x.numel()) {
+      const c10::cuda::CUDAGuard guard(x.device());
+      const Tensor x2 = readable(rows_of(x, k)), u1 = readable(rows_of(w1, k)), u2 = readable(rows_of(w2, n));
+      h = matrix(x2.size(0), n, x);
+      if (save && act) z = matrix(x2.size(0), n, x);
+      product((int)act, x2, u1, b1.defined() ? b1.contiguous() : b1, Tensor(), h, z);
+      product(KDA_ACT_NONE, h, u2, b2.defined() ? b2.contiguous() : b2, r.defined() ? rows_of(r, out) : r, y.view({-1, out}),
+              Tensor());
+      if (save) ctx->save_for_backward({x2, u1, u2, h, z});
+    } else if (save) {
+      ctx->save_for_backward({x, w1, w2, h, z});
+    }
+    if (save) {
+      ctx->saved_data["act"] = act;
+      ctx->saved_data["sizes"] = x.sizes().vec();
+      ctx->saved_data["bias1"] = b1.defined();
+      ctx->saved_data["bias2"] = b2.defined();
+      ctx->saved_data["residual"] = r.defined();
+    }
+    return y;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list dys) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor x = saved[0].detach(), w1 = saved[1].detach(), w2 = saved[2].detach(), h = saved[3], z = saved[4],
+                 dy = dys[0].detach();
+    const int64_t n = w1.size(0), k = w1.size(1), out = w2.size(0);
+    const int act = (int)ctx->saved_data["act"].toInt();
+    const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
+    Needs needs{ctx};
+    const bool need_x = needs(true), need_w1 = needs(true), need_b1 = needs(ctx->saved_data["bias1"].toBool()),
+               need_w2 = needs(true), need_b2 = needs(ctx->saved_data["bias2"].toBool());
+    variable_list g(8);
+    if (needs(ctx->saved_data["residual"].toBool())) g[5] = dy;
+    if (x.numel() == 0) {
+      if (need_x) g[0] = at::zeros(sizes, x.options());
+      if (need_w1) g[1] = at::zeros_like(w1);
+      if (need_b1) g[2] = at::zeros({n}, w1.options());
+      if (need_w2) g[3] = at::zeros_like(w2);
+      if (need_b2) g[4] = at::zeros({out}, w2.options());
+    } else if (need_x || need_w1 || need_b1 || need_w2 || need_b2) {
+      const c10::cuda::CUDAGuard guard(x.device());
+      const Tensor dy2 = readable(rows_of(dy, out));
+      if (need_w2 || need_b2) wgrad(dy2, h, need_b2, g[3], g[4]);
+      if (need_x || need_w1 || need_b1) {
+        const Tensor dz = matrix(dy2.size(0), n, x);
+        dgrad(act, dy2, w2, z, dz);
+        if (need_x) {
+          g[0] = at::empty(sizes, x.options());
+          dgrad(KDA_ACT_NONE, dz, w1, Tensor(), g[0].view({-1, k}));
+        }
+        if (need_w1 || need_b1) wgrad(dz, x, need_b1, g[1], g[2]);
+      }
+      if (!need_w1) g[1] = Tensor();
+      if (!need_w2) g[3] = Tensor();
+    }
+    return once(g);
+  }
+};
+
+std::string shape_of(const Tensor &t) {
+  std::string s = "(";
+  for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
+  return s + ")";
+}
+Tensor operand(PyObject *o, const char *name, bool optional) {
+  if (optional && o == Py_None) return Tensor();
+  if (!THPVariable_Check(o)) throw Refused{std::string(name) + ": expected a torch tensor"};
+  return THPVariable_Unpack(o);
+}
+struct Layer {
+  const char *name;
+  const Tensor &w, &b;
+};
+void check_operands(const Tensor &x, const Tensor &r, std::initializer_list<Layer> layers) {
+  need(x.is_cuda(), "linear products take CUDA tensors; there is no CPU path");
+  need(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, "linear products take bfloat16 or float16");
+  need(x.dim() >= 1, "x must have at least one dimension");
+  int64_t k = x.size(-1);
+  auto like_x = [&](const Tensor &t) {
+    need(t.device() == x.device() && t.scalar_type() == x.scalar_type(), "all operands must share x's dtype and device");
+  };
+  for (const Layer &l : layers) {
+    if (l.w.dim() != 2 || l.w.size(1) != k || l.w.size(0) < 1 || k < 1)
+      throw Refused{std::string(l.name) + " must be (out_features, " + std::to_string(k) + "), got " + shape_of(l.w)};
+    like_x(l.w);
+    k = l.w.size(0);
+    if (!l.b.defined()) continue;
+    if (l.b.dim() != 1 || l.b.size(0) != k)
+      throw Refused{"the bias of " + std::string(l.name) + " must be (" + std::to_string(k) + "), got " + shape_of(l.b)};
+    like_x(l.b);
+  }
+  if (!r.defined()) return;
+  like_x(r);
+  if (r.sizes() != at::IntArrayRef(with_last(x, k)))
+    throw Refused{"residual must have x's leading dimensions and " + std::to_string(k) + " columns, got " + shape_of(r)};
+}
+template <typename... T>
+bool grads_wanted(const T &...t) {
+  return at::GradMode::is_enabled() && ((t.defined() && t.requires_grad()) || ...);
+}
+
+// linear_act(x, w, b or None, act, residual or None) -> y
+PyObject *linear_act(PyObject *, PyObject *args) {
+  PyObject *xo, *wo, *bo, *ro;
+  int act;
+  if (!PyArg_ParseTuple(args, "OOOiO", &xo, &wo, &bo, &act, &ro)) return nullptr;
+  return guarded([&]() -> PyObject * {
+    const Tensor x = operand(xo, "x", false), w = operand(wo, "weight", false), b = operand(bo, "bias", true),
+                 r = operand(ro, "residual", true);
+    check_operands(x, r, {{"weight", w, b}});
+    return THPVariable_Wrap(LinearAct::apply(x, w, maybe(b), maybe(r), (int64_t)act, grads_wanted(x, w, b, r)));
+  });
+}
+// mlp(x, w1, b1 or None, w2, b2 or None, act, residual or None) -> y
+PyObject *mlp(PyObject *, PyObject *args) {
+  PyObject *xo, *w1o, *b1o, *w2o, *b2o, *ro;
+  int act;
+  if (!PyArg_ParseTuple(args, "OOOOOiO", &xo, &w1o, &b1o, &w2o, &b2o, &act, &ro)) return nullptr;
+  return guarded([&]() -> PyObject * {
+    const Tensor x = operand(xo, "x", false), w1 = operand(w1o, "w1", false), b1 = operand(b1o, "b1", true),
+                 w2 = operand(w2o, "w2", false), b2 = operand(b2o, "b2", true), r = operand(ro, "residual", true);
+    check_operands(x, r, {{"w1", w1, b1}, {"w2", w2, b2}});
+    return THPVariable_Wrap(Mlp::apply(x, w1, maybe(b1), w2, maybe(b2), maybe(r), (int64_t)act, grads_wanted(x, w1, b1, w2, b2, r)));
+  });
+}
+
 PyMethodDef methods[] = {{"adamw_table", adamw_table, METH_VARARGS, nullptr},
                          {"grad_table", grad_table, METH_VARARGS, nullptr},
                          {"unlike", unlike, METH_VARARGS, nullptr},
+                         {"linear_act", linear_act, METH_VARARGS, nullptr},
+                         {"mlp", mlp, METH_VARARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensors", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -49,6 +49,6 @@ def test_backward_refusals():
     assert st(L.kda_linear_dgrad(bf, 0, 4, 8, 16, A, 12, A, 16, n, 0, A, 16, n)) == "MISALIGNED"
     assert st(L.kda_linear_wgrad(bf, 4, 8, 16, A, 8, A, 16, A, 16, A, n, 0, n)) == "WORKSPACE"
     assert st(L.kda_linear_wgrad(bf, 4, 8, 16, A, 8, A, 16, A, 15, n, n, 0, n)) == "INVALID_ARG"
-    assert L.kda_linear_wgrad_workspace_bytes(4, 8, 16) >= 8 * 4 and L.kda_linear_wgrad_workspace_bytes(0, 8, 16) == 0
+    assert L.kda_linear_wgrad_workspace_bytes(4, 8, 16, 1) >= 8 * 4 and L.kda_linear_wgrad_workspace_bytes(0, 8, 16, 1) == 0
     assert st(L.kda_act_grad(bf, 1, 4, 8, A, 8, n, 0, A, 8, n)) == "INVALID_ARG"
     assert st(L.kda_act_grad(bf, 0, 4, 8, A + 1, 8, n, 0, A, 8, n)) == "MISALIGNED"
