@@ -248,19 +248,21 @@ KDA_API int kda_bwd_noalloc(const KdaDesc *desc, const void *q, const void *k, c
  *                      which also brings a matrix into the alignment the others need
  *   kda_linear_dgrad:  dx [M][K] = dz [M][N] w [N][K]; with an activation times act'(z [M][K]), the
  *                      saved input of the activation that x came from
- *   kda_linear_wgrad:  dw [N][K] = dz^T x, db [N] = column sums of dz (db may be NULL); its workspace
- *                      is what kda_linear_wgrad_workspace_bytes asks for (0: none)
- * bias, residual and db may be NULL.  Counterpart: the nn.Linear layers of the reference's
- * blocks and their MLP (HybridBlock, nope_gdn_mlx.py:4009-4090). */
+ *   kda_linear_wgrad:  dw [N][K] = dz^T x, db [N] = column sums of dz (needs a workspace)
+ * bias, residual and db may be NULL.  kda_linear_workspace_bytes says what workspace (16-byte
+ * aligned) a call on the current device takes (op: KDA_LINEAR_*); with ws NULL a product whose
+ * tiles do not fill the GPU is not split along its sum, and takes longer.  Counterpart: the
+ * nn.Linear layers of the reference's blocks and their MLP (HybridBlock, nope_gdn_mlx.py:4009-4090). */
 enum kda_act { KDA_ACT_NONE = 0, KDA_ACT_RELU = 1, KDA_ACT_SILU = 2, KDA_ACT_GELU = 3, KDA_ACT_GELU_TANH = 4 };
+enum kda_linear_op { KDA_LINEAR_FWD = 0, KDA_LINEAR_DGRAD = 1, KDA_LINEAR_WGRAD = 2 };
 
+KDA_API size_t kda_linear_workspace_bytes(int op, int64_t M, int64_t N, int64_t K, int with_db);
 KDA_API int kda_linear_fwd(int dtype, int act, int64_t M, int64_t N, int64_t K, const void *x, int64_t ldx,
                            const void *w, int64_t ldw, const void *bias, const void *residual, int64_t ldr,
-                           void *y, int64_t ldy, void *z, int64_t ldz, void *stream);
+                           void *y, int64_t ldy, void *z, int64_t ldz, void *ws, size_t ws_bytes, void *stream);
 KDA_API int kda_linear_dgrad(int dtype, int act, int64_t M, int64_t N, int64_t K, const void *dz, int64_t ldd,
                              const void *w, int64_t ldw, const void *z, int64_t ldz, void *dx, int64_t ldx,
-                             void *stream);
-KDA_API size_t kda_linear_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, int with_db);
+                             void *ws, size_t ws_bytes, void *stream);
 KDA_API int kda_linear_wgrad(int dtype, int64_t M, int64_t N, int64_t K, const void *dz, int64_t ldd,
                              const void *x, int64_t ldx, void *dw, int64_t ldw, void *db, void *ws,
                              size_t ws_bytes, void *stream);

@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(_HERE, "libkda_b200.so")
 KDA_ABI_VERSION = 7
 KDA_F32, KDA_BF16, KDA_F16 = 0, 1, 2
 KDA_ACT_NONE, KDA_ACT_RELU, KDA_ACT_SILU, KDA_ACT_GELU, KDA_ACT_GELU_TANH = range(5)
+KDA_LINEAR_FWD, KDA_LINEAR_DGRAD, KDA_LINEAR_WGRAD = range(3)
 KDA_FLAG_FORCE_GENERIC = 0x1
 KDA_FLAG_DEBUG_WAIT_TIMEOUT = 0x2
 
@@ -33,8 +34,7 @@ EXPORTS = ("kda_abi_version", "kda_strerror", "kda_check_desc", "kda_workspace_b
            "kda_l2norm_silu_fwd", "kda_l2norm_silu_bwd", "kda_gated_rmsnorm_fwd", "kda_gated_rmsnorm_bwd",
            "kda_conv_silu_fwd", "kda_conv_silu_bwd",
            "kda_adamw_workspace_bytes", "kda_adamw_step", "kda_grad_norm", "kda_decode_state8",
-           "kda_linear_fwd", "kda_linear_dgrad", "kda_linear_wgrad_workspace_bytes", "kda_linear_wgrad",
-           "kda_act_grad")
+           "kda_linear_workspace_bytes", "kda_linear_fwd", "kda_linear_dgrad", "kda_linear_wgrad", "kda_act_grad")
 
 
 class KdaStrides(ctypes.Structure):
@@ -120,13 +120,13 @@ def _declare(L):
     # the tensor table (KdaAdamWTensor) is passed as an array of 9 int64 per tensor
     L.kda_adamw_workspace_bytes.restype = S
     L.kda_adamw_workspace_bytes.argtypes = [i64]
-    L.kda_linear_wgrad_workspace_bytes.restype = S
-    L.kda_linear_wgrad_workspace_bytes.argtypes = [i64, i64, i64, I]
+    L.kda_linear_workspace_bytes.restype = S
+    L.kda_linear_workspace_bytes.argtypes = [I, i64, i64, i64, I]
     for n, a in (("kda_adamw_step", [ctypes.POINTER(KdaAdamW), P, i64, P, P, P, P, S, P]),
                  ("kda_grad_norm", [P, i64, P, P, S, P]),
                  ("kda_decode_state8", [i64, I, P, P, P, P]),
-                 ("kda_linear_fwd", [I, I, i64, i64, i64, P, i64, P, i64, P, P, i64, P, i64, P, i64, P]),
-                 ("kda_linear_dgrad", [I, I, i64, i64, i64, P, i64, P, i64, P, i64, P, i64, P]),
+                 ("kda_linear_fwd", [I, I, i64, i64, i64, P, i64, P, i64, P, P, i64, P, i64, P, i64, P, S, P]),
+                 ("kda_linear_dgrad", [I, I, i64, i64, i64, P, i64, P, i64, P, i64, P, i64, P, S, P]),
                  ("kda_linear_wgrad", [I, i64, i64, i64, P, i64, P, i64, P, i64, P, P, S, P]),
                  ("kda_act_grad", [I, I, i64, i64, P, i64, P, i64, P, i64, P])):
         getattr(L, n).restype = I

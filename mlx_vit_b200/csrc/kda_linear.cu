@@ -11,7 +11,10 @@
 // half of B each) walks its tiles with one thread copying operand blocks of 64 k by TMA into a
 // ring of stages, one thread issuing the products, and eight warps taking finished accumulators
 // from tensor memory through the epilogue while the next tile's products run (two accumulators).
-// Rows, columns and k past the end are TMA's zero fill and clipped stores.
+// Rows, columns and k past the end are TMA's zero fill and clipped stores.  Where the tiles are too few
+// to fill the GPU, k is split: each part writes its float32 tile to a workspace and a second kernel
+// adds the parts in order and runs the epilogue.  A few rows (M <= 32) take a kernel of their own
+// that streams the weights once through registers.
 #include <initializer_list>
 
 #include "kda_act.cuh"
@@ -38,12 +41,13 @@ constexpr int kPolls = 1 << 20;   // bound of a wait: some tens of milliseconds 
 enum { kInNone = 0, kInAdd = 1, kInActGrad = 2 };
 
 struct alignas(64) Args {
-  CUtensorMap a, b, out, in, z;
-  int64_t ldo, ldi;
+  CUtensorMap a, b, out, in, z;   // split: out is the workspace of partial tiles
+  int64_t ldo, ldi, ldz, ldp;
   const void *bias, *in_ptr;
-  void *out_ptr;
-  float *sums;          // ONES: [tiles_n][m] partial column sums of A
-  int m, n, k, tiles_m, tiles_n;
+  void *out_ptr, *z_ptr;
+  float *part;          // split: [splits][tiles_m 128 CG][ldp] partial products
+  float *sums;          // ONES: [splits tiles_n][m] partial column sums of A
+  int m, n, k, tiles_m, tiles_n, splits, per_split;  // per_split: blocks of 64 k a part takes
   uint32_t idesc, idesc_ones;
   int act, in_kind, out_tma, in_tma, save_z;
 };
@@ -188,6 +192,66 @@ __device__ __forceinline__ void tile_out(const uint8_t *st, T *p, int64_t ld, in
   }
 }
 
+// One 32 x 64 chunk of an accumulator to a warp's staging rows: bias, the activation (kForward) or
+// its derivative at the staged z (kGrad), the staged residual, and z itself.
+enum { kPlain = 0, kForward = 1, kGrad = 2 };
+template <typename T, int KIND, int ACT>
+__device__ __forceinline__ void finish8(float (&v)[8], uint4 *slot, bool add) {
+  using P = Pair<T>;
+  if (KIND == kGrad && ACT != KDA_ACT_NONE) {
+    const uint4 zi = *slot;
+    const uint32_t w[4] = {zi.x, zi.y, zi.z, zi.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 z = P::unpack(w[j]);
+      v[2 * j] *= activate_grad(ACT, z.x);
+      v[2 * j + 1] *= activate_grad(ACT, z.y);
+    }
+  } else if (KIND == kForward) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = activate(ACT, v[j]);
+    if (add) {
+      const uint4 ri = *slot;
+      const uint32_t w[4] = {ri.x, ri.y, ri.z, ri.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 x = P::unpack(w[j]);
+        v[2 * j] += x.x;
+        v[2 * j + 1] += x.y;
+      }
+    }
+  }
+}
+template <typename T, int KIND, int ACT>
+__device__ __forceinline__ void chunk(const Args &g, uint32_t acc, uint8_t *so, uint8_t *sz, const float *bs, int lane) {
+  using P = Pair<T>;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t r[32];
+    tmem_ld32(acc + 32 * h, r);
+    tmem_wait_ld();
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {  // 8 columns: one 16-byte chunk of the row
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[8 * u + j]);
+      if (KIND == kForward && g.bias) {
+        const float4 b0 = *reinterpret_cast<const float4 *>(bs + 32 * h + 8 * u);
+        const float4 b1 = *reinterpret_cast<const float4 *>(bs + 32 * h + 8 * u + 4);
+        v[0] += b0.x; v[1] += b0.y; v[2] += b0.z; v[3] += b0.w;
+        v[4] += b1.x; v[5] += b1.y; v[6] += b1.z; v[7] += b1.w;
+      }
+      const uint32_t at = chunk_at(lane, 4 * h + u);
+      uint4 *slot = reinterpret_cast<uint4 *>(so + at);
+      if (KIND == kForward && g.save_z)
+        *reinterpret_cast<uint4 *>(sz + at) =
+            make_uint4(P::pack(v[0], v[1]), P::pack(v[2], v[3]), P::pack(v[4], v[5]), P::pack(v[6], v[7]));
+      finish8<T, KIND, ACT>(v, slot, g.in_kind == kInAdd);
+      *slot = make_uint4(P::pack(v[0], v[1]), P::pack(v[2], v[3]), P::pack(v[4], v[5]), P::pack(v[6], v[7]));
+    }
+  }
+}
+
 template <typename T, int CG, int BN, bool A_MN, bool B_MN, bool ONES>
 __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ Args g) {
   using S = Shape<CG, BN, ONES>;
@@ -202,12 +266,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   }
   uint8_t *staging = sm + S::kStages * S::kStage, *ones = staging + kStaging;
   float *bias_sm = reinterpret_cast<float *>(ones + S::kOnes);
-  // barriers: full[stages], empty[stages], acc_full[2], acc_empty[2], in[8 warps]; then tensor memory's address
+  // barriers: full[stages], empty[stages], acc_full[2], acc_empty[2], in[8 warps][2]; then tensor memory's address
   const uint32_t bars = smem_u32(bias_sm) + kEpiWarps * 256;
   const uint32_t full = bars, empty = full + 8 * S::kStages, acc_full = empty + 8 * S::kStages,
-                 acc_empty = acc_full + 16, in_bar = acc_empty + 16, tmem_at = in_bar + 8 * kEpiWarps;
+                 acc_empty = acc_full + 16, in_bar = acc_empty + 16, tmem_at = in_bar + 16 * kEpiWarps;
   const int kblocks = (g.k + kBlockK - 1) / kBlockK;
-  const int tiles = g.tiles_m * g.tiles_n, first = blockIdx.x / CG, step = gridDim.x / CG;
+  const int tiles = g.tiles_m * g.tiles_n, units = tiles * g.splits, first = blockIdx.x / CG, step = gridDim.x / CG;
 
   if (tid == 0) {
     for (int s = 0; s < S::kStages; ++s) {
@@ -218,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       mbar_init(acc_full + 8 * i, 1);
       mbar_init(acc_empty + 8 * i, kEpiWarps * CG);
     }
-    for (int w = 0; w < kEpiWarps; ++w) mbar_init(in_bar + 8 * w, 1);
+    for (int w = 0; w < 2 * kEpiWarps; ++w) mbar_init(in_bar + 8 * w, 1);
     mbar_fence_init();
   }
   if (ONES)
@@ -237,10 +301,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       // ---- operand copies; both CTAs' bytes of a stage arrive on the first CTA's barrier ----
       const uint32_t full_lead = CG == 2 ? map_rank(full, 0) : full;
       uint32_t it = 0;
-      for (int t = first; ok && t < tiles; t += step) {
+      for (int u = first; ok && u < units; u += step) {
+        const int t = u % tiles, kb0 = u / tiles * g.per_split, kb1 = min(kblocks, kb0 + g.per_split);
         const int m0 = (t / g.tiles_n) * 128 * CG + (int)rank * 128;
         const int n0 = (t % g.tiles_n) * BN + (int)rank * (BN / CG);
-        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const uint32_t s = it % S::kStages, ph = (it / S::kStages) & 1;
           if (!(ok = wait_cluster(empty + 8 * s, ph ^ 1))) break;
           if (rank == 0) mbar_expect_tx(full + 8 * s, S::kStage * CG);
@@ -269,14 +334,15 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     if (lane == 0 && rank == 0) {
       // ---- products ----
       uint32_t it = 0, n = 0;
-      for (int t = first; ok && t < tiles; t += step, ++n) {
+      for (int u = first; ok && u < units; u += step, ++n) {
+        const int t = u % tiles, kb0 = u / tiles * g.per_split, kb1 = min(kblocks, kb0 + g.per_split);
         const uint32_t buf = n % S::kBufs, use = n / S::kBufs;
         const uint32_t d = tmem + buf * S::kAcc;
         if (!(ok = wait_cluster(acc_empty + 8 * buf, (use & 1) ^ 1))) break;
         tc_fence_after();
         const int tn = t % g.tiles_n;
         bool summed = false;
-        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const uint32_t s = it % S::kStages, ph = (it / S::kStages) & 1;
           if (!(ok = wait_cluster(full + 8 * s, ph))) break;
           tc_fence_after();
@@ -284,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
 #pragma unroll
           for (int k = 0; k < kBlockK / 16; ++k)
             mma<CG>(d, A_MN ? desc_mn(at, k) : desc_k(at, k), B_MN ? desc_mn(bt, k) : desc_k(bt, k), g.idesc,
-                    kb > 0 || k > 0);
+                    kb > kb0 || k > 0);
           if (ONES && kb % g.tiles_n == tn) {  // the column sums' share of this column tile
 #pragma unroll
             for (int k = 0; k < kBlockK / 16; ++k)
@@ -302,18 +368,37 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     // ---- epilogue: warp (q, half) takes rows 32 q .. 32 q + 31 of every second 64-column chunk ----
     const int e = warp - kEpiWarp, q = warp & 3, half = e >> 2;
     uint8_t *st = staging + e * 8192;
-    const uint32_t st_at = smem_u32(st), my_in = in_bar + 8 * e;
+    const uint32_t st_at = smem_u32(st), my_in = in_bar + 16 * e;
     float *bs = bias_sm + e * 64;
     const uint32_t empty_lead = CG == 2 ? map_rank(acc_empty, 0) : acc_empty;
-    const T *bias = static_cast<const T *>(g.bias);
-    uint32_t n = 0, in_phase = 0, flip = 0;
-    for (int t = first; ok && t < tiles; t += step, ++n) {
+    uint32_t n = 0, in_phase = 0, flip = 0;  // in_phase: bit b for staging tile b
+    // with a z to save the second staging tile is z's, else the chunks alternate
+    const bool in_tma = g.in_kind && g.in_tma && g.splits == 1, ahead = in_tma && !g.save_z;
+    for (int u = first; ok && u < units; u += step, ++n) {
+      const int t = u % tiles, part = u / tiles;
       const uint32_t buf = n % S::kBufs, use = n / S::kBufs;
       const int tm = t / g.tiles_n, tn = t % g.tiles_n;
       const int row0 = tm * 128 * CG + (int)rank * 128 + 32 * q;
+      auto fetch = [&](int b, int col0) {  // residual or z of a chunk into staging tile b (lane 0)
+        mbar_expect_tx(my_in + 8 * b, 4096);
+        load_box<1>(st_at + 4096 * b, &g.in, col0, row0, my_in + 8 * b);
+      };
+      if (ahead) {  // ahead of the accumulator: this tile's two chunks
+        if (lane == 0) store_wait_read<0>();
+        __syncwarp();
+        if (lane == 0) {
+          fence_proxy_async_smem();
+          for (int i = 0; i < 2; ++i) {
+            const int c = half + 2 * i, col0 = tn * BN + 64 * c;
+            if (c < BN / 64 && row0 < g.m && col0 < g.n) fetch((flip + i) & 1, col0);
+          }
+        }
+      }
       ok = wait_cluster(acc_full + 8 * buf, use & 1);
       if (!__all_sync(0xFFFFFFFFu, ok)) {
         ok = false;
+        for (int i = 0; ahead && i < 2; ++i)  // gave up: let the copies in flight land
+          mbar_wait(my_in + 8 * i, (in_phase >> i) & 1, 1 << 16);
         break;
       }
       tc_fence_after();
@@ -322,92 +407,80 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
         uint32_t v;
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n" : "=r"(v) : "r"(acc + BN));
         tmem_wait_ld();
-        if (row0 + lane < g.m) g.sums[(int64_t)tn * g.m + row0 + lane] = tn < kblocks ? __uint_as_float(v) : 0.f;
+        const int kb0 = part * g.per_split, kb1 = min(kblocks, kb0 + g.per_split);
+        const int mine = kb0 + ((tn - kb0) % g.tiles_n + g.tiles_n) % g.tiles_n;  // first block that this column tile summed
+        if (row0 + lane < g.m)
+          g.sums[((int64_t)part * g.tiles_n + tn) * g.m + row0 + lane] = mine < kb1 ? __uint_as_float(v) : 0.f;
       }
       for (int c = half; c < BN / 64; c += 2) {
         const int col0 = tn * BN + 64 * c;
         if (row0 >= g.m || col0 >= g.n) break;
+        if (g.splits > 1) {  // the float32 tile as it is, 32 columns a store
+          const int prow = part * g.tiles_m * 128 * CG + row0;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t r[32];
+            tmem_ld32(acc + 64 * c + 32 * h, r);
+            if (lane == 0) store_wait_read<1>();
+            __syncwarp();
+            tmem_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<uint4 *>(st + 4096 * h + chunk_at(lane, j)) =
+                  make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              store_box(&g.out, st_at + 4096 * h, col0 + 32 * h, prow);
+              store_commit();
+            }
+          }
+          continue;
+        }
         const int rows = min(32, g.m - row0), cols = min(64, g.n - col0);
-        // this chunk's staging tile: with a z to save the second one is z's
-        const int b = g.save_z ? 0 : (flip++ & 1);
+        const int b = g.save_z ? 0 : flip++ & 1;
         uint8_t *so = st + b * 4096;
         const uint32_t so_at = st_at + b * 4096;
-        if (lane == 0) {  // its last store has been read (one newer one may still be)
-          if (g.save_z || !g.out_tma) store_wait_read<0>();
-          else store_wait_read<1>();
-        }
-        __syncwarp();
-        if (g.in_kind) {
-          if (g.in_tma) {
-            if (lane == 0) {
-              fence_proxy_async_smem();
-              mbar_expect_tx(my_in, 4096);
-              load_box<1>(so_at, &g.in, col0, row0, my_in);
-            }
-            ok = mbar_wait(my_in, in_phase, kPolls);
-            in_phase ^= 1;
-            if (!__all_sync(0xFFFFFFFFu, ok)) {
-              ok = false;
-              break;
-            }
-          } else {
-            tile_in<T>(so, static_cast<const T *>(g.in_ptr) + row0 * g.ldi + col0, g.ldi, rows, cols, lane);
-            __syncwarp();
+        if (!ahead) {
+          if (lane == 0) {  // this staging tile's last store has been read (a newer one of the other may still be)
+            if (g.save_z) store_wait_read<0>();
+            else store_wait_read<1>();
+          }
+          __syncwarp();
+          if (in_tma && lane == 0) {
+            fence_proxy_async_smem();
+            fetch(b, col0);
           }
         }
-        if (bias) {
+        if (in_tma) {
+          ok = mbar_wait(my_in + 8 * b, (in_phase >> b) & 1, kPolls);
+          in_phase ^= 1u << b;
+          if (!__all_sync(0xFFFFFFFFu, ok)) {
+            ok = false;
+            break;
+          }
+        } else if (g.in_kind) {
+          tile_in<T>(so, static_cast<const T *>(g.in_ptr) + row0 * g.ldi + col0, g.ldi, rows, cols, lane);
+          __syncwarp();
+        }
+        if (g.bias) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int j = lane + 32 * h;
-            bs[j] = j < cols ? to_f<T>(bias[col0 + j]) : 0.f;
+            bs[j] = j < cols ? to_f<T>(static_cast<const T *>(g.bias)[col0 + j]) : 0.f;
           }
           __syncwarp();
         }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t r[32];
-          tmem_ld32(acc + 64 * c + 32 * h, r);
-          tmem_wait_ld();
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {  // 8 columns: one 16-byte chunk of the row
-            float v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[8 * u + j]);
-            if (bias) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) v[j] += bs[32 * h + 8 * u + j];
-            }
-            const uint32_t at = chunk_at(lane, 4 * h + u);
-            uint4 *slot = reinterpret_cast<uint4 *>(so + at);
-            if (g.save_z)
-              *reinterpret_cast<uint4 *>(st + 4096 + at) =
-                  make_uint4(P::pack(v[0], v[1]), P::pack(v[2], v[3]), P::pack(v[4], v[5]), P::pack(v[6], v[7]));
-            if (g.in_kind == kInActGrad) {
-              const uint4 zi = *slot;
-              const uint32_t w[4] = {zi.x, zi.y, zi.z, zi.w};
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const float2 z = P::unpack(w[j]);
-                v[2 * j] *= activate_grad(g.act, z.x);
-                v[2 * j + 1] *= activate_grad(g.act, z.y);
-              }
-            } else {
-              if (g.act != KDA_ACT_NONE) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = activate(g.act, v[j]);
-              }
-              if (g.in_kind == kInAdd) {
-                const uint4 ri = *slot;
-                const uint32_t w[4] = {ri.x, ri.y, ri.z, ri.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const float2 x = P::unpack(w[j]);
-                  v[2 * j] += x.x;
-                  v[2 * j + 1] += x.y;
-                }
-              }
-            }
-            *slot = make_uint4(P::pack(v[0], v[1]), P::pack(v[2], v[3]), P::pack(v[4], v[5]), P::pack(v[6], v[7]));
+        if constexpr (A_MN) {
+          chunk<T, kPlain, KDA_ACT_NONE>(g, acc + 64 * c, so, st + 4096, bs, lane);
+        } else {
+          constexpr int kind = B_MN ? kGrad : kForward;
+          switch (g.act) {
+            case KDA_ACT_RELU: chunk<T, kind, KDA_ACT_RELU>(g, acc + 64 * c, so, st + 4096, bs, lane); break;
+            case KDA_ACT_SILU: chunk<T, kind, KDA_ACT_SILU>(g, acc + 64 * c, so, st + 4096, bs, lane); break;
+            case KDA_ACT_GELU: chunk<T, kind, KDA_ACT_GELU>(g, acc + 64 * c, so, st + 4096, bs, lane); break;
+            case KDA_ACT_GELU_TANH: chunk<T, kind, KDA_ACT_GELU_TANH>(g, acc + 64 * c, so, st + 4096, bs, lane); break;
+            default: chunk<T, kind, KDA_ACT_NONE>(g, acc + 64 * c, so, st + 4096, bs, lane);
           }
         }
         fence_proxy_async_smem();
@@ -440,14 +513,150 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   if (warp == 2) dealloc<CG>(tmem, S::kCols);
 }
 
-// db[j] = sum over the partials, in their order
+// Adds the parts of a split product in their order and runs the epilogue; the blocks behind the
+// last row of blocks add the partial column sums.
+constexpr int kJoinRows = 4;  // rows a block of 64 x 4 threads takes; a thread takes 8 columns
 template <typename T>
-__global__ void __launch_bounds__(256) sums_kernel(const float *part, int parts, int m, T *db) {
-  const int j = blockIdx.x * 256 + threadIdx.x;
-  if (j >= m) return;
-  float s = 0.f;
-  for (int i = 0; i < parts; ++i) s += part[(int64_t)i * m + j];
-  db[j] = from_f<T>(s);
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args g, int64_t part_rows, int col_blocks,
+                                                   int64_t tile_blocks, int parts, T *db) {
+  using P = Pair<T>;
+  const int64_t blk = blockIdx.x;
+  if (blk >= tile_blocks) {  // db[j] = sum over the partials
+    const int64_t j = (blk - tile_blocks) * 256 + threadIdx.y * 64 + threadIdx.x;
+    if (j >= g.m) return;
+    float s = 0.f;
+    for (int i = 0; i < parts; ++i) s += g.sums[(int64_t)i * g.m + j];
+    db[j] = from_f<T>(s);
+    return;
+  }
+  const int64_t row = blk / col_blocks * kJoinRows + threadIdx.y;
+  const int col = (int)(blk % col_blocks) * 512 + threadIdx.x * 8;
+  if (row >= g.m || col >= g.n) return;
+  float v[8] = {};
+  for (int p = 0; p < g.splits; ++p) {  // whole vectors: the workspace's columns are padded to tiles
+    const float4 *src = reinterpret_cast<const float4 *>(g.part + (p * part_rows + row) * g.ldp + col);
+    const float4 a = src[0], b = src[1];
+    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+    v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+  }
+  const int k = min(8, g.n - col);
+  if (g.bias) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < k) v[j] += to_f<T>(static_cast<const T *>(g.bias)[col + j]);
+  }
+  if (g.save_z) {
+    T *z = static_cast<T *>(g.z_ptr) + row * g.ldz + col;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < k) z[j] = from_f<T>(v[j]);
+  }
+  float x[8];
+  if (g.in_kind) {
+    const T *in = static_cast<const T *>(g.in_ptr) + row * g.ldi + col;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = j < k ? to_f<T>(in[j]) : 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (g.in_kind == kInActGrad) v[j] *= activate_grad(g.act, x[j]);
+    else v[j] = activate(g.act, v[j]) + (g.in_kind == kInAdd ? x[j] : 0.f);
+  }
+  T *out = static_cast<T *>(g.out_ptr) + row * g.ldo + col;
+  if (k == 8 && g.out_tma) {
+    *reinterpret_cast<uint4 *>(out) = make_uint4(P::pack(v[0], v[1]), P::pack(v[2], v[3]), P::pack(v[4], v[5]), P::pack(v[6], v[7]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < k) out[j] = from_f<T>(v[j]);
+  }
+}
+
+// ---- a few rows: y = act(x W^T + bias) + residual with M <= 32 ----
+// The weights' bytes bound it: each is read once, straight into the fragments of m16n8k16 products
+// whose 16 rows are 16 outputs and whose 8 columns are 8 of x's rows.  k may be summed in any order, so
+// a lane's share of a product is 8 consecutive k (one 16-byte load of W, one of x) instead of
+// the layout's four pairs.  A CTA owns 16 outputs, its warps take k 64 at a time in turn, and their
+// sums meet in shared memory.
+template <typename T>
+__device__ __forceinline__ void mma_m16n8k16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// 8 elements of a row from column k on; columns past the end count as zero.  The load itself is
+// a whole aligned 16 bytes, whose first byte lies in the row, so it stays in its page.
+__device__ __forceinline__ uint4 load_k8(const void *row, int k, int K) {
+  if (k >= K) return make_uint4(0, 0, 0, 0);
+  uint4 u = __ldg(reinterpret_cast<const uint4 *>(static_cast<const char *>(row) + 2 * (int64_t)k));
+  const int left = K - k;
+  if (left < 8) {
+    uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] &= left > 2 * j + 1 ? 0xFFFFFFFFu : left > 2 * j ? 0xFFFFu : 0u;
+    u = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return u;
+}
+struct FewArgs {
+  const void *x, *w, *bias, *res;
+  void *y, *z;
+  int64_t ldx, ldw, ldr, ldy, ldz;
+  int m, n, k, act;
+};
+constexpr int kFewRows = 32;
+template <typename T, int MT, int WARPS>  // MT groups of 8 rows of x
+__global__ void __launch_bounds__(32 * WARPS) few_rows_kernel(const FewArgs a) {
+  __shared__ float red[WARPS][16][8 * MT + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const int n0 = blockIdx.x * 16;
+  const char *w0 = static_cast<const char *>(a.w) + 2 * a.ldw * min(n0 + g, a.n - 1);
+  const char *w1 = static_cast<const char *>(a.w) + 2 * a.ldw * min(n0 + g + 8, a.n - 1);
+  const char *xr[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) xr[t] = static_cast<const char *>(a.x) + 2 * a.ldx * min(8 * t + g, a.m - 1);
+  float d[MT][4] = {};
+  constexpr int U = 4;  // 32-k groups in flight: 64 k of this turn and of the next
+  for (int k0 = 64 * warp; k0 < a.k; k0 += 64 * WARPS * (U / 2)) {
+    uint4 p[U], q[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int k = k0 + (j >> 1) * 64 * WARPS + (j & 1) * 32 + 8 * c;
+      p[j] = load_k8(w0, k, a.k);
+      q[j] = load_k8(w1, k, a.k);
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int k = k0 + (j >> 1) * 64 * WARPS + (j & 1) * 32 + 8 * c;
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        const uint4 x = load_k8(xr[t], k, a.k);
+        mma_m16n8k16<T>(d[t], p[j].x, q[j].x, p[j].y, q[j].y, x.x, x.y);
+        mma_m16n8k16<T>(d[t], p[j].z, q[j].z, p[j].w, q[j].w, x.z, x.w);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) red[warp][g + 8 * (i >> 1)][8 * t + 2 * c + (i & 1)] = d[t][i];
+  __syncthreads();
+  for (int o = threadIdx.x; o < 16 * a.m; o += 32 * WARPS) {
+    const int j = o & 15, row = o >> 4, n = n0 + j;
+    if (n >= a.n) continue;
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) v += red[i][j][row];
+    if (a.bias) v += to_f<T>(static_cast<const T *>(a.bias)[n]);
+    if (a.z) static_cast<T *>(a.z)[row * a.ldz + n] = from_f<T>(v);
+    v = activate(a.act, v);
+    if (a.res) v += to_f<T>(static_cast<const T *>(a.res)[row * a.ldr + n]);
+    static_cast<T *>(a.y)[row * a.ldy + n] = from_f<T>(v);
+  }
 }
 
 // dz = dy act'(z) over a [rows][cols] matrix (z null: a copy), any strides and alignments
@@ -476,25 +685,64 @@ static int device_sms() {
   return n;
 }
 
+// ---- which tiles, and into how many parts k is split ----
+struct Plan {
+  int cg, bn, splits, per_split;
+};
+static Plan plan_for(int64_t m, int64_t n, int64_t k, int sms, bool may_split) {
+  struct Tile {
+    int cg, bn;
+    double busy, alone, kb;  // us a block of 64 k where the GPU is full, and where it is not; KB it reads
+  };
+  static const Tile tiles[] = {{2, 256, 0.40, 0.30, 64}, {1, 128, 0.40, 0.20, 32}, {1, 64, 0.31, 0.16, 24}};
+  const int64_t blocks = (k + kBlockK - 1) / kBlockK;
+  Plan best = {};
+  double best_us = 1e300;
+  for (const Tile &t : tiles) {
+    const int64_t count = ((m + 128 * t.cg - 1) / (128 * t.cg)) * ((n + t.bn - 1) / t.bn), units = sms / t.cg;
+    for (int64_t s = 1; s <= (may_split ? 16 : 1); ++s) {
+      const int64_t per = (blocks + s - 1) / s, parts = (blocks + per - 1) / per;
+      if (parts != s || (s > 1 && per < 4)) continue;
+      const int64_t waves = (count * s + units - 1) / units;
+      const double load = (double)(count * s < units ? count * s : units) / units;
+      const double per_block = t.alone + (t.busy - t.alone) * load;
+      double us = waves * per * per_block + 2.0 * t.bn / 256;
+      if (s > 1) us += 3.0 + (double)m * n * (4.0 * s * 2 + 2) * 1e-6 / 7.0;
+      if (us < best_us) {
+        best_us = us;
+        best = {t.cg, t.bn, (int)s, (int)per};
+      }
+    }
+  }
+  return best;
+}
+static int64_t part_rows(const Plan &p, int64_t m) { return (m + 128 * p.cg - 1) / (128 * p.cg) * (128 * p.cg); }
+static int64_t part_cols(const Plan &p, int64_t n) { return (n + p.bn - 1) / p.bn * p.bn; }
+static size_t part_bytes(const Plan &p, int64_t m, int64_t n) {
+  return p.splits > 1 ? (size_t)p.splits * part_rows(p, m) * part_cols(p, n) * sizeof(float) : 0;
+}
+static size_t sums_bytes(const Plan &p, int64_t m, int64_t n) {
+  return ((size_t)p.splits * ((n + p.bn - 1) / p.bn) * m * sizeof(float) + 15) / 16 * 16;
+}
+
 template <typename T, int CG, int BN, bool A_MN, bool B_MN, bool ONES>
 static int launch(Args &g, int sms, cudaStream_t st) {
   using S = Shape<CG, BN, ONES>;
   auto kernel = gemm_kernel<T, CG, BN, A_MN, B_MN, ONES>;
   g.tiles_m = (g.m + 128 * CG - 1) / (128 * CG);
   g.tiles_n = (g.n + BN - 1) / BN;
-  constexpr uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+  constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
   auto idesc = [&](int n, bool b_mn) {
     return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)A_MN << 15) | ((uint32_t)b_mn << 16) |
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
   };
   g.idesc = idesc(BN, B_MN);
   g.idesc_ones = idesc(kOnesN, false);
-  const cudaError_t a = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-  if (a != cudaSuccess) return KDA_ERR_CUDA;
-  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n, units = sms / CG;
-  if (tiles > (1ll << 30)) return KDA_ERR_UNSUPPORTED;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess) return KDA_ERR_CUDA;
+  const int64_t count = (int64_t)g.tiles_m * g.tiles_n * g.splits, units = sms / CG;
+  if (count > (1ll << 30)) return KDA_ERR_UNSUPPORTED;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((tiles < units ? tiles : units) * CG));
+  cfg.gridDim = dim3((unsigned)((count < units ? count : units) * CG));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = st;
@@ -510,25 +758,53 @@ static int launch(Args &g, int sms, cudaStream_t st) {
   return KDA_OK;
 }
 
-// The tile shape.  A pair of CTAs on 256 x 256 reads the least shared memory per product and is
-// taken where its tiles fill the GPU; smaller products take smaller tiles so that more SMs work.
-template <int BN, int CG>
-static int64_t tiles_of(int64_t m, int64_t n) {
-  return ((m + 128 * CG - 1) / (128 * CG)) * ((n + BN - 1) / BN);
-}
+// One product: the tiles (and parts), then whatever of parts and column sums is left to add.
 template <typename T, bool A_MN, bool B_MN, bool ONES>
-static int dispatch(Args &g, const void *a, int64_t lda, const void *b, int64_t ldb, cudaStream_t st) {
-  const int sms = device_sms();
-  if (!sms) return KDA_ERR_CUDA;
-  int cg = 1, bn = 64;
-  if (tiles_of<256, 2>(g.m, g.n) * 4 >= sms / 2 * 3) cg = 2, bn = 256;
-  else if (tiles_of<128, 1>(g.m, g.n) * 4 >= sms * 3) bn = 128;
+static int run(Args &g, const Plan &p, const void *a, int64_t lda, const void *b, int64_t ldb, void *ws, void *db, int sms,
+               cudaStream_t st) {
   int s;
   if ((s = A_MN ? tma_map_rows16(&g.a, a, g.k, g.m, lda, 64) : tma_map_rows16(&g.a, a, g.m, g.k, lda, 128))) return s;
-  if ((s = B_MN ? tma_map_rows16(&g.b, b, g.k, g.n, ldb, 64) : tma_map_rows16(&g.b, b, g.n, g.k, ldb, bn / cg))) return s;
-  if (cg == 2) return launch<T, 2, 256, A_MN, B_MN, ONES>(g, sms, st);
-  if (bn == 128) return launch<T, 1, 128, A_MN, B_MN, ONES>(g, sms, st);
-  return launch<T, 1, 64, A_MN, B_MN, ONES>(g, sms, st);
+  if ((s = B_MN ? tma_map_rows16(&g.b, b, g.k, g.n, ldb, 64) : tma_map_rows16(&g.b, b, g.n, g.k, ldb, p.bn / p.cg))) return s;
+  g.splits = p.splits;
+  g.per_split = p.per_split;
+  char *at = static_cast<char *>(ws);
+  if (ONES) {
+    g.sums = reinterpret_cast<float *>(at);
+    at += sums_bytes(p, g.m, g.n);
+  }
+  const int64_t rows = part_rows(p, g.m);
+  if (p.splits > 1) {
+    g.part = reinterpret_cast<float *>(at);
+    g.ldp = part_cols(p, g.n);
+    if ((s = tma_map_rows32(&g.out, at, p.splits * rows, g.ldp, g.ldp, 32))) return s;
+  }
+  s = p.cg == 2    ? launch<T, 2, 256, A_MN, B_MN, ONES>(g, sms, st)
+      : p.bn == 128 ? launch<T, 1, 128, A_MN, B_MN, ONES>(g, sms, st)
+                    : launch<T, 1, 64, A_MN, B_MN, ONES>(g, sms, st);
+  if (s || (p.splits == 1 && !ONES)) return s;
+  const int col_blocks = (g.n + 511) / 512;
+  const int64_t tile_blocks = p.splits > 1 ? (int64_t)((g.m + kJoinRows - 1) / kJoinRows) * col_blocks : 0;
+  const int64_t blocks = tile_blocks + (ONES ? (g.m + 255) / 256 : 0);
+  join_kernel<T><<<(unsigned)blocks, dim3(64, 4), 0, st>>>(g, rows, col_blocks, tile_blocks, p.splits * g.tiles_n,
+                                                           static_cast<T *>(db));
+  if (cudaGetLastError() != cudaSuccess) return KDA_ERR_CUDA;
+  count_launch();
+  return KDA_OK;
+}
+
+template <typename T, int MT>
+static int few_rows(const FewArgs &a, int sms, cudaStream_t st) {
+  const int grid = (a.n + 15) / 16;
+  // twice the warps where the outputs alone do not fill the GPU (and k has turns for them)
+  if (grid < 2 * sms && a.k > 512) few_rows_kernel<T, MT, 16><<<grid, 512, 0, st>>>(a);
+  else few_rows_kernel<T, MT, 8><<<grid, 256, 0, st>>>(a);
+  if (cudaGetLastError() != cudaSuccess) return KDA_ERR_CUDA;
+  count_launch();
+  return KDA_OK;
+}
+template <typename T>
+static int few_rows(const FewArgs &a, int sms, cudaStream_t st) {
+  return a.m <= 8 ? few_rows<T, 1>(a, sms, st) : a.m <= 16 ? few_rows<T, 2>(a, sms, st) : few_rows<T, 4>(a, sms, st);
 }
 
 static int set_out(Args &g, void *p, int64_t ld) {
@@ -559,6 +835,13 @@ static bool even(std::initializer_list<const void *> ps) {
   return true;
 }
 
+// The plan for a product, and whether the workspace holds it; without one k is not split.
+static int plan_in(Plan &p, int64_t m, int64_t n, int64_t k, int sms, bool sums, const void *ws, size_t ws_bytes) {
+  p = plan_for(m, n, k, sms, ws != nullptr);
+  const size_t need = part_bytes(p, m, n) + (sums ? sums_bytes(p, m, n) : 0);
+  return need && (!ws || (uintptr_t)ws % 16 || ws_bytes < need) ? KDA_ERR_WORKSPACE : KDA_OK;
+}
+
 int device_status(bool reset) {
   int v = 0;
   const int zero = 0;
@@ -576,9 +859,20 @@ using namespace kda::linear;
 
 extern "C" {
 
+size_t kda_linear_workspace_bytes(int op, int64_t M, int64_t N, int64_t K, int with_db) {
+  if (check(KDA_BF16, KDA_ACT_NONE, M, N, K)) return 0;
+  int sms = device_sms();
+  if (!sms) sms = 148;  // no device: the size on a B200
+  if (op == KDA_LINEAR_FWD) return M <= kFewRows ? 0 : part_bytes(plan_for(M, N, K, sms, true), M, N);
+  if (op == KDA_LINEAR_DGRAD) return part_bytes(plan_for(M, K, N, sms, true), M, K);
+  if (op != KDA_LINEAR_WGRAD) return 0;
+  const Plan p = plan_for(N, K, M, sms, true);
+  return part_bytes(p, N, K) + (with_db ? sums_bytes(p, N, K) : 0);
+}
+
 int kda_linear_fwd(int dtype, int act, int64_t M, int64_t N, int64_t K, const void *x, int64_t ldx, const void *w,
                    int64_t ldw, const void *bias, const void *residual, int64_t ldr, void *y, int64_t ldy, void *z,
-                   int64_t ldz, void *stream) {
+                   int64_t ldz, void *ws, size_t ws_bytes, void *stream) {
   int s = check(dtype, act, M, N, K);
   if (s) return s;
   if (!x || !w || !y || !ld_ok(ldx, K) || !ld_ok(ldw, K) || !ld_ok(ldy, N) || (residual && !ld_ok(ldr, N)) ||
@@ -586,39 +880,49 @@ int kda_linear_fwd(int dtype, int act, int64_t M, int64_t N, int64_t K, const vo
     return KDA_ERR_INVALID_ARG;
   if (!tma_able(x, ldx) || !tma_able(w, ldw) || (z && !tma_able(z, ldz)) || !even({bias, residual, y}))
     return KDA_ERR_MISALIGNED;
+  const int sms = device_sms();
+  if (!sms) return KDA_ERR_CUDA;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (M <= kFewRows) {
+    const FewArgs a = {x, w, bias, residual, y, z, ldx, ldw, ldr, ldy, ldz, (int)M, (int)N, (int)K, act};
+    return dtype == KDA_BF16 ? few_rows<__nv_bfloat16>(a, sms, st) : few_rows<__half>(a, sms, st);
+  }
+  Plan p;
+  if ((s = plan_in(p, M, N, K, sms, 0, ws, ws_bytes))) return s;
   Args g = {};
   g.m = (int)M; g.n = (int)N; g.k = (int)K; g.act = act; g.bias = bias;
   if ((s = set_out(g, y, ldy))) return s;
   if (residual && (s = set_in(g, kInAdd, residual, ldr))) return s;
   if (z) {
     g.save_z = 1;
+    g.z_ptr = z;
+    g.ldz = ldz;
     if ((s = kda::tma_map_rows16(&g.z, z, M, N, ldz, 32))) return s;
   }
-  cudaStream_t st = (cudaStream_t)stream;
-  return dtype == KDA_BF16 ? dispatch<__nv_bfloat16, false, false, false>(g, x, ldx, w, ldw, st)
-                           : dispatch<__half, false, false, false>(g, x, ldx, w, ldw, st);
+  return dtype == KDA_BF16 ? run<__nv_bfloat16, false, false, false>(g, p, x, ldx, w, ldw, ws, nullptr, sms, st)
+                           : run<__half, false, false, false>(g, p, x, ldx, w, ldw, ws, nullptr, sms, st);
 }
 
 int kda_linear_dgrad(int dtype, int act, int64_t M, int64_t N, int64_t K, const void *dz, int64_t ldd, const void *w,
-                     int64_t ldw, const void *z, int64_t ldz, void *dx, int64_t ldx, void *stream) {
+                     int64_t ldw, const void *z, int64_t ldz, void *dx, int64_t ldx, void *ws, size_t ws_bytes,
+                     void *stream) {
   int s = check(dtype, act, M, N, K);
   if (s) return s;
   if (!dz || !w || !dx || !ld_ok(ldd, N) || !ld_ok(ldw, K) || !ld_ok(ldx, K) || (z && !ld_ok(ldz, K)) ||
       (act != KDA_ACT_NONE && !z))
     return KDA_ERR_INVALID_ARG;
   if (!tma_able(dz, ldd) || !tma_able(w, ldw) || !even({z, dx})) return KDA_ERR_MISALIGNED;
+  const int sms = device_sms();
+  if (!sms) return KDA_ERR_CUDA;
+  Plan p;
+  if ((s = plan_in(p, M, K, N, sms, 0, ws, ws_bytes))) return s;
   Args g = {};
   g.m = (int)M; g.n = (int)K; g.k = (int)N; g.act = act;
   if ((s = set_out(g, dx, ldx))) return s;
   if (act != KDA_ACT_NONE && (s = set_in(g, kInActGrad, z, ldz))) return s;
   cudaStream_t st = (cudaStream_t)stream;
-  return dtype == KDA_BF16 ? dispatch<__nv_bfloat16, false, true, false>(g, dz, ldd, w, ldw, st)
-                           : dispatch<__half, false, true, false>(g, dz, ldd, w, ldw, st);
-}
-
-size_t kda_linear_wgrad_workspace_bytes(int64_t M, int64_t N, int64_t K, int with_db) {
-  if (!with_db || check(KDA_BF16, KDA_ACT_NONE, M, N, K)) return 0;
-  return (size_t)((K + 63) / 64) * N * sizeof(float);
+  return dtype == KDA_BF16 ? run<__nv_bfloat16, false, true, false>(g, p, dz, ldd, w, ldw, ws, nullptr, sms, st)
+                           : run<__half, false, true, false>(g, p, dz, ldd, w, ldw, ws, nullptr, sms, st);
 }
 
 int kda_linear_wgrad(int dtype, int64_t M, int64_t N, int64_t K, const void *dz, int64_t ldd, const void *x, int64_t ldx,
@@ -627,25 +931,20 @@ int kda_linear_wgrad(int dtype, int64_t M, int64_t N, int64_t K, const void *dz,
   if (s) return s;
   if (!dz || !x || !dw || !ld_ok(ldd, N) || !ld_ok(ldx, K) || !ld_ok(ldw, K)) return KDA_ERR_INVALID_ARG;
   if (!tma_able(dz, ldd) || !tma_able(x, ldx) || !even({dw, db})) return KDA_ERR_MISALIGNED;
-  if (db && (!ws || (uintptr_t)ws % 16 || ws_bytes < kda_linear_wgrad_workspace_bytes(M, N, K, 1)))
-    return KDA_ERR_WORKSPACE;
+  const int sms = device_sms();
+  if (db && !ws) return KDA_ERR_WORKSPACE;
+  if (!sms) return KDA_ERR_CUDA;
+  Plan p;
+  if ((s = plan_in(p, N, K, M, sms, db != nullptr, ws, ws_bytes))) return s;
   Args g = {};
   g.m = (int)N; g.n = (int)K; g.k = (int)M;
   if ((s = set_out(g, dw, ldw))) return s;
   cudaStream_t st = (cudaStream_t)stream;
-  g.sums = static_cast<float *>(ws);
-  if (!db)
-    return dtype == KDA_BF16 ? dispatch<__nv_bfloat16, true, true, false>(g, dz, ldd, x, ldx, st)
-                             : dispatch<__half, true, true, false>(g, dz, ldd, x, ldx, st);
-  s = dtype == KDA_BF16 ? dispatch<__nv_bfloat16, true, true, true>(g, dz, ldd, x, ldx, st)
-                        : dispatch<__half, true, true, true>(g, dz, ldd, x, ldx, st);
-  if (s) return s;
-  const unsigned grid = (unsigned)((N + 255) / 256);
-  if (dtype == KDA_BF16) sums_kernel<<<grid, 256, 0, st>>>(g.sums, g.tiles_n, (int)N, static_cast<__nv_bfloat16 *>(db));
-  else sums_kernel<<<grid, 256, 0, st>>>(g.sums, g.tiles_n, (int)N, static_cast<__half *>(db));
-  if (cudaGetLastError() != cudaSuccess) return KDA_ERR_CUDA;
-  kda::count_launch();
-  return KDA_OK;
+  if (db)
+    return dtype == KDA_BF16 ? run<__nv_bfloat16, true, true, true>(g, p, dz, ldd, x, ldx, ws, db, sms, st)
+                             : run<__half, true, true, true>(g, p, dz, ldd, x, ldx, ws, db, sms, st);
+  return dtype == KDA_BF16 ? run<__nv_bfloat16, true, true, false>(g, p, dz, ldd, x, ldx, ws, db, sms, st)
+                           : run<__half, true, true, false>(g, p, dz, ldd, x, ldx, ws, db, sms, st);
 }
 
 int kda_act_grad(int dtype, int act, int64_t rows, int64_t cols, const void *dy, int64_t ldy, const void *z, int64_t ldz,

@@ -96,18 +96,25 @@ int tma_map_bthd(CUtensorMap *map, const void *base, int64_t B, int64_t T, int64
   return r == CUDA_SUCCESS ? KDA_OK : KDA_ERR_INVALID_ARG;
 }
 
-int tma_map_rows16(CUtensorMap *map, const void *base, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+static int map_rows(CUtensorMap *map, const void *base, int64_t rows, int64_t cols, int64_t ld, int box_rows, int es) {
   PFN_cuTensorMapEncodeTiled fn = encode_fn();
   if (!fn || !ensure_context()) return KDA_ERR_CUDA;
-  if ((uintptr_t)base % 16 || (ld * 2) % 16) return KDA_ERR_MISALIGNED;
+  if ((uintptr_t)base % 16 || (ld * es) % 16) return KDA_ERR_MISALIGNED;
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)(ld * 2)};
-  const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(ld * es)};
+  const cuuint32_t box[2] = {(cuuint32_t)(128 / es), (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(base), dims, strides, box, estr,
+  const CUresult r = fn(map, es == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void *>(base), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? KDA_OK : KDA_ERR_INVALID_ARG;
+}
+
+int tma_map_rows16(CUtensorMap *map, const void *base, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+  return map_rows(map, base, rows, cols, ld, box_rows, 2);
+}
+int tma_map_rows32(CUtensorMap *map, const void *base, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+  return map_rows(map, base, rows, cols, ld, box_rows, 4);
 }
 
 }  // namespace kda

@@ -30,6 +30,8 @@ int tma_map_bthd(CUtensorMap *map, const void *base, int64_t B, int64_t T, int64
 // row) with a box of box_rows x 64 columns, 128-byte swizzle.  KDA_ERR_MISALIGNED unless base and
 // row pitch are multiples of 16 bytes.
 int tma_map_rows16(CUtensorMap *map, const void *base, int64_t rows, int64_t cols, int64_t ld, int box_rows);
+// The same for float32 elements, a box of box_rows x 32 columns.
+int tma_map_rows32(CUtensorMap *map, const void *base, int64_t rows, int64_t cols, int64_t ld, int box_rows);
 
 // x: first column of the box (a multiple of 64 for bf16, of 32 for fp32)
 __device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap *map, int h, int t0, int b,

@@ -241,24 +241,32 @@ Tensor readable(const Tensor &t) {
   act_grad(KDA_ACT_NONE, t, Tensor(), out);
   return out;
 }
+struct Workspace {
+  Tensor t;
+  size_t n;
+  Workspace(int op, int64_t m, int64_t n_, int64_t k, bool db, const Tensor &like) : n(kda_linear_workspace_bytes(op, m, n_, k, db)) {
+    if (n) t = at::empty({(int64_t)n}, like.options().dtype(at::kByte));
+  }
+};
 void product(int act, const Tensor &x, const Tensor &w, const Tensor &b, const Tensor &r, const Tensor &y, const Tensor &z) {
+  const Workspace ws(KDA_LINEAR_FWD, x.size(0), w.size(0), w.size(1), false, x);
   done(kda_linear_fwd(dtype_of(x), act, x.size(0), w.size(0), w.size(1), ptr(x), pitch(x), ptr(w), pitch(w), ptr(b),
-                      ptr(r), pitch(r), ptr(y), pitch(y), ptr(z), pitch(z), stream()),
+                      ptr(r), pitch(r), ptr(y), pitch(y), ptr(z), pitch(z), ptr(ws.t), ws.n, stream()),
        "kda_linear_fwd");
 }
 void dgrad(int act, const Tensor &dz, const Tensor &w, const Tensor &z, const Tensor &dx) {
+  const Workspace ws(KDA_LINEAR_DGRAD, dz.size(0), w.size(0), w.size(1), false, dz);
   done(kda_linear_dgrad(dtype_of(dz), act, dz.size(0), w.size(0), w.size(1), ptr(dz), pitch(dz), ptr(w), pitch(w), ptr(z),
-                        pitch(z), ptr(dx), pitch(dx), stream()),
+                        pitch(z), ptr(dx), pitch(dx), ptr(ws.t), ws.n, stream()),
        "kda_linear_dgrad");
 }
 void wgrad(const Tensor &dz, const Tensor &x, bool want_db, Tensor &dw, Tensor &db) {
   const int64_t m = dz.size(0), n = dz.size(1), k = x.size(1);
   dw = at::empty({n, k}, x.options());
   if (want_db) db = at::empty({n}, x.options());
-  const size_t nws = kda_linear_wgrad_workspace_bytes(m, n, k, want_db);
-  Tensor ws;
-  if (nws) ws = at::empty({(int64_t)nws}, x.options().dtype(at::kByte));
-  done(kda_linear_wgrad(dtype_of(x), m, n, k, ptr(dz), pitch(dz), ptr(x), pitch(x), ptr(dw), k, ptr(db), ptr(ws), nws, stream()),
+  const Workspace ws(KDA_LINEAR_WGRAD, m, n, k, want_db, x);
+  done(kda_linear_wgrad(dtype_of(x), m, n, k, ptr(dz), pitch(dz), ptr(x), pitch(x), ptr(dw), k, ptr(db), ptr(ws.t), ws.n,
+                        stream()),
        "kda_linear_wgrad");
 }
 std::vector<int64_t> with_last(const Tensor &x, int64_t n) {

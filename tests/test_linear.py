@@ -25,7 +25,7 @@ A = 1 << 20
 
 def fwd(**kw):
     a = dict(dtype=_lib.KDA_BF16, act=0, M=4, N=8, K=16, x=A, ldx=16, w=A, ldw=16, b=None, r=None, ldr=0, y=A, ldy=8, z=None,
-             ldz=0, st=None)
+             ldz=0, ws=None, nws=0, st=None)
     a.update(kw)
     return _lib.STATUS[_lib.lib().kda_linear_fwd(*a.values())]
 
@@ -45,10 +45,15 @@ def test_backward_refusals():
     L, n = _lib.lib(), ctypes.c_void_p(None)
     st = lambda s: _lib.STATUS[s].replace("KDA_ERR_", "")  # noqa: E731
     bf = _lib.KDA_BF16
-    assert st(L.kda_linear_dgrad(bf, 3, 4, 8, 16, A, 8, A, 16, n, 0, A, 16, n)) == "INVALID_ARG"  # no z
-    assert st(L.kda_linear_dgrad(bf, 0, 4, 8, 16, A, 12, A, 16, n, 0, A, 16, n)) == "MISALIGNED"
+    assert st(L.kda_linear_dgrad(bf, 3, 4, 8, 16, A, 8, A, 16, n, 0, A, 16, n, 0, n)) == "INVALID_ARG"  # no z
+    assert st(L.kda_linear_dgrad(bf, 0, 4, 8, 16, A, 12, A, 16, n, 0, A, 16, n, 0, n)) == "MISALIGNED"
     assert st(L.kda_linear_wgrad(bf, 4, 8, 16, A, 8, A, 16, A, 16, A, n, 0, n)) == "WORKSPACE"
     assert st(L.kda_linear_wgrad(bf, 4, 8, 16, A, 8, A, 16, A, 15, n, n, 0, n)) == "INVALID_ARG"
-    assert L.kda_linear_wgrad_workspace_bytes(4, 8, 16, 1) >= 8 * 4 and L.kda_linear_wgrad_workspace_bytes(0, 8, 16, 1) == 0
+    for op in (_lib.KDA_LINEAR_FWD, _lib.KDA_LINEAR_DGRAD, _lib.KDA_LINEAR_WGRAD):
+        assert L.kda_linear_workspace_bytes(op, 0, 8, 16, 1) == 0
+        assert L.kda_linear_workspace_bytes(op, 1000, 8, 1 << 20, 1) >= 0
+    assert L.kda_linear_workspace_bytes(_lib.KDA_LINEAR_WGRAD, 4, 8, 16, 1) >= 8 * 4
+    assert L.kda_linear_workspace_bytes(_lib.KDA_LINEAR_WGRAD, 12544, 2304, 768, 0) > 2304 * 768 * 4  # split
+    assert L.kda_linear_workspace_bytes(7, 4, 8, 16, 1) == 0
     assert st(L.kda_act_grad(bf, 1, 4, 8, A, 8, n, 0, A, 8, n)) == "INVALID_ARG"
     assert st(L.kda_act_grad(bf, 0, 4, 8, A + 1, 8, n, 0, A, 8, n)) == "MISALIGNED"

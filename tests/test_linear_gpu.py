@@ -121,6 +121,29 @@ def test_large_tiles(cuda, m, n, k):
     check_linear(m, n, k, "bf16", "gelu", True, True)
 
 
+@pytest.mark.parametrize("m,n,k,act", [(300, 200, 5000, "gelu"), (200, 6000, 100, "silu"), (20000, 130, 200, "none"),
+                                       (9000, 700, 260, "gelu_tanh"), (40, 33, 9001, "relu"), (333, 1027, 3001, "none")])
+def test_split_sums(cuda, m, n, k, act):
+    """Long sums over few tiles: k in parts, joined with every epilogue, in each of the three products."""
+    check_linear(m, n, k, "bf16", act, True, True, seed=4)
+    check_linear(m, n, k, "fp16", act, False, False, seed=5, pad=8)
+
+
+def test_unsplit_without_workspace(cuda):
+    g = gen(15)
+    x, w = rnd(g, 200, 4096, dt=torch.bfloat16), rnd(g, 72, 4096, dt=torch.bfloat16, scale=0.02)
+    L = _lib.lib()
+    assert L.kda_linear_workspace_bytes(_lib.KDA_LINEAR_FWD, 200, 72, 4096, 0) > 0
+    y = torch.empty(200, 72, dtype=torch.bfloat16, device=cuda)
+    args = (_lib.KDA_BF16, 0, 200, 72, 4096, x.data_ptr(), 4096, w.data_ptr(), 4096, None, None, 0, y.data_ptr(), 72, None, 0)
+    s = torch.cuda.current_stream().cuda_stream
+    _lib.check(L.kda_linear_fwd(*args, None, 0, s), "fwd")
+    want, e = product(x.double(), w.double())
+    near(y, want, e + 2.0 ** -8 * want.abs() * 1.01, "y")
+    ws = torch.empty(64, dtype=torch.uint8, device=cuda)
+    assert _lib.STATUS[L.kda_linear_fwd(*args, ws.data_ptr(), 64, s)] == "KDA_ERR_WORKSPACE"
+
+
 def test_wgrad_large_tiles(cuda):
     check_linear(300, 2600, 4200, "bf16", "none", True, False)
 
@@ -274,7 +297,7 @@ def test_rows_behind_the_last_are_left_alone(cuda):
         buf = torch.full((80, n), 7.0, dtype=torch.bfloat16, device=cuda)
         L = _lib.lib()
         _lib.check(L.kda_linear_fwd(_lib.KDA_BF16, 0, 70, n, 64, x.data_ptr(), 64, w.data_ptr(), 64, None, None, 0,
-                                    buf.data_ptr(), n, None, 0, torch.cuda.current_stream().cuda_stream), "fwd")
+                                    buf.data_ptr(), n, None, 0, None, 0, torch.cuda.current_stream().cuda_stream), "fwd")
         assert (buf[70:] == 7).all() and torch.equal(buf[:70], linear_act(x, w))
 
 
