@@ -82,16 +82,7 @@ __device__ __forceinline__ void cluster_sync() {
 __device__ __forceinline__ void arrive_cluster(uint32_t addr) {  // addr: a shared::cluster address
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" :: "r"(addr) : "memory");
 }
-__device__ __forceinline__ bool wait_cluster(uint32_t mbar, uint32_t parity) {  // bounded, as mbar_wait
-  for (int i = 0; i < kPolls; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok) : "r"(mbar), "r"(parity) : "memory");
-    if (ok) return true;
-  }
-  return false;
-}
+__device__ __forceinline__ bool wait(uint32_t mbar, uint32_t parity) { return mbar_wait(mbar, parity, kPolls); }
 
 template <int CG>
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t mbar) {
@@ -112,14 +103,35 @@ __device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.com
 template <int N>
 __device__ __forceinline__ void store_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;\n" :: "n"(N) : "memory"); }
 
+// One thread of a converged warp.  The copying and the issuing warp run their loops whole and elect a
+// thread for each instruction: its operands stay warp-uniform, in uniform registers.  (A loop
+// inside `if (lane == 0)` moved every operand there first: 0.33 us for a block of 64 k at the least,
+// whatever the tile.)
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+// The low words of umma_desc(): start address and leading offset; kDescHigh: stride 1024, version,
+// 128-byte swizzle.  A K step is 32 bytes further (K-major) or 16 rows (MN-major).
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+template <bool MN>
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr) { return (saddr >> 4) | ((MN ? 8192u >> 4 : 1u) << 16); }
+template <bool MN>
+constexpr uint32_t kDescStep = MN ? 2048 >> 4 : 32 >> 4;
+
 template <int CG>
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  if constexpr (CG == 1) tc_mma(d, a, b, idesc, accumulate);
+__device__ __forceinline__ void mma(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b64 a, b;\n mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}\n"
+        :: "r"(d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(kDescHigh) : "memory");
   else
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
-        :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+        "{\n .reg .pred p;\n .reg .b64 a, b;\n mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, p;\n}\n"
+        :: "r"(d), "r"(a_low), "r"(b_low), "r"(idesc), "r"(accumulate), "r"(kDescHigh) : "memory");
 }
 template <int CG>
 __device__ __forceinline__ void commit(uint32_t mbar) {  // to the barrier at this offset in every CTA of the pair
@@ -297,19 +309,18 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   bool ok = true;
 
   if (warp == 0) {
-    if (lane == 0) {
-      // ---- operand copies; both CTAs' bytes of a stage arrive on the first CTA's barrier ----
-      const uint32_t full_lead = CG == 2 ? map_rank(full, 0) : full;
-      uint32_t it = 0;
-      for (int u = first; ok && u < units; u += step) {
-        const int t = u % tiles, kb0 = u / tiles * g.per_split, kb1 = min(kblocks, kb0 + g.per_split);
-        const int m0 = (t / g.tiles_n) * 128 * CG + (int)rank * 128;
-        const int n0 = (t % g.tiles_n) * BN + (int)rank * (BN / CG);
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const uint32_t s = it % S::kStages, ph = (it / S::kStages) & 1;
-          if (!(ok = wait_cluster(empty + 8 * s, ph ^ 1))) break;
+    // ---- operand copies; both CTAs' bytes of a stage arrive on the first CTA's barrier ----
+    const uint32_t full_lead = CG == 2 ? map_rank(full, 0) : full;
+    uint32_t s = 0, ph = 1, issued = 0;
+    for (int u = first; ok && u < units; u += step) {
+      const int t = u % tiles, kb0 = u / tiles * g.per_split, kb1 = min(kblocks, kb0 + g.per_split);
+      const int m0 = (t / g.tiles_n) * 128 * CG + (int)rank * 128;
+      const int n0 = (t % g.tiles_n) * BN + (int)rank * (BN / CG);
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!(ok = wait(empty + 8 * s, ph))) break;
+        const uint32_t at = base + s * S::kStage, bt = at + kStageA, fb = full_lead + 8 * s;
+        if (elect()) {
           if (rank == 0) mbar_expect_tx(full + 8 * s, S::kStage * CG);
-          const uint32_t at = base + s * S::kStage, bt = at + kStageA, fb = full_lead + 8 * s;
           if (A_MN) {
             load_box<CG>(at, &g.a, m0, kb * kBlockK, fb);
             load_box<CG>(at + 8192, &g.a, m0 + 64, kb * kBlockK, fb);
@@ -324,46 +335,51 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
             load_box<CG>(bt, &g.b, kb * kBlockK, n0, fb);
           }
         }
+        __syncwarp();
+        ++issued;
+        if (++s == S::kStages) s = 0, ph ^= 1;
       }
-      if (!ok && rank == 0)  // gave up: let the copies in flight land before the CTA ends
-        for (uint32_t i = it > S::kStages ? it - S::kStages : 0; i < it; ++i)
-          mbar_wait(full + 8 * (i % S::kStages), (i / S::kStages) & 1, 1 << 16);
     }
-    __syncwarp();
+    if (!ok && rank == 0)  // gave up: let the copies in flight land before the CTA ends
+      for (uint32_t i = issued > S::kStages ? issued - S::kStages : 0; i < issued; ++i)
+        mbar_wait(full + 8 * (i % S::kStages), (i / S::kStages) & 1, 1 << 16);
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       // ---- products ----
-      uint32_t it = 0, n = 0;
+      const uint32_t a_low = desc_low<A_MN>(base), b_low = desc_low<B_MN>(base + kStageA);
+      const uint32_t ones_low = desc_low<false>(smem_u32(ones));
+      uint32_t s = 0, ph = 0, n = 0;
       for (int u = first; ok && u < units; u += step, ++n) {
         const int t = u % tiles, kb0 = u / tiles * g.per_split, kb1 = min(kblocks, kb0 + g.per_split);
         const uint32_t buf = n % S::kBufs, use = n / S::kBufs;
         const uint32_t d = tmem + buf * S::kAcc;
-        if (!(ok = wait_cluster(acc_empty + 8 * buf, (use & 1) ^ 1))) break;
+        if (!(ok = wait(acc_empty + 8 * buf, (use & 1) ^ 1))) break;
         tc_fence_after();
         const int tn = t % g.tiles_n;
         bool summed = false;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const uint32_t s = it % S::kStages, ph = (it / S::kStages) & 1;
-          if (!(ok = wait_cluster(full + 8 * s, ph))) break;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!(ok = wait(full + 8 * s, ph))) break;
           tc_fence_after();
-          const uint32_t at = base + s * S::kStage, bt = at + kStageA;
-#pragma unroll
-          for (int k = 0; k < kBlockK / 16; ++k)
-            mma<CG>(d, A_MN ? desc_mn(at, k) : desc_k(at, k), B_MN ? desc_mn(bt, k) : desc_k(bt, k), g.idesc,
-                    kb > kb0 || k > 0);
-          if (ONES && kb % g.tiles_n == tn) {  // the column sums' share of this column tile
+          const uint32_t al = a_low + s * (S::kStage >> 4), bl = b_low + s * (S::kStage >> 4);
+          const bool sum = ONES && kb % g.tiles_n == tn;  // the column sums' share of this column tile
+          if (elect()) {
 #pragma unroll
             for (int k = 0; k < kBlockK / 16; ++k)
-              mma<CG>(d + BN, A_MN ? desc_mn(at, k) : desc_k(at, k), desc_k(smem_u32(ones), 0), g.idesc_ones,
-                      summed || k > 0);
-            summed = true;
+              mma<CG>(d, al + k * kDescStep<A_MN>, bl + k * kDescStep<B_MN>, g.idesc, kb > kb0 || k > 0);
+            if (sum) {
+#pragma unroll
+              for (int k = 0; k < kBlockK / 16; ++k)
+                mma<CG>(d + BN, al + k * kDescStep<A_MN>, ones_low, g.idesc_ones, summed || k > 0);
+            }
+            commit<CG>(empty + 8 * s);
+            if (kb + 1 == kb1) commit<CG>(acc_full + 8 * buf);
           }
-          commit<CG>(empty + 8 * s);
+          __syncwarp();
+          summed |= sum;
+          if (++s == S::kStages) s = 0, ph ^= 1;
         }
-        if (ok) commit<CG>(acc_full + 8 * buf);
       }
     }
-    __syncwarp();
   } else if (warp >= kEpiWarp) {
     // ---- epilogue: warp (q, half) takes rows 32 q .. 32 q + 31 of every second 64-column chunk ----
     const int e = warp - kEpiWarp, q = warp & 3, half = e >> 2;
@@ -394,7 +410,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
           }
         }
       }
-      ok = wait_cluster(acc_full + 8 * buf, use & 1);
+      if (lane == 0) ok = wait(acc_full + 8 * buf, use & 1);  // one lane polls: the others' polls cost the issuing warps
+      __syncwarp();
       if (!__all_sync(0xFFFFFFFFu, ok)) {
         ok = false;
         for (int i = 0; ahead && i < 2; ++i)  // gave up: let the copies in flight land
@@ -453,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
           }
         }
         if (in_tma) {
-          ok = mbar_wait(my_in + 8 * b, (in_phase >> b) & 1, kPolls);
+          ok = wait(my_in + 8 * b, (in_phase >> b) & 1);
           in_phase ^= 1u << b;
           if (!__all_sync(0xFFFFFFFFu, ok)) {
             ok = false;
