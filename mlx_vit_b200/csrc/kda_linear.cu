@@ -29,11 +29,11 @@ namespace linear {
 // set to a KDA_ERR_* code by a bounded wait that gave up (read by kda_device_status)
 static __device__ int g_linear_status;
 
-constexpr int kThreads = 384;     // producer, issuer, allocator, idle, 8 epilogue warps
-constexpr int kEpiWarp = 4, kEpiWarps = 8;
+constexpr int kThreads = 640;     // producer, issuer, allocator, idle, 16 epilogue warps
+constexpr int kEpiWarp = 4, kEpiWarps = 16;
 constexpr int kBlockK = 64;       // k per stage: 128 bytes, the swizzle's width
 constexpr int kStageA = 128 * 128;
-constexpr int kStaging = kEpiWarps * 2 * 4096;  // two 32 x 64 tiles a warp
+constexpr int kStaging = kEpiWarps * 4096;  // a 32 x 64 tile a warp
 constexpr int kOnesN = 32;        // columns of the product with ones that sums dz's columns
 constexpr int kSmemMax = 232448;
 constexpr int kPolls = 1 << 20;   // bound of a wait: some tens of milliseconds and more, against microseconds of work
@@ -49,7 +49,8 @@ struct alignas(64) Args {
   float *sums;          // ONES: [splits tiles_n][m] partial column sums of A
   int m, n, k, tiles_m, tiles_n, splits, per_split;  // per_split: blocks of 64 k a part takes
   uint32_t idesc, idesc_ones;
-  int act, in_kind, out_tma, in_tma, save_z;
+  int act, in_kind, out_tma, in_tma, save_z, sum_first;
+  void *db;             // ONES, sum_first: where the sums go
 };
 
 template <int CG, int BN, bool ONES>
@@ -57,7 +58,7 @@ struct Shape {
   static constexpr int kStageB = BN / CG * 128;
   static constexpr int kStage = kStageA + kStageB;
   static constexpr int kOnes = ONES ? kOnesN / CG * 128 : 0;
-  static constexpr int kFixed = kStaging + kOnes + kEpiWarps * 256 + 512;
+  static constexpr int kFixed = kStaging + kOnes + kEpiWarps * 128 + 512;
   static constexpr int kStages = (kSmemMax - kFixed) / kStage < 8 ? (kSmemMax - kFixed) / kStage : 8;
   static constexpr int kAcc = BN + (ONES ? kOnesN : 0);   // tensor-memory columns of one accumulator
   static constexpr int kBufs = 2 * kAcc <= 512 ? 2 : 1;
@@ -215,13 +216,19 @@ __device__ __forceinline__ void finish8(float (&v)[8], uint4 *slot, bool add) {
     const uint32_t w[4] = {zi.x, zi.y, zi.z, zi.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float2 z = P::unpack(w[j]);
-      v[2 * j] *= activate_grad(ACT, z.x);
-      v[2 * j + 1] *= activate_grad(ACT, z.y);
+      const float2 d = mul2(make_float2(v[2 * j], v[2 * j + 1]), activate_grad2(ACT, P::unpack(w[j])));
+      v[2 * j] = d.x;
+      v[2 * j + 1] = d.y;
     }
   } else if (KIND == kForward) {
+    if (ACT != KDA_ACT_NONE) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = activate(ACT, v[j]);
+      for (int j = 0; j < 4; ++j) {
+        const float2 a = activate2(ACT, make_float2(v[2 * j], v[2 * j + 1]));
+        v[2 * j] = a.x;
+        v[2 * j + 1] = a.y;
+      }
+    }
     if (add) {
       const uint4 ri = *slot;
       const uint32_t w[4] = {ri.x, ri.y, ri.z, ri.w};
@@ -234,8 +241,9 @@ __device__ __forceinline__ void finish8(float (&v)[8], uint4 *slot, bool add) {
     }
   }
 }
+// `keep`: the accumulator with its bias as it is (z), else finished.  bs: the chunk's bias.
 template <typename T, int KIND, int ACT>
-__device__ __forceinline__ void chunk(const Args &g, uint32_t acc, uint8_t *so, uint8_t *sz, const float *bs, int lane) {
+__device__ __forceinline__ void chunk(const Args &g, uint32_t acc, uint8_t *so, const T *bs, int lane, bool keep) {
   using P = Pair<T>;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -248,20 +256,28 @@ __device__ __forceinline__ void chunk(const Args &g, uint32_t acc, uint8_t *so, 
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[8 * u + j]);
       if (KIND == kForward && g.bias) {
-        const float4 b0 = *reinterpret_cast<const float4 *>(bs + 32 * h + 8 * u);
-        const float4 b1 = *reinterpret_cast<const float4 *>(bs + 32 * h + 8 * u + 4);
-        v[0] += b0.x; v[1] += b0.y; v[2] += b0.z; v[3] += b0.w;
-        v[4] += b1.x; v[5] += b1.y; v[6] += b1.z; v[7] += b1.w;
+        const uint4 bi = *reinterpret_cast<const uint4 *>(bs + 32 * h + 8 * u);
+        const uint32_t w[4] = {bi.x, bi.y, bi.z, bi.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 x = add2(make_float2(v[2 * j], v[2 * j + 1]), P::unpack(w[j]));
+          v[2 * j] = x.x;
+          v[2 * j + 1] = x.y;
+        }
       }
-      const uint32_t at = chunk_at(lane, 4 * h + u);
-      uint4 *slot = reinterpret_cast<uint4 *>(so + at);
-      if (KIND == kForward && g.save_z)
-        *reinterpret_cast<uint4 *>(sz + at) =
-            make_uint4(P::pack(v[0], v[1]), P::pack(v[2], v[3]), P::pack(v[4], v[5]), P::pack(v[6], v[7]));
-      finish8<T, KIND, ACT>(v, slot, g.in_kind == kInAdd);
+      uint4 *slot = reinterpret_cast<uint4 *>(so + chunk_at(lane, 4 * h + u));
+      if (!keep) finish8<T, KIND, ACT>(v, slot, g.in_kind == kInAdd);
       *slot = make_uint4(P::pack(v[0], v[1]), P::pack(v[2], v[3]), P::pack(v[4], v[5]), P::pack(v[6], v[7]));
     }
   }
+}
+
+// Tile t's place: groups of kGroup rows of tiles, column by column, so that the CTAs at work at one time
+// read few distinct rows of either operand.
+constexpr int kGroup = 8;
+__device__ __forceinline__ int2 place(int t, int tiles_m, int tiles_n) {
+  const int group = t / (kGroup * tiles_n), in = t - group * kGroup * tiles_n, rows = min(kGroup, tiles_m - group * kGroup);
+  return make_int2(group * kGroup + in % rows, in / rows);
 }
 
 template <typename T, int CG, int BN, bool A_MN, bool B_MN, bool ONES>
@@ -277,11 +293,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     return;
   }
   uint8_t *staging = sm + S::kStages * S::kStage, *ones = staging + kStaging;
-  float *bias_sm = reinterpret_cast<float *>(ones + S::kOnes);
-  // barriers: full[stages], empty[stages], acc_full[2], acc_empty[2], in[8 warps][2]; then tensor memory's address
-  const uint32_t bars = smem_u32(bias_sm) + kEpiWarps * 256;
+  T *bias_sm = reinterpret_cast<T *>(ones + S::kOnes);
+  // barriers: full[stages], empty[stages], acc_full[2], acc_empty[2], in[epilogue warps]; then tensor memory's address
+  const uint32_t bars = smem_u32(bias_sm) + kEpiWarps * 128;
   const uint32_t full = bars, empty = full + 8 * S::kStages, acc_full = empty + 8 * S::kStages,
-                 acc_empty = acc_full + 16, in_bar = acc_empty + 16, tmem_at = in_bar + 16 * kEpiWarps;
+                 acc_empty = acc_full + 16, in_bar = acc_empty + 16, tmem_at = in_bar + 8 * kEpiWarps;
   const int kblocks = (g.k + kBlockK - 1) / kBlockK;
   const int tiles = g.tiles_m * g.tiles_n, units = tiles * g.splits, first = blockIdx.x / CG, step = gridDim.x / CG;
 
@@ -294,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       mbar_init(acc_full + 8 * i, 1);
       mbar_init(acc_empty + 8 * i, kEpiWarps * CG);
     }
-    for (int w = 0; w < 2 * kEpiWarps; ++w) mbar_init(in_bar + 8 * w, 1);
+    for (int w = 0; w < kEpiWarps; ++w) mbar_init(in_bar + 8 * w, 1);
     mbar_fence_init();
   }
   if (ONES)
@@ -314,8 +330,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     uint32_t s = 0, ph = 1, issued = 0;
     for (int u = first; ok && u < units; u += step) {
       const int t = u % tiles, kb0 = u / tiles * g.per_split, kb1 = min(kblocks, kb0 + g.per_split);
-      const int m0 = (t / g.tiles_n) * 128 * CG + (int)rank * 128;
-      const int n0 = (t % g.tiles_n) * BN + (int)rank * (BN / CG);
+      const int2 at_tile = place(t, g.tiles_m, g.tiles_n);
+      const int m0 = at_tile.x * 128 * CG + (int)rank * 128, n0 = at_tile.y * BN + (int)rank * (BN / CG);
       for (int kb = kb0; kb < kb1; ++kb) {
         if (!(ok = wait(empty + 8 * s, ph))) break;
         const uint32_t at = base + s * S::kStage, bt = at + kStageA, fb = full_lead + 8 * s;
@@ -355,13 +371,14 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
         const uint32_t d = tmem + buf * S::kAcc;
         if (!(ok = wait(acc_empty + 8 * buf, (use & 1) ^ 1))) break;
         tc_fence_after();
-        const int tn = t % g.tiles_n;
+        const int tn = ONES ? place(t, g.tiles_m, g.tiles_n).y : 0;
         bool summed = false;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!(ok = wait(full + 8 * s, ph))) break;
           tc_fence_after();
           const uint32_t al = a_low + s * (S::kStage >> 4), bl = b_low + s * (S::kStage >> 4);
-          const bool sum = ONES && kb % g.tiles_n == tn;  // the column sums' share of this column tile
+          // the column sums: the first column tile's, or each column tile's share
+          const bool sum = ONES && (g.sum_first ? tn == 0 : kb % g.tiles_n == tn);
           if (elect()) {
 #pragma unroll
             for (int k = 0; k < kBlockK / 16; ++k)
@@ -381,137 +398,129 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       }
     }
   } else if (warp >= kEpiWarp) {
-    // ---- epilogue: warp (q, half) takes rows 32 q .. 32 q + 31 of every second 64-column chunk ----
-    const int e = warp - kEpiWarp, q = warp & 3, half = e >> 2;
-    uint8_t *st = staging + e * 8192;
-    const uint32_t st_at = smem_u32(st), my_in = in_bar + 16 * e;
-    float *bs = bias_sm + e * 64;
+    // ---- epilogue: warp (q, c) takes rows 32 q .. 32 q + 31 of the tile's 64-column chunk c.  Sixteen
+    // warps, so that each scheduler has four to hide an accumulator's and a store's latency with ----
+    const int e = warp - kEpiWarp, q = warp & 3, c = e >> 2;
+    uint8_t *st = staging + e * 4096;
+    const uint32_t st_at = smem_u32(st), my_in = in_bar + 8 * e;
+    T *bs = bias_sm + e * 64;
     const uint32_t empty_lead = CG == 2 ? map_rank(acc_empty, 0) : acc_empty;
-    uint32_t n = 0, in_phase = 0, flip = 0;  // in_phase: bit b for staging tile b
-    // with a z to save the second staging tile is z's, else the chunks alternate
+    uint32_t n = 0, in_phase = 0;
     const bool in_tma = g.in_kind && g.in_tma && g.splits == 1, ahead = in_tma && !g.save_z;
     for (int u = first; ok && u < units; u += step, ++n) {
       const int t = u % tiles, part = u / tiles;
       const uint32_t buf = n % S::kBufs, use = n / S::kBufs;
-      const int tm = t / g.tiles_n, tn = t % g.tiles_n;
-      const int row0 = tm * 128 * CG + (int)rank * 128 + 32 * q;
-      auto fetch = [&](int b, int col0) {  // residual or z of a chunk into staging tile b (lane 0)
-        mbar_expect_tx(my_in + 8 * b, 4096);
-        load_box<1>(st_at + 4096 * b, &g.in, col0, row0, my_in + 8 * b);
+      const int2 at_tile = place(t, g.tiles_m, g.tiles_n);
+      const int tn = at_tile.y, row0 = at_tile.x * 128 * CG + (int)rank * 128 + 32 * q, col0 = tn * BN + 64 * c;
+      const bool mine = c < BN / 64 && row0 < g.m && col0 < g.n;
+      const int rows = min(32, g.m - row0), cols = min(64, g.n - col0);
+      auto fetch = [&] {  // residual or z into the staging tile (one lane)
+        fence_proxy_async_smem();
+        mbar_expect_tx(my_in, 4096);
+        load_box<1>(st_at, &g.in, col0, row0, my_in);
       };
-      if (ahead) {  // ahead of the accumulator: this tile's two chunks
-        if (lane == 0) store_wait_read<0>();
-        __syncwarp();
-        if (lane == 0) {
-          fence_proxy_async_smem();
-          for (int i = 0; i < 2; ++i) {
-            const int c = half + 2 * i, col0 = tn * BN + 64 * c;
-            if (c < BN / 64 && row0 < g.m && col0 < g.n) fetch((flip + i) & 1, col0);
-          }
+      // ahead of the accumulator: the staging tile's last store has been read, its next input, the bias
+      if (lane == 0) store_wait_read<0>();
+      __syncwarp();
+      if (ahead && mine && lane == 0) fetch();
+      if (g.bias && mine && g.splits == 1) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int j = lane + 32 * h;
+          bs[j] = j < cols ? static_cast<const T *>(g.bias)[col0 + j] : T(0.f);
         }
+        __syncwarp();
       }
-      if (lane == 0) ok = wait(acc_full + 8 * buf, use & 1);  // one lane polls: the others' polls cost the issuing warps
+      if (lane == 0) ok = wait(acc_full + 8 * buf, use & 1);
       __syncwarp();
       if (!__all_sync(0xFFFFFFFFu, ok)) {
         ok = false;
-        for (int i = 0; ahead && i < 2; ++i)  // gave up: let the copies in flight land
-          mbar_wait(my_in + 8 * i, (in_phase >> i) & 1, 1 << 16);
+        if (ahead && mine) mbar_wait(my_in, in_phase, 1 << 16);  // gave up: let the copy in flight land
         break;
       }
       tc_fence_after();
       const uint32_t acc = tmem + buf * S::kAcc + ((uint32_t)(32 * q) << 16);
-      if (ONES && half == 0) {
+      if (ONES && c == 0 && (!g.sum_first || tn == 0)) {
         uint32_t v;
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n" : "=r"(v) : "r"(acc + BN));
         tmem_wait_ld();
-        const int kb0 = part * g.per_split, kb1 = min(kblocks, kb0 + g.per_split);
-        const int mine = kb0 + ((tn - kb0) % g.tiles_n + g.tiles_n) % g.tiles_n;  // first block that this column tile summed
-        if (row0 + lane < g.m)
-          g.sums[((int64_t)part * g.tiles_n + tn) * g.m + row0 + lane] = mine < kb1 ? __uint_as_float(v) : 0.f;
-      }
-      for (int c = half; c < BN / 64; c += 2) {
-        const int col0 = tn * BN + 64 * c;
-        if (row0 >= g.m || col0 >= g.n) break;
-        if (g.splits > 1) {  // the float32 tile as it is, 32 columns a store
-          const int prow = part * g.tiles_m * 128 * CG + row0;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t r[32];
-            tmem_ld32(acc + 64 * c + 32 * h, r);
-            if (lane == 0) store_wait_read<1>();
-            __syncwarp();
-            tmem_wait_ld();
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              *reinterpret_cast<uint4 *>(st + 4096 * h + chunk_at(lane, j)) =
-                  make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              store_box(&g.out, st_at + 4096 * h, col0 + 32 * h, prow);
-              store_commit();
-            }
+        const float f = __uint_as_float(v);
+        if (row0 + lane < g.m) {
+          if (g.sum_first) {
+            static_cast<T *>(g.db)[row0 + lane] = from_f<T>(f);
+          } else {
+            const int kb0 = part * g.per_split, kb1 = min(kblocks, kb0 + g.per_split);
+            const int some = kb0 + ((tn - kb0) % g.tiles_n + g.tiles_n) % g.tiles_n;  // first block this column tile sums
+            g.sums[((int64_t)part * g.tiles_n + tn) * g.m + row0 + lane] = some < kb1 ? f : 0.f;
           }
-          continue;
         }
-        const int rows = min(32, g.m - row0), cols = min(64, g.n - col0);
-        const int b = g.save_z ? 0 : flip++ & 1;
-        uint8_t *so = st + b * 4096;
-        const uint32_t so_at = st_at + b * 4096;
-        if (!ahead) {
-          if (lane == 0) {  // this staging tile's last store has been read (a newer one of the other may still be)
-            if (g.save_z) store_wait_read<0>();
-            else store_wait_read<1>();
+      }
+      if (mine && g.splits > 1) {  // the float32 tile as it is, 32 columns a store
+        const int prow = part * g.tiles_m * 128 * CG + row0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t r[32];
+          tmem_ld32(acc + 64 * c + 32 * h, r);
+          if (h && lane == 0) store_wait_read<0>();
+          __syncwarp();
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4 *>(st + chunk_at(lane, j)) = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            store_box(&g.out, st_at, col0 + 32 * h, prow);
+            store_commit();
+          }
+        }
+      } else if (mine) {
+        if (g.save_z) {
+          chunk<T, B_MN ? kPlain : kForward, KDA_ACT_NONE>(g, acc + 64 * c, st, bs, lane, true);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            store_box(&g.z, st_at, col0, row0);
+            store_commit();
+            store_wait_read<0>();
+            if (in_tma) fetch();
           }
           __syncwarp();
-          if (in_tma && lane == 0) {
-            fence_proxy_async_smem();
-            fetch(b, col0);
-          }
         }
         if (in_tma) {
-          ok = wait(my_in + 8 * b, (in_phase >> b) & 1);
-          in_phase ^= 1u << b;
+          ok = wait(my_in, in_phase);
+          in_phase ^= 1;
           if (!__all_sync(0xFFFFFFFFu, ok)) {
             ok = false;
             break;
           }
         } else if (g.in_kind) {
-          tile_in<T>(so, static_cast<const T *>(g.in_ptr) + row0 * g.ldi + col0, g.ldi, rows, cols, lane);
-          __syncwarp();
-        }
-        if (g.bias) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int j = lane + 32 * h;
-            bs[j] = j < cols ? to_f<T>(static_cast<const T *>(g.bias)[col0 + j]) : 0.f;
-          }
+          tile_in<T>(st, static_cast<const T *>(g.in_ptr) + row0 * g.ldi + col0, g.ldi, rows, cols, lane);
           __syncwarp();
         }
         if constexpr (A_MN) {
-          chunk<T, kPlain, KDA_ACT_NONE>(g, acc + 64 * c, so, st + 4096, bs, lane);
+          chunk<T, kPlain, KDA_ACT_NONE>(g, acc + 64 * c, st, bs, lane, false);
         } else {
           constexpr int kind = B_MN ? kGrad : kForward;
           switch (g.act) {
-            case KDA_ACT_RELU: chunk<T, kind, KDA_ACT_RELU>(g, acc + 64 * c, so, st + 4096, bs, lane); break;
-            case KDA_ACT_SILU: chunk<T, kind, KDA_ACT_SILU>(g, acc + 64 * c, so, st + 4096, bs, lane); break;
-            case KDA_ACT_GELU: chunk<T, kind, KDA_ACT_GELU>(g, acc + 64 * c, so, st + 4096, bs, lane); break;
-            case KDA_ACT_GELU_TANH: chunk<T, kind, KDA_ACT_GELU_TANH>(g, acc + 64 * c, so, st + 4096, bs, lane); break;
-            default: chunk<T, kind, KDA_ACT_NONE>(g, acc + 64 * c, so, st + 4096, bs, lane);
+            case KDA_ACT_RELU: chunk<T, kind, KDA_ACT_RELU>(g, acc + 64 * c, st, bs, lane, false); break;
+            case KDA_ACT_SILU: chunk<T, kind, KDA_ACT_SILU>(g, acc + 64 * c, st, bs, lane, false); break;
+            case KDA_ACT_GELU: chunk<T, kind, KDA_ACT_GELU>(g, acc + 64 * c, st, bs, lane, false); break;
+            case KDA_ACT_GELU_TANH: chunk<T, kind, KDA_ACT_GELU_TANH>(g, acc + 64 * c, st, bs, lane, false); break;
+            default: chunk<T, kind, KDA_ACT_NONE>(g, acc + 64 * c, st, bs, lane, false);
           }
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (!g.out_tma)
-          tile_out<T>(so, static_cast<T *>(g.out_ptr) + row0 * g.ldo + col0, g.ldo, rows, cols, lane);
-        if (lane == 0) {
-          if (g.out_tma) store_box(&g.out, so_at, col0, row0);
-          if (g.save_z) store_box(&g.z, st_at + 4096, col0, row0);
-          store_commit();
+        if (g.out_tma) {
+          if (lane == 0) {
+            store_box(&g.out, st_at, col0, row0);
+            store_commit();
+          }
+        } else {
+          tile_out<T>(st, static_cast<T *>(g.out_ptr) + row0 * g.ldo + col0, g.ldo, rows, cols, lane);
         }
-        __syncwarp();
       }
-      if (!ok) break;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
@@ -789,6 +798,11 @@ static int run(Args &g, const Plan &p, const void *a, int64_t lda, const void *b
     g.sums = reinterpret_cast<float *>(at);
     at += sums_bytes(p, g.m, g.n);
   }
+  // One CTA on a tile waits for its operands' copies, and the first column tile has the tensor cores'
+  // time for all sums; a pair is bound by them, so its column tiles share the sums and they are
+  // added afterwards (as they are where k is split).
+  g.sum_first = ONES && p.cg == 1 && p.splits == 1;
+  g.db = db;
   const int64_t rows = part_rows(p, g.m);
   if (p.splits > 1) {
     g.part = reinterpret_cast<float *>(at);
@@ -798,7 +812,7 @@ static int run(Args &g, const Plan &p, const void *a, int64_t lda, const void *b
   s = p.cg == 2    ? launch<T, 2, 256, A_MN, B_MN, ONES>(g, sms, st)
       : p.bn == 128 ? launch<T, 1, 128, A_MN, B_MN, ONES>(g, sms, st)
                     : launch<T, 1, 64, A_MN, B_MN, ONES>(g, sms, st);
-  if (s || (p.splits == 1 && !ONES)) return s;
+  if (s || (p.splits == 1 && (!ONES || g.sum_first))) return s;
   const int col_blocks = (g.n + 511) / 512;
   const int64_t tile_blocks = p.splits > 1 ? (int64_t)((g.m + kJoinRows - 1) / kJoinRows) * col_blocks : 0;
   const int64_t blocks = tile_blocks + (ONES ? (g.m + 255) / 256 : 0);
