@@ -600,26 +600,33 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
 
 // ---- a few rows: y = act(x W^T + bias) + residual with M <= 32 ----
 // The weights' bytes bound it: each is read once, straight into the fragments of m16n8k16 products
-// whose 16 rows are 16 outputs and whose 8 columns are 8 of x's rows.  k may be summed in any order, so
-// a lane's share of a product is 8 consecutive k (one 16-byte load of W, one of x) instead of
-// the layout's four pairs.  A CTA owns 16 outputs, its warps take k 64 at a time in turn, and their
-// sums meet in shared memory.
+// whose 16 rows are rows of x and whose 8 columns are 8 outputs.  k may be summed in any order, so a
+// lane's share of two products is 8 consecutive k (one 16-byte load of W, one of each row of x)
+// instead of the layout's pairs.  `kw` warps share 8 outputs, each with its range of k, and the next eight
+// loads of W a lane (4 KB a warp) are in flight while the last eight are multiplied; x comes
+// through the first-level cache, which W's loads pass by.  The warps' sums meet in shared memory.
 template <typename T>
 __device__ __forceinline__ void mma_m16n8k16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                              uint32_t b1) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// 8 elements of a row from column k on; columns past the end count as zero.  The load itself is
+// 16 bytes of a row of W, which no one reads again, and of x, which every warp reads.
+__device__ __forceinline__ uint4 load_once(const char *p) {
+  uint4 u;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
+  return u;
+}
+// `left` elements of 8 exist (none, if not positive); the others count as zero.  The load itself is
 // a whole aligned 16 bytes, whose first byte lies in the row, so it stays in its page.
-__device__ __forceinline__ uint4 load_k8(const void *row, int k, int K) {
-  if (k >= K) return make_uint4(0, 0, 0, 0);
-  uint4 u = __ldg(reinterpret_cast<const uint4 *>(static_cast<const char *>(row) + 2 * (int64_t)k));
-  const int left = K - k;
+__device__ __forceinline__ uint4 load_some(const char *p, int left) {
+  uint4 u = make_uint4(0, 0, 0, 0);
+  if (left > 0) u = __ldg(reinterpret_cast<const uint4 *>(p));
   if (left < 8) {
     uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -634,49 +641,78 @@ struct FewArgs {
   int64_t ldx, ldw, ldr, ldy, ldz;
   int m, n, k, act;
 };
-constexpr int kFewRows = 32;
-template <typename T, int MT, int WARPS>  // MT groups of 8 rows of x
-__global__ void __launch_bounds__(32 * WARPS) few_rows_kernel(const FewArgs a) {
-  __shared__ float red[WARPS][16][8 * MT + 1];
+constexpr int kFewRows = 32, kFewWarps = 8;
+template <typename T, int MT>  // MT groups of 8 rows of x: 1, 2 or 4
+__global__ void __launch_bounds__(32 * kFewWarps, 2) few_rows_kernel(const FewArgs a, int kw, int range) {
+  __shared__ float red[kFewWarps][8 * MT][9];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-  const int n0 = blockIdx.x * 16;
-  const char *w0 = static_cast<const char *>(a.w) + 2 * a.ldw * min(n0 + g, a.n - 1);
-  const char *w1 = static_cast<const char *>(a.w) + 2 * a.ldw * min(n0 + g + 8, a.n - 1);
+  const int blocks = kFewWarps / kw, block0 = blockIdx.x * blocks;  // groups of 8 outputs of this CTA
+  const int n0 = (block0 + warp / kw) * 8, from = warp % kw * range, to = min(from + range, a.k);
+  const char *wr = static_cast<const char *>(a.w) + 2 * a.ldw * min(n0 + g, a.n - 1);
   const char *xr[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) xr[t] = static_cast<const char *>(a.x) + 2 * a.ldx * min(8 * t + g, a.m - 1);
-  float d[MT][4] = {};
-  constexpr int U = 4;  // 32-k groups in flight: 64 k of this turn and of the next
-  for (int k0 = 64 * warp; k0 < a.k; k0 += 64 * WARPS * (U / 2)) {
-    uint4 p[U], q[U];
+  constexpr int U = 8, P = (MT + 1) / 2;
+  float d[P][4] = {};
+  if (n0 < a.n) {
+    wr += 2 * (from + 8 * c);
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int k = k0 + (j >> 1) * 64 * WARPS + (j & 1) * 32 + 8 * c;
-      p[j] = load_k8(w0, k, a.k);
-      q[j] = load_k8(w1, k, a.k);
+    for (int t = 0; t < MT; ++t) xr[t] += 2 * (from + 8 * c);
+    const int whole = to > from ? (to - from) / (32 * U) : 0;
+    uint4 next[U];
+    if (whole) {
+#pragma unroll
+      for (int j = 0; j < U; ++j) next[j] = load_once(wr + 64 * j);
     }
+    for (int i = 0; i < whole; ++i) {
+      uint4 w[U];
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      const int k = k0 + (j >> 1) * 64 * WARPS + (j & 1) * 32 + 8 * c;
+      for (int j = 0; j < U; ++j) w[j] = next[j];
+      wr += 64 * U;
+      if (i + 1 < whole) {
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const uint4 x = load_k8(xr[t], k, a.k);
-        mma_m16n8k16<T>(d[t], p[j].x, q[j].x, p[j].y, q[j].y, x.x, x.y);
-        mma_m16n8k16<T>(d[t], p[j].z, q[j].z, p[j].w, q[j].w, x.z, x.w);
+        for (int j = 0; j < U; ++j) next[j] = load_once(wr + 64 * j);
       }
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          const uint4 x0 = __ldg(reinterpret_cast<const uint4 *>(xr[2 * p] + 64 * j));
+          uint4 x1 = make_uint4(0, 0, 0, 0);
+          if (2 * p + 1 < MT) x1 = __ldg(reinterpret_cast<const uint4 *>(xr[MT > 1 ? 2 * p + 1 : 0] + 64 * j));
+          mma_m16n8k16<T>(d[p], x0.x, x1.x, x0.y, x1.y, w[j].x, w[j].y);
+          mma_m16n8k16<T>(d[p], x0.z, x1.z, x0.w, x1.w, w[j].z, w[j].w);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < MT; ++t) xr[t] += 64 * U;
+    }
+    for (int k = from + 32 * U * whole + 8 * c; k - 8 * c < to; k += 32) {  // the range's rest
+      const uint4 w = load_some(wr, to - k);
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const uint4 x0 = load_some(xr[2 * p], to - k);
+        uint4 x1 = make_uint4(0, 0, 0, 0);
+        if (2 * p + 1 < MT) x1 = load_some(xr[MT > 1 ? 2 * p + 1 : 0], to - k);
+        mma_m16n8k16<T>(d[p], x0.x, x1.x, x0.y, x1.y, w.x, w.y);
+        mma_m16n8k16<T>(d[p], x0.z, x1.z, x0.w, x1.w, w.z, w.w);
+      }
+      wr += 64;
+#pragma unroll
+      for (int t = 0; t < MT; ++t) xr[t] += 64;
     }
   }
 #pragma unroll
-  for (int t = 0; t < MT; ++t)
+  for (int p = 0; p < P; ++p)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) red[warp][g + 8 * (i >> 1)][8 * t + 2 * c + (i & 1)] = d[t][i];
+    for (int i = 0; i < 4; ++i)
+      if (16 * p + 8 * (i >> 1) < 8 * MT) red[warp][16 * p + g + 8 * (i >> 1)][2 * c + (i & 1)] = d[p][i];
   __syncthreads();
-  for (int o = threadIdx.x; o < 16 * a.m; o += 32 * WARPS) {
-    const int j = o & 15, row = o >> 4, n = n0 + j;
+  for (int o = threadIdx.x; o < 8 * blocks * a.m; o += 32 * kFewWarps) {
+    const int j = o % (8 * blocks), row = o / (8 * blocks), n = 8 * block0 + j;
     if (n >= a.n) continue;
     float v = 0.f;
-#pragma unroll
-    for (int i = 0; i < WARPS; ++i) v += red[i][j][row];
+    for (int i = 0; i < kw; ++i) v += red[(j >> 3) * kw + i][row][j & 7];
     if (a.bias) v += to_f<T>(static_cast<const T *>(a.bias)[n]);
     if (a.z) static_cast<T *>(a.z)[row * a.ldz + n] = from_f<T>(v);
     v = activate(a.act, v);
@@ -825,10 +861,12 @@ static int run(Args &g, const Plan &p, const void *a, int64_t lda, const void *b
 
 template <typename T, int MT>
 static int few_rows(const FewArgs &a, int sms, cudaStream_t st) {
-  const int grid = (a.n + 15) / 16;
-  // twice the warps where the outputs alone do not fill the GPU (and k has turns for them)
-  if (grid < 2 * sms && a.k > 512) few_rows_kernel<T, MT, 16><<<grid, 512, 0, st>>>(a);
-  else few_rows_kernel<T, MT, 8><<<grid, 256, 0, st>>>(a);
+  // warps per 8 outputs: enough that some 12 warps an SM stream weights, at most a CTA's
+  const int groups = (a.n + 7) / 8;
+  int kw = 1;
+  while (kw < kFewWarps && (int64_t)groups * kw < 12ll * sms) kw *= 2;
+  const int range = ((a.k + 31) / 32 + kw - 1) / kw * 32, per = kFewWarps / kw;
+  few_rows_kernel<T, MT><<<(groups + per - 1) / per, 32 * kFewWarps, 0, st>>>(a, kw, range);
   if (cudaGetLastError() != cudaSuccess) return KDA_ERR_CUDA;
   count_launch();
   return KDA_OK;
