@@ -642,77 +642,94 @@ struct FewArgs {
   int m, n, k, act;
 };
 constexpr int kFewRows = 32, kFewWarps = 8;
-template <typename T, int MT>  // MT groups of 8 rows of x: 1, 2 or 4
+// MT groups of 8 rows of x (1, 2 or 4) by NB groups of 8 outputs a warp: with more rows of x two, so that a
+// load of x serves two products
+template <typename T, int MT, int NB>
 __global__ void __launch_bounds__(32 * kFewWarps, 2) few_rows_kernel(const FewArgs a, int kw, int range) {
-  __shared__ float red[kFewWarps][8 * MT][9];
+  __shared__ float red[kFewWarps][8 * MT][8 * NB + 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-  const int blocks = kFewWarps / kw, block0 = blockIdx.x * blocks;  // groups of 8 outputs of this CTA
-  const int n0 = (block0 + warp / kw) * 8, from = warp % kw * range, to = min(from + range, a.k);
-  const char *wr = static_cast<const char *>(a.w) + 2 * a.ldw * min(n0 + g, a.n - 1);
-  const char *xr[MT];
+  const int blocks = kFewWarps / kw, block0 = blockIdx.x * blocks;  // groups of 8 NB outputs of this CTA
+  const int n0 = (block0 + warp / kw) * 8 * NB, from = warp % kw * range, to = min(from + range, a.k);
+  const char *wr[NB], *xr[MT];
 #pragma unroll
-  for (int t = 0; t < MT; ++t) xr[t] = static_cast<const char *>(a.x) + 2 * a.ldx * min(8 * t + g, a.m - 1);
-  constexpr int U = 8, P = (MT + 1) / 2;
-  float d[P][4] = {};
+  for (int b = 0; b < NB; ++b)
+    wr[b] = static_cast<const char *>(a.w) + 2 * (a.ldw * min(n0 + 8 * b + g, a.n - 1) + from + 8 * c);
+#pragma unroll
+  for (int t = 0; t < MT; ++t) xr[t] = static_cast<const char *>(a.x) + 2 * (a.ldx * min(8 * t + g, a.m - 1) + from + 8 * c);
+  constexpr int U = 8 / NB, P = (MT + 1) / 2;
+  float d[NB][P][4] = {};
+  auto products = [&](const uint4 (&w)[NB], const uint4 (&x)[2 * P]) {
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        mma_m16n8k16<T>(d[b][p], x[2 * p].x, x[2 * p + 1].x, x[2 * p].y, x[2 * p + 1].y, w[b].x, w[b].y);
+        mma_m16n8k16<T>(d[b][p], x[2 * p].z, x[2 * p + 1].z, x[2 * p].w, x[2 * p + 1].w, w[b].z, w[b].w);
+      }
+  };
   if (n0 < a.n) {
-    wr += 2 * (from + 8 * c);
-#pragma unroll
-    for (int t = 0; t < MT; ++t) xr[t] += 2 * (from + 8 * c);
     const int whole = to > from ? (to - from) / (32 * U) : 0;
-    uint4 next[U];
+    uint4 next[U][NB];
     if (whole) {
 #pragma unroll
-      for (int j = 0; j < U; ++j) next[j] = load_once(wr + 64 * j);
+      for (int j = 0; j < U; ++j)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) next[j][b] = load_once(wr[b] + 64 * j);
     }
     for (int i = 0; i < whole; ++i) {
-      uint4 w[U];
+      uint4 w[U][NB];
 #pragma unroll
-      for (int j = 0; j < U; ++j) w[j] = next[j];
-      wr += 64 * U;
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) w[j][b] = next[j][b];
+        wr[b] += 64 * U;
+      }
       if (i + 1 < whole) {
 #pragma unroll
-        for (int j = 0; j < U; ++j) next[j] = load_once(wr + 64 * j);
+        for (int j = 0; j < U; ++j)
+#pragma unroll
+          for (int b = 0; b < NB; ++b) next[j][b] = load_once(wr[b] + 64 * j);
       }
 #pragma unroll
       for (int j = 0; j < U; ++j) {
+        uint4 x[2 * P];
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-          const uint4 x0 = __ldg(reinterpret_cast<const uint4 *>(xr[2 * p] + 64 * j));
-          uint4 x1 = make_uint4(0, 0, 0, 0);
-          if (2 * p + 1 < MT) x1 = __ldg(reinterpret_cast<const uint4 *>(xr[MT > 1 ? 2 * p + 1 : 0] + 64 * j));
-          mma_m16n8k16<T>(d[p], x0.x, x1.x, x0.y, x1.y, w[j].x, w[j].y);
-          mma_m16n8k16<T>(d[p], x0.z, x1.z, x0.w, x1.w, w[j].z, w[j].w);
-        }
+        for (int t = 0; t < 2 * P; ++t)
+          x[t] = t < MT ? __ldg(reinterpret_cast<const uint4 *>(xr[t < MT ? t : 0] + 64 * j)) : make_uint4(0, 0, 0, 0);
+        products(w[j], x);
       }
 #pragma unroll
       for (int t = 0; t < MT; ++t) xr[t] += 64 * U;
     }
     for (int k = from + 32 * U * whole + 8 * c; k - 8 * c < to; k += 32) {  // the range's rest
-      const uint4 w = load_some(wr, to - k);
+      uint4 w[NB], x[2 * P];
 #pragma unroll
-      for (int p = 0; p < P; ++p) {
-        const uint4 x0 = load_some(xr[2 * p], to - k);
-        uint4 x1 = make_uint4(0, 0, 0, 0);
-        if (2 * p + 1 < MT) x1 = load_some(xr[MT > 1 ? 2 * p + 1 : 0], to - k);
-        mma_m16n8k16<T>(d[p], x0.x, x1.x, x0.y, x1.y, w.x, w.y);
-        mma_m16n8k16<T>(d[p], x0.z, x1.z, x0.w, x1.w, w.z, w.w);
+      for (int b = 0; b < NB; ++b) {
+        w[b] = load_some(wr[b], to - k);
+        wr[b] += 64;
       }
-      wr += 64;
 #pragma unroll
-      for (int t = 0; t < MT; ++t) xr[t] += 64;
+      for (int t = 0; t < 2 * P; ++t) {
+        x[t] = t < MT ? load_some(xr[t < MT ? t : 0], to - k) : make_uint4(0, 0, 0, 0);
+        if (t < MT) xr[t] += 64;
+      }
+      products(w, x);
     }
   }
 #pragma unroll
-  for (int p = 0; p < P; ++p)
+  for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (16 * p + 8 * (i >> 1) < 8 * MT) red[warp][16 * p + g + 8 * (i >> 1)][2 * c + (i & 1)] = d[p][i];
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (16 * p + 8 * (i >> 1) < 8 * MT) red[warp][16 * p + g + 8 * (i >> 1)][8 * b + 2 * c + (i & 1)] = d[b][p][i];
   __syncthreads();
-  for (int o = threadIdx.x; o < 8 * blocks * a.m; o += 32 * kFewWarps) {
-    const int j = o % (8 * blocks), row = o / (8 * blocks), n = 8 * block0 + j;
+  const int outs = 8 * NB * blocks;
+  for (int o = threadIdx.x; o < outs * a.m; o += 32 * kFewWarps) {
+    const int j = o % outs, row = o / outs, n = 8 * NB * block0 + j;
     if (n >= a.n) continue;
     float v = 0.f;
-    for (int i = 0; i < kw; ++i) v += red[(j >> 3) * kw + i][row][j & 7];
+    for (int i = 0; i < kw; ++i) v += red[j / (8 * NB) * kw + i][row][j % (8 * NB)];
     if (a.bias) v += to_f<T>(static_cast<const T *>(a.bias)[n]);
     if (a.z) static_cast<T *>(a.z)[row * a.ldz + n] = from_f<T>(v);
     v = activate(a.act, v);
@@ -859,21 +876,21 @@ static int run(Args &g, const Plan &p, const void *a, int64_t lda, const void *b
   return KDA_OK;
 }
 
-template <typename T, int MT>
+template <typename T, int MT, int NB>
 static int few_rows(const FewArgs &a, int sms, cudaStream_t st) {
-  // warps per 8 outputs: enough that some 12 warps an SM stream weights, at most a CTA's
-  const int groups = (a.n + 7) / 8;
+  // warps per group of outputs: enough that some 12 warps an SM stream weights, at most a CTA's
+  const int groups = (a.n + 8 * NB - 1) / (8 * NB);
   int kw = 1;
   while (kw < kFewWarps && (int64_t)groups * kw < 12ll * sms) kw *= 2;
   const int range = ((a.k + 31) / 32 + kw - 1) / kw * 32, per = kFewWarps / kw;
-  few_rows_kernel<T, MT><<<(groups + per - 1) / per, 32 * kFewWarps, 0, st>>>(a, kw, range);
+  few_rows_kernel<T, MT, NB><<<(groups + per - 1) / per, 32 * kFewWarps, 0, st>>>(a, kw, range);
   if (cudaGetLastError() != cudaSuccess) return KDA_ERR_CUDA;
   count_launch();
   return KDA_OK;
 }
 template <typename T>
 static int few_rows(const FewArgs &a, int sms, cudaStream_t st) {
-  return a.m <= 8 ? few_rows<T, 1>(a, sms, st) : a.m <= 16 ? few_rows<T, 2>(a, sms, st) : few_rows<T, 4>(a, sms, st);
+  return a.m <= 8 ? few_rows<T, 1, 1>(a, sms, st) : a.m <= 16 ? few_rows<T, 2, 2>(a, sms, st) : few_rows<T, 4, 2>(a, sms, st);
 }
 
 static int set_out(Args &g, void *p, int64_t ld) {
