@@ -274,8 +274,8 @@ KDA_API int kda_act_grad(int dtype, int act, int64_t rows, int64_t cols, const v
  * The states m, v: float32 [numel] (state_bits 32), or 8-bit codes [numel] with one exponent byte
  * per 256 consecutive elements, m_exp, v_exp [ceil(numel / 256)] (state_bits 8; all zero bytes
  * are the zero state).  ema: float32 [numel], read only where KdaAdamW.use_ema is set.  Every
- * pointer needs its element's alignment only; 16 bytes (8 for codes) are faster.  The tensors of one call must not
- * overlap. */
+ * pointer needs its element's alignment only; 32 bytes (16 for 16-bit elements, 8 for codes) are
+ * faster.  The tensors of one call must not overlap. */
 typedef struct KdaAdamWTensor {
   void *p;
   const void *g;

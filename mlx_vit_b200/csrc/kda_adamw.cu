@@ -25,7 +25,8 @@
 namespace kda {
 namespace adamw {
 
-constexpr int kThreads = 256, kPer = 8, kChunk = kThreads * kPer, kBlock = 32 * kPer;
+constexpr int kThreads = 256, kPer = 8, kBlock = 32 * kPer;
+constexpr int kPass = kThreads * kPer, kChunk = 2 * kPass;  // elements a CTA takes at once; two passes a chunk
 constexpr int kCap = 448, kCapSmall = 64;  // tensors a launch holds (72 bytes each; parameters end at 32764 bytes)
 
 constexpr int kCtasPerSm = 4;       // resident CTAs the update's grid is sized for (64 registers a thread)
@@ -122,13 +123,13 @@ __device__ __forceinline__ uint32_t gather(uint32_t a, uint32_t b, uint32_t c, u
   return __byte_perm(ab, cd, 0x5410);
 }
 
-// ---- vectors of kPer elements ----
+// ---- vectors of kPer elements; float32's as one 32-byte access (two of 16 bytes take a tenth longer
+// over the whole step) ----
 template <typename T>
 __device__ __forceinline__ void load_vec(const T *p, float (&x)[kPer]) {
   if constexpr (sizeof(T) == 4) {
-    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]) : "l"(p));
   } else {
     union { uint4 u; T t[8]; } q;
     q.u = *reinterpret_cast<const uint4 *>(p);
@@ -139,8 +140,8 @@ __device__ __forceinline__ void load_vec(const T *p, float (&x)[kPer]) {
 template <typename T>
 __device__ __forceinline__ void store_vec(T *p, const float (&x)[kPer]) {
   if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4 *>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4 *>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                 :: "l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]) : "memory");
   } else {
     union { uint4 u; T t[8]; } q;
 #pragma unroll
@@ -283,6 +284,153 @@ __device__ __forceinline__ void update(const Entry &e, int64_t i, uint32_t tenso
   }
 }
 
+// ---- a lane whose eight elements all exist and are aligned: the same with 8-bit states in fewer
+// instructions.  The step is bound by them, not by its 10 bytes an element, so products and sums go
+// two to an instruction, zero codes and values below the least code take branches of their own (rare
+// but in tensors without gradients), and codes are picked from bits 20-27 by bytes. ----
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}\n"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}\n"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+      " fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}\n"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// decode8 where no code is zero
+template <bool SIGNED>
+__device__ __forceinline__ void decode8_live(uint2 u, int e, uint32_t (&x)[4]) {
+  const uint32_t shift = (uint32_t)(e - (SIGNED ? kLowM : kLowV)) * 0x00800080u;  // a negative one borrows nothing
+  const uint32_t w[4] = {__byte_perm(u.x, 0, 0x4140), __byte_perm(u.x, 0, 0x4342), __byte_perm(u.y, 0, 0x4140),
+                         __byte_perm(u.y, 0, 0x4342)};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[j] = (SIGNED ? w[j] & 0x007F007Fu : w[j]) * 16u + shift;
+    if (SIGNED) x[j] |= (w[j] << 8) & 0x80008000u;
+  }
+}
+__device__ __forceinline__ bool all_live(uint2 m, uint2 v) {  // no zero byte in m (without signs) and v
+  const uint32_t a = ((m.x & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) & ((m.y & 0x7F7F7F7Fu) + 0x7F7F7F7Fu);
+  const uint32_t zx = (v.x - 0x01010101u) & ~v.x, zy = (v.y - 0x01010101u) & ~v.y;
+  return ((~a | zx | zy) & 0x80808080u) == 0;
+}
+// bits 20-27 of four words as four bytes
+__device__ __forceinline__ uint32_t pick(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x7632) >> 4, __byte_perm(c, d, 0x7632) >> 4, 0x6420);
+}
+
+// what a lane reads of its eight elements, as it lies in memory: held for both passes of a chunk, so that
+// the second's loads pass while the first is worked on
+template <typename T>
+struct Raw {
+  uint4 g[sizeof(T) / 2], p[sizeof(T) / 2];
+  uint2 m, v;
+  int me, ve;
+  __device__ __forceinline__ void load(const Entry &e, int64_t i) {
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(T) / 2; ++j) {
+      g[j] = reinterpret_cast<const uint4 *>(static_cast<const T *>(e.g) + i)[j];
+      p[j] = reinterpret_cast<const uint4 *>(static_cast<const T *>(e.p) + i)[j];
+    }
+    m = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(e.m) + i);
+    v = *reinterpret_cast<const uint2 *>(static_cast<const uint8_t *>(e.v) + i);
+    me = e.me[i / kBlock];
+    ve = e.ve[i / kBlock];
+  }
+  static __device__ __forceinline__ void values(const uint4 (&u)[sizeof(T) / 2], float (&x)[kPer]) {
+    const T *t = reinterpret_cast<const T *>(u);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) x[j] = to_f<T>(t[j]);
+  }
+};
+
+template <typename T, bool EMA>
+__device__ __forceinline__ void update8(const Raw<T> &in, const Entry &e, int64_t i, uint32_t tensor, const Hyper &h) {
+  uint8_t *mp = static_cast<uint8_t *>(e.m) + i, *vp = static_cast<uint8_t *>(e.v) + i;
+  uint8_t *me = e.me + i / kBlock, *ve = e.ve + i / kBlock;
+  float p[kPer], g[kPer];
+  Raw<T>::values(in.g, g);
+  Raw<T>::values(in.p, p);
+  const uint2 mc = in.m, vc = in.v;
+  const int me0 = in.me, ve0 = in.ve;
+  uint32_t mx[4], vx[4];
+  if (all_live(mc, vc)) {
+    decode8_live<true>(mc, me0, mx);
+    decode8_live<false>(vc, ve0, vx);
+  } else {
+    decode8<true>(mc, me0, mx);
+    decode8<false>(vc, ve0, vx);
+  }
+  const float nan = __uint_as_float(0x7FC00000u);  // what a block that is not finite decodes to
+  const float2 b1 = both(me0 == 255 ? nan : h.b1), b2 = both(ve0 == 255 ? nan : h.b2);
+  float m[kPer], v[kPer];
+  uint32_t mtop = 0, vtop = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; j += 2) {
+    const float2 gj = mul2(make_float2(g[j], g[j + 1]), both(h.coef));
+    const float2 mj = add2(mul2(make_float2(bf16_of(mx, j), bf16_of(mx, j + 1)), b1), mul2(gj, both(h.b1c)));
+    const float2 vj = add2(mul2(make_float2(bf16_of(vx, j), bf16_of(vx, j + 1)), b2), mul2(mul2(gj, gj), both(h.b2c)));
+    const float2 d = fma2(make_float2(sqrt_fast<true>(vj.x), sqrt_fast<true>(vj.y)), both(h.c2), both(h.eps));
+    const float2 s = mul2(mj, both(-h.c1));
+    const float2 pj = fma2(make_float2(p[j], p[j + 1]), both(h.decay),
+                           make_float2(div_fast<true>(s.x, d.x), div_fast<true>(s.y, d.y)));
+    p[j] = pj.x; p[j + 1] = pj.y;
+    m[j] = mj.x; m[j + 1] = mj.y;
+    v[j] = vj.x; v[j + 1] = vj.y;
+    mtop = max(mtop, max(__float_as_uint(mj.x) & 0x7FFFFFFFu, __float_as_uint(mj.y) & 0x7FFFFFFFu));
+    vtop = max(vtop, max(__float_as_uint(vj.x), __float_as_uint(vj.y)));  // v has no sign, but for a NaN's
+  }
+  store_vec(static_cast<T *>(e.p) + i, p);
+  const int me1 = min((int)block_exp(__reduce_max_sync(0xFFFFFFFFu, mtop)), 255);
+  const int ve1 = min((int)block_exp(__reduce_max_sync(0xFFFFFFFFu, vtop)), 255);
+  const int mbase = (me1 - kLowM) * (1 << 23), vbase = (ve1 - kLowV) * (1 << 23);
+  const int mleast = max(mbase + (1 << 20), (int)kTiny), vleast = max(vbase + (1 << 20), (int)kTiny);
+  const uint32_t at = (uint32_t)i ^ mix(h.key ^ tensor);  // i is a multiple of kPer: (i + j) ^ key = at ^ j
+  uint32_t tm[kPer], tv[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const uint32_t r = mix(at ^ (uint32_t)j);
+    const uint32_t rm = ((r << 4) & 0xFFFF0u) | 8u, rv = ((r >> 12) & 0xFFFF0u) | 8u;
+    const uint32_t a = __float_as_uint(m[j]) & 0x7FFFFFFFu, b = __float_as_uint(v[j]);
+    tm[j] = a + rm - (uint32_t)mbase;
+    tv[j] = b + rv - (uint32_t)vbase;
+    if ((int)a < mleast) {
+      tm[j] = encode<true>(a, mbase, rm) << 20;
+      if (tm[j] == 0) m[j] = 0.f;  // zero has no sign
+    }
+    if ((int)b < vleast) tv[j] = encode<false>(b & 0x7FFFFFFFu, vbase, rv) << 20;
+  }
+  uint2 mn = make_uint2(pick(tm[0], tm[1], tm[2], tm[3]), pick(tm[4], tm[5], tm[6], tm[7]));
+  mn.x |= gather(__float_as_uint(m[0]), __float_as_uint(m[1]), __float_as_uint(m[2]), __float_as_uint(m[3]), true) & 0x80808080u;
+  mn.y |= gather(__float_as_uint(m[4]), __float_as_uint(m[5]), __float_as_uint(m[6]), __float_as_uint(m[7]), true) & 0x80808080u;
+  *reinterpret_cast<uint2 *>(mp) = mn;
+  *reinterpret_cast<uint2 *>(vp) = make_uint2(pick(tv[0], tv[1], tv[2], tv[3]), pick(tv[4], tv[5], tv[6], tv[7]));
+  if (i % kBlock == 0) {
+    *me = (uint8_t)me1;
+    *ve = (uint8_t)ve1;
+  }
+  if constexpr (EMA) {
+    float s[kPer];
+    load_vec(e.ema + i, s);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      s[j] = __fadd_rn(__fmul_rn(s[j], h.ema_d), __fmul_rn(to_f<T>(from_f<T>(p[j])), h.ema_c));
+    store_vec(e.ema + i, s);
+  }
+}
+
 template <int CAP>
 __device__ __forceinline__ uint32_t find_tensor(const Table<CAP> &t, uint32_t lo, uint32_t chunk) {
   uint32_t hi = t.count - 1;
@@ -292,6 +440,23 @@ __device__ __forceinline__ uint32_t find_tensor(const Table<CAP> &t, uint32_t lo
     else hi = mid - 1;
   }
   return lo;
+}
+
+// a thread's two passes of a chunk, from element i on
+template <typename T, bool EIGHT, bool EMA>
+__device__ __forceinline__ void chunk(const Entry &e, int64_t i, uint32_t tensor, const Hyper &h) {
+  const int64_t warp_at = i - (threadIdx.x & 31) * kPer;
+  if (EIGHT && e.vec && warp_at + kPass + kBlock <= e.n) {  // the warp's elements all exist, aligned
+    Raw<T> a, b;
+    a.load(e, i);
+    b.load(e, i + kPass);
+    update8<T, EMA>(a, e, i, tensor, h);
+    update8<T, EMA>(b, e, i + kPass, tensor, h);
+    return;
+  }
+#pragma unroll 1
+  for (int pass = 0; pass < 2 && warp_at + pass * kPass < e.n; ++pass)
+    update<T, EIGHT, EMA>(e, i + pass * kPass, tensor, h);
 }
 
 template <bool EIGHT, bool EMA, int CAP>
@@ -308,11 +473,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) adamw_kernel(const __gri
     ti = find_tensor(t, ti, c);
     const Entry &e = t.e[ti];
     const int64_t i = (int64_t)(c - e.first) * kChunk + threadIdx.x * kPer;
-    if (i - (threadIdx.x & 31) * kPer >= e.n) continue;  // the whole warp lies behind the end
     const uint32_t tensor = t.index0 + ti;
-    if (e.dtype == KDA_F32) update<float, EIGHT, EMA>(e, i, tensor, h);
-    else if (e.dtype == KDA_BF16) update<__nv_bfloat16, EIGHT, EMA>(e, i, tensor, h);
-    else update<__half, EIGHT, EMA>(e, i, tensor, h);
+    if (e.dtype == KDA_F32) chunk<float, EIGHT, EMA>(e, i, tensor, h);
+    else if (e.dtype == KDA_BF16) chunk<__nv_bfloat16, EIGHT, EMA>(e, i, tensor, h);
+    else chunk<__half, EIGHT, EMA>(e, i, tensor, h);
   }
 }
 
@@ -346,9 +510,9 @@ __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant
     ti = find_tensor(t, ti, c);
     const Entry &e = t.e[ti];
     const int64_t i = (int64_t)(c - e.first) * kChunk + threadIdx.x * kPer;
-    if (e.dtype == KDA_F32) s += squares<float>(e, i);
-    else if (e.dtype == KDA_BF16) s += squares<__nv_bfloat16>(e, i);
-    else s += squares<__half>(e, i);
+    if (e.dtype == KDA_F32) s += squares<float>(e, i) + squares<float>(e, i + kPass);
+    else if (e.dtype == KDA_BF16) s += squares<__nv_bfloat16>(e, i) + squares<__nv_bfloat16>(e, i + kPass);
+    else s += squares<__half>(e, i) + squares<__half>(e, i + kPass);
   }
   s = block_sum(s);
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
@@ -392,7 +556,7 @@ template <bool SIGNED>
 __global__ void __launch_bounds__(kThreads) decode_kernel(int64_t n, const uint8_t *code, const uint8_t *exp,
                                                           __nv_bfloat16 *out, bool vec_ok) {
   for (int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kPer; i < n;
-       i += (int64_t)gridDim.x * kChunk) {
+       i += (int64_t)gridDim.x * kPass) {
     const int k = n - i >= kPer ? kPer : (int)(n - i);
     const bool vec = vec_ok && k == kPer;
     const int e = exp[i / kBlock];
@@ -450,10 +614,10 @@ static int for_tables(const KdaAdamWTensor *x, int64_t count, bool grads_only, b
       e.n = a.numel;
       e.first = (uint32_t)chunks;
       e.dtype = (uint16_t)a.dtype;
-      bool vec = multiple(a.g, 16);
+      const uintptr_t own = a.dtype == KDA_F32 ? 32 : 16, state = eight ? 8 : 32;
+      bool vec = multiple(a.g, own);
       if (!grads_only)
-        vec = vec && multiple(a.p, 16) && multiple(a.m, eight ? 8 : 16) && multiple(a.v, eight ? 8 : 16) &&
-              multiple(a.ema, 16);
+        vec = vec && multiple(a.p, own) && multiple(a.m, state) && multiple(a.v, state) && multiple(a.ema, 32);
       e.vec = vec;
       chunks += more;
       ++t.count;
@@ -616,7 +780,7 @@ int kda_decode_state8(int64_t n, int is_signed, const uint8_t *code, const uint8
   if (!multiple(out, 2)) return KDA_ERR_MISALIGNED;
   const int sms = sm_count();
   if (!sms) return KDA_ERR_CUDA;
-  const int64_t need = (n + kChunk - 1) / kChunk, most = (int64_t)sms * kCtasPerSmRead;
+  const int64_t need = (n + kPass - 1) / kPass, most = (int64_t)sms * kCtasPerSmRead;
   const int grid = (int)(need < most ? need : most);
   const bool vec = multiple(code, 8) && multiple(out, 16);
   cudaStream_t st = (cudaStream_t)stream;
