@@ -285,18 +285,12 @@ __device__ __forceinline__ void update(const Entry &e, int64_t i, uint32_t tenso
 }
 
 // ---- a lane whose eight elements all exist and are aligned: the same with 8-bit states in fewer
-// instructions.  The step is bound by them, not by its 10 bytes an element, so products and sums go
+// instructions.  The step is bound by them, not by its 10 bytes an element, so p's products and sums go
 // two to an instruction, zero codes and values below the least code take branches of their own (rare
 // but in tensors without gradients), and codes are picked from bits 20-27 by bytes. ----
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 d;
   asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}\n"
-      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 d;
-  asm("{\n .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 d, a, b;\n mov.b64 {%0, %1}, d;\n}\n"
       : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
@@ -374,14 +368,19 @@ __device__ __forceinline__ void update8(const Raw<T> &in, const Entry &e, int64_
     decode8<false>(vc, ve0, vx);
   }
   const float nan = __uint_as_float(0x7FC00000u);  // what a block that is not finite decodes to
-  const float2 b1 = both(me0 == 255 ? nan : h.b1), b2 = both(ve0 == 255 ? nan : h.b2);
+  const float b1 = me0 == 255 ? nan : h.b1, b2 = ve0 == 255 ? nan : h.b2;
   float m[kPer], v[kPer];
   uint32_t mtop = 0, vtop = 0;
 #pragma unroll
   for (int j = 0; j < kPer; j += 2) {
-    const float2 gj = mul2(make_float2(g[j], g[j + 1]), both(h.coef));
-    const float2 mj = add2(mul2(make_float2(bf16_of(mx, j), bf16_of(mx, j + 1)), b1), mul2(gj, both(h.b1c)));
-    const float2 vj = add2(mul2(make_float2(bf16_of(vx, j), bf16_of(vx, j + 1)), b2), mul2(mul2(gj, gj), both(h.b2c)));
+    float mv[2][2];
+#pragma unroll
+    for (int l = 0; l < 2; ++l) {  // m and v one by one: ptxas joins a packed product and sum into one rounding
+      const float gl = __fmul_rn(g[j + l], h.coef);
+      mv[0][l] = __fadd_rn(__fmul_rn(bf16_of(mx, j + l), b1), __fmul_rn(gl, h.b1c));
+      mv[1][l] = __fadd_rn(__fmul_rn(bf16_of(vx, j + l), b2), __fmul_rn(__fmul_rn(gl, gl), h.b2c));
+    }
+    const float2 mj = make_float2(mv[0][0], mv[0][1]), vj = make_float2(mv[1][0], mv[1][1]);
     const float2 d = fma2(make_float2(sqrt_fast<true>(vj.x), sqrt_fast<true>(vj.y)), both(h.c2), both(h.eps));
     const float2 s = mul2(mj, both(-h.c1));
     const float2 pj = fma2(make_float2(p[j], p[j + 1]), both(h.decay),

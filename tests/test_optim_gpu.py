@@ -104,6 +104,23 @@ def test_step_matches_the_formulas(cuda, dtype, bits, offset):
         check_step(p, g, m, v, run, dtype, bits, step, 7, emas=emas, ema_decay=0.99)
 
 
+@pytest.mark.parametrize("bits", [8, 32])
+def test_large_tensor_of_many_binades(cuda, bits):
+    """Millions of elements that differ by many binades: values below the least code, and one rounding
+    too few in m or v would show in some codes of a million."""
+    n, gen = 6_000_000, torch.Generator(device=cuda).manual_seed(17)
+    spread = torch.exp2(torch.randn(n, generator=gen, device=cuda) * 2)
+    p, g = torch.randn(n, generator=gen, device=cuda), torch.randn(n, generator=gen, device=cuda) * spread
+    if bits == 8:
+        m, v = optim.zeros_state8(p), optim.zeros_state8(p)
+    else:
+        m, v = torch.zeros_like(p), torch.zeros_like(p)
+    for step in (1, 2, 3):
+        g = g * torch.randn(n, generator=gen, device=cuda)
+        check_step([p], [g], [m], [v], lambda: optim.adamw_step([p], [g], [m], [v], step=step, seed=9, **HYP), "fp32", bits,
+                   step, 9)
+
+
 @pytest.mark.parametrize("count", [1, 64, 65, 449, 1000])
 def test_tables_of_many_tensors(cuda, count):
     """More tensors than a launch holds; the hash goes by the index in the whole list."""
