@@ -9,6 +9,8 @@ pre-norm block with a GELU MLP (``HybridBlock``, :4009-4090), a tubelet embeddin
 classification head.  The recurrence and both gates run in the library's fused kernels
 (``cuda_kda_gated``), the q / k prologue (SiLU + L2 norm) and the output's gated RMSNorm in its
 one-pass row kernels (``rowops``); everything else is PyTorch (cuBLAS GEMMs, elementwise kernels).
+With ``fused_linear`` the output projection takes the residual add and the MLP its bias, GELU and
+residual into the products' own kernels (``linear``).
 
 Parameters follow the reference's initialisation where it sets one: A ~ U[1, 16] as A_log,
 dt_bias = 0, RMSNorm weight 1, conv weights ~ U(+-1/sqrt(K)) with zero bias.
@@ -22,6 +24,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .kda import cuda_kda_gated
+from .linear import linear_act, mlp
 from .rowops import conv_silu, gated_rmsnorm
 
 
@@ -87,7 +90,8 @@ class GatedDeltaLayer(nn.Module):
         self.o_proj = nn.Linear(tot, hidden, bias=False)
         self.fused_rows = True  # conv + SiLU (+ L2 norm) in the library's fused kernels; False: torch ops
 
-    def forward(self, x, state=None):
+    def forward(self, x, state=None, residual=None):
+        """(output, new state); with ``residual`` the output projection adds it in its epilogue."""
         B, L, _ = x.shape
         H, D = self.H, self.D
         bf = torch.bfloat16
@@ -110,14 +114,17 @@ class GatedDeltaLayer(nn.Module):
                                       allow_neg_eigval=self.allow_neg)
         gate = self.g_proj_2(self.g_proj_1(x)).view(B, L, H, D)
         o = self.o_norm(o, gate).reshape(B, L, H * D)
+        if residual is not None:
+            return linear_act(o.to(bf), self.o_proj.weight.to(bf), None, "none", residual.to(bf)), new_state
         return self.o_proj(o), new_state
 
 
 class KDABlock(nn.Module):
     """Pre-norm block: x + layer(LN(x)), x + MLP(LN(x)) (``HybridBlock`` with block_type "gdn")."""
 
-    def __init__(self, dim: int, heads: int, mlp_ratio: float = 4.0, chunk_size: int = 64):
+    def __init__(self, dim: int, heads: int, mlp_ratio: float = 4.0, chunk_size: int = 64, fused_linear: bool = False):
         super().__init__()
+        self.fused_linear = fused_linear  # the library's products (bf16); False: torch ops
         self.norm1 = nn.LayerNorm(dim, eps=1e-6)
         self.layer = GatedDeltaLayer(dim, heads, dim // heads, chunk_size)
         self.norm2 = nn.LayerNorm(dim, eps=1e-6)
@@ -125,6 +132,11 @@ class KDABlock(nn.Module):
         self.mlp = nn.Sequential(nn.Linear(dim, h), nn.GELU(), nn.Linear(h, dim))
 
     def forward(self, x):
+        if self.fused_linear:
+            bf, fc1, fc2 = torch.bfloat16, self.mlp[0], self.mlp[2]
+            x, _ = self.layer(self.norm1(x), residual=x)
+            return mlp(self.norm2(x).to(bf), fc1.weight.to(bf), fc1.bias.to(bf), fc2.weight.to(bf), fc2.bias.to(bf),
+                       "gelu", x)
         y, _ = self.layer(self.norm1(x))
         x = x + y
         return x + self.mlp(self.norm2(x))
@@ -135,10 +147,10 @@ class NoPEGDNVideo(nn.Module):
     linear head.  Input clips are channels-last (B, T, H, W, C) as the reference's loaders give."""
 
     def __init__(self, img_size=224, frames=16, tubelet=(2, 16, 16), in_ch=3, dim=768, depth=12,
-                 heads=12, mlp_ratio=4.0, num_classes=400, chunk_size=64):
+                 heads=12, mlp_ratio=4.0, num_classes=400, chunk_size=64, fused_linear=False):
         super().__init__()
         self.embed = nn.Conv3d(in_ch, dim, kernel_size=tubelet, stride=tubelet)
-        self.blocks = nn.ModuleList(KDABlock(dim, heads, mlp_ratio, chunk_size) for _ in range(depth))
+        self.blocks = nn.ModuleList(KDABlock(dim, heads, mlp_ratio, chunk_size, fused_linear) for _ in range(depth))
         self.norm = nn.LayerNorm(dim, eps=1e-6)
         self.head = nn.Linear(dim, num_classes)
         self.tokens = (frames // tubelet[0]) * (img_size // tubelet[1]) * (img_size // tubelet[2])
