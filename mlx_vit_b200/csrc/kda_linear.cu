@@ -15,6 +15,7 @@
 // to fill the GPU, k is split: each part writes its float32 tile to a workspace and a second kernel
 // adds the parts in order and runs the epilogue.  A few rows (M <= 32) take a kernel of their own
 // that streams the weights once through registers.
+#include <atomic>
 #include <initializer_list>
 
 #include "kda_act.cuh"
@@ -185,12 +186,18 @@ template <> struct Pair<__half> {
 // matrix (a row pitch or a base that 16 bytes do not divide): coalesced 2-byte accesses.
 template <typename T>
 __device__ __forceinline__ void tile_in(uint8_t *st, const T *p, int64_t ld, int rows, int cols, int lane) {
-  for (int r = 0; r < 32; ++r) {
+#pragma unroll 1
+  for (int r0 = 0; r0 < 32; r0 += 8) {
+    T v[8][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = lane + 32 * h;
-      const T v = r < rows && c < cols ? p[r * ld + c] : T(0.f);
-      *reinterpret_cast<T *>(st + chunk_at(r, c >> 3) + (c & 7) * 2) = v;
+    for (int i = 0; i < 16; ++i) {
+      const int r = r0 + (i >> 1), c = lane + 32 * (i & 1);
+      v[i >> 1][i & 1] = r < rows && c < cols ? p[r * ld + c] : T(0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int r = r0 + (i >> 1), c = lane + 32 * (i & 1);
+      *reinterpret_cast<T *>(st + chunk_at(r, c >> 3) + (c & 7) * 2) = v[i >> 1][i & 1];
     }
   }
 }
@@ -738,15 +745,50 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) few_rows_kernel(const FewAr
   }
 }
 
-// dz = dy act'(z) over a [rows][cols] matrix (z null: a copy), any strides and alignments
+// dz = dy act'(z) over a [rows][cols] matrix (z null: a copy), any strides and alignments: a thread takes
+// 8 columns of a row, each matrix by 16 bytes where its rows allow it.  Bound by its bytes.
 template <typename T>
 __global__ void __launch_bounds__(256) act_grad_kernel(int act, int64_t rows, int cols, const T *dy, int64_t ldy, const T *z,
-                                                       int64_t ldz, T *dz, int64_t ldd) {
-  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
-    for (int c = blockIdx.x * 256 + threadIdx.x; c < cols; c += gridDim.x * 256) {
-      float v = to_f<T>(dy[r * ldy + c]);
-      if (z) v *= activate_grad(act, to_f<T>(z[r * ldz + c]));
-      dz[r * ldd + c] = from_f<T>(v);
+                                                       int64_t ldz, T *dz, int64_t ldd, int vec_y, int vec_z, int vec_d) {
+  using P = Pair<T>;
+  auto load = [&](const T *p, bool vec, int k, float (&x)[8]) {
+    if (vec) {
+      const uint4 u = *reinterpret_cast<const uint4 *>(p);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = P::unpack(w[j]);
+        x[2 * j] = f.x;
+        x[2 * j + 1] = f.y;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = j < k ? to_f<T>(p[j]) : 0.f;
+    }
+  };
+  const int groups = (cols + 7) / 8;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < rows * groups; t += (int64_t)gridDim.x * 256) {
+    const int64_t r = t / groups;
+    const int c = (int)(t - r * groups) * 8, k = cols - c;
+    float x[8];
+    load(dy + r * ldy + c, vec_y && k >= 8, k, x);
+    if (z) {
+      float y[8];
+      load(z + r * ldz + c, vec_z && k >= 8, k, y);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 g = activate_grad2(act, make_float2(y[2 * j], y[2 * j + 1]));
+        x[2 * j] *= g.x;
+        x[2 * j + 1] *= g.y;
+      }
+    }
+    T *out = dz + r * ldd + c;
+    if (vec_d && k >= 8) {
+      *reinterpret_cast<uint4 *>(out) = make_uint4(P::pack(x[0], x[1]), P::pack(x[2], x[3]), P::pack(x[4], x[5]), P::pack(x[6], x[7]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < k) out[j] = from_f<T>(x[j]);
     }
   }
 }
@@ -757,10 +799,10 @@ static bool tma_able(const void *p, int64_t ld) { return (uintptr_t)p % 16 == 0 
 static int device_sms() {
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  static int known[64];  // written once with the same value by whoever comes first
-  if (dev < 64 && known[dev]) return known[dev];
+  static std::atomic<int> known[64];
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed))) return n;
   if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  if (dev < 64) known[dev] = n;
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 
@@ -817,7 +859,14 @@ static int launch(Args &g, int sms, cudaStream_t st) {
   };
   g.idesc = idesc(BN, B_MN);
   g.idesc_ones = idesc(kOnesN, false);
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess) return KDA_ERR_CUDA;
+  static std::atomic<uint64_t> allowed{0};  // devices (of the first 64) where the kernel may use that much shared memory
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return KDA_ERR_CUDA;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem) != cudaSuccess) return KDA_ERR_CUDA;
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
   const int64_t count = (int64_t)g.tiles_m * g.tiles_n * g.splits, units = sms / CG;
   if (count > (1ll << 30)) return KDA_ERR_UNSUPPORTED;
   cudaLaunchConfig_t cfg = {};
@@ -1040,15 +1089,20 @@ int kda_act_grad(int dtype, int act, int64_t rows, int64_t cols, const void *dy,
   if (!dy || !dz || !ld_ok(ldy, cols) || !ld_ok(ldd, cols) || (z && !ld_ok(ldz, cols)) || (act != KDA_ACT_NONE && !z))
     return KDA_ERR_INVALID_ARG;
   if (!even({dy, z, dz})) return KDA_ERR_MISALIGNED;
-  const dim3 grid((unsigned)((cols + 255) / 256 < 64 ? (cols + 255) / 256 : 64), (unsigned)(rows < 4096 ? rows : 4096));
+  const int sms = device_sms();
+  if (!sms) return KDA_ERR_CUDA;
+  const int64_t need = (rows * ((cols + 7) / 8) + 255) / 256, most = (int64_t)sms * 8;
+  const unsigned grid = (unsigned)(need < most ? need : most);
+  const int vy = tma_able(dy, ldy), vz = tma_able(z, ldz), vd = tma_able(dz, ldd);  // 16-byte rows
+  const void *zz = act ? z : nullptr;
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == KDA_BF16)
     act_grad_kernel<<<grid, 256, 0, st>>>(act, rows, (int)cols, static_cast<const __nv_bfloat16 *>(dy), ldy,
-                                          static_cast<const __nv_bfloat16 *>(act ? z : nullptr), ldz,
-                                          static_cast<__nv_bfloat16 *>(dz), ldd);
+                                          static_cast<const __nv_bfloat16 *>(zz), ldz, static_cast<__nv_bfloat16 *>(dz), ldd,
+                                          vy, vz, vd);
   else
     act_grad_kernel<<<grid, 256, 0, st>>>(act, rows, (int)cols, static_cast<const __half *>(dy), ldy,
-                                          static_cast<const __half *>(act ? z : nullptr), ldz, static_cast<__half *>(dz), ldd);
+                                          static_cast<const __half *>(zz), ldz, static_cast<__half *>(dz), ldd, vy, vz, vd);
   if (cudaGetLastError() != cudaSuccess) return KDA_ERR_CUDA;
   kda::count_launch();
   return KDA_OK;
