@@ -244,17 +244,19 @@ KDA_API int kda_bwd_noalloc(const KdaDesc *desc, const void *q, const void *k, c
  * Sizes up to 2^30 each.
  *   kda_linear_fwd:    y [M][N] = act(x [M][K] w [N][K]^T + bias [N]) + residual [M][N];
  *                      z [M][N] (may be NULL) receives x w^T + bias, rounded, for the backward
- *   kda_act_grad:      dz = dy act'(z) over [rows][cols]; with KDA_ACT_NONE a copy (z may be NULL),
- *                      which also brings a matrix into the alignment the others need
+ *   kda_act_grad:      dz = dy act'(z) over [rows][cols] and its column sums db [cols]; with KDA_ACT_NONE
+ *                      (z may be NULL) a copy, which also brings a matrix into the alignment the
+ *                      others need; dz may be NULL where the sums alone are wanted
  *   kda_linear_dgrad:  dx [M][K] = dz [M][N] w [N][K]; with an activation times act'(z [M][K]), the
- *                      saved input of the activation that x came from
- *   kda_linear_wgrad:  dw [N][K] = dz^T x, db [N] = column sums of dz (needs a workspace)
+ *                      saved input of the activation that x came from; db [K]: dx's column sums
+ *   kda_linear_wgrad:  dw [N][K] = dz^T x
  * bias, residual and db may be NULL.  kda_linear_workspace_bytes says what workspace (16-byte
- * aligned) a call on the current device takes (op: KDA_LINEAR_*); with ws NULL a product whose
- * tiles do not fill the GPU is not split along its sum, and takes longer.  Counterpart: the
+ * aligned) a call on the current device takes (op: KDA_LINEAR_*, KDA_LINEAR_ACT_GRAD with M rows and
+ * N columns); db needs it, and with ws NULL a product whose tiles do not fill the GPU is not split along
+ * its sum, and takes longer.  Results do not depend on the order in which blocks run.  Counterpart: the
  * nn.Linear layers of the reference's blocks and their MLP (HybridBlock, nope_gdn_mlx.py:4009-4090). */
 enum kda_act { KDA_ACT_NONE = 0, KDA_ACT_RELU = 1, KDA_ACT_SILU = 2, KDA_ACT_GELU = 3, KDA_ACT_GELU_TANH = 4 };
-enum kda_linear_op { KDA_LINEAR_FWD = 0, KDA_LINEAR_DGRAD = 1, KDA_LINEAR_WGRAD = 2 };
+enum kda_linear_op { KDA_LINEAR_FWD = 0, KDA_LINEAR_DGRAD = 1, KDA_LINEAR_WGRAD = 2, KDA_LINEAR_ACT_GRAD = 3 };
 
 KDA_API size_t kda_linear_workspace_bytes(int op, int64_t M, int64_t N, int64_t K, int with_db);
 KDA_API int kda_linear_fwd(int dtype, int act, int64_t M, int64_t N, int64_t K, const void *x, int64_t ldx,
@@ -262,12 +264,13 @@ KDA_API int kda_linear_fwd(int dtype, int act, int64_t M, int64_t N, int64_t K, 
                            void *y, int64_t ldy, void *z, int64_t ldz, void *ws, size_t ws_bytes, void *stream);
 KDA_API int kda_linear_dgrad(int dtype, int act, int64_t M, int64_t N, int64_t K, const void *dz, int64_t ldd,
                              const void *w, int64_t ldw, const void *z, int64_t ldz, void *dx, int64_t ldx,
-                             void *ws, size_t ws_bytes, void *stream);
+                             void *db, void *ws, size_t ws_bytes, void *stream);
 KDA_API int kda_linear_wgrad(int dtype, int64_t M, int64_t N, int64_t K, const void *dz, int64_t ldd,
-                             const void *x, int64_t ldx, void *dw, int64_t ldw, void *db, void *ws,
-                             size_t ws_bytes, void *stream);
+                             const void *x, int64_t ldx, void *dw, int64_t ldw, void *ws, size_t ws_bytes,
+                             void *stream);
 KDA_API int kda_act_grad(int dtype, int act, int64_t rows, int64_t cols, const void *dy, int64_t ldy,
-                         const void *z, int64_t ldz, void *dz, int64_t ldd, void *stream);
+                         const void *z, int64_t ldz, void *dz, int64_t ldd, void *db, void *ws,
+                         size_t ws_bytes, void *stream);
 
 /* ---- AdamW over many tensors at once ----
  * One tensor of the step.  p (updated) and g have dtype `dtype`, numel contiguous elements each.

@@ -15,7 +15,7 @@ LIB_PATH = os.path.join(_HERE, "libkda_b200.so")
 KDA_ABI_VERSION = 7
 KDA_F32, KDA_BF16, KDA_F16 = 0, 1, 2
 KDA_ACT_NONE, KDA_ACT_RELU, KDA_ACT_SILU, KDA_ACT_GELU, KDA_ACT_GELU_TANH = range(5)
-KDA_LINEAR_FWD, KDA_LINEAR_DGRAD, KDA_LINEAR_WGRAD = range(3)
+KDA_LINEAR_FWD, KDA_LINEAR_DGRAD, KDA_LINEAR_WGRAD, KDA_LINEAR_ACT_GRAD = range(4)
 KDA_FLAG_FORCE_GENERIC = 0x1
 KDA_FLAG_DEBUG_WAIT_TIMEOUT = 0x2
 
@@ -126,9 +126,9 @@ def _declare(L):
                  ("kda_grad_norm", [P, i64, P, P, S, P]),
                  ("kda_decode_state8", [i64, I, P, P, P, P]),
                  ("kda_linear_fwd", [I, I, i64, i64, i64, P, i64, P, i64, P, P, i64, P, i64, P, i64, P, S, P]),
-                 ("kda_linear_dgrad", [I, I, i64, i64, i64, P, i64, P, i64, P, i64, P, i64, P, S, P]),
-                 ("kda_linear_wgrad", [I, i64, i64, i64, P, i64, P, i64, P, i64, P, P, S, P]),
-                 ("kda_act_grad", [I, I, i64, i64, P, i64, P, i64, P, i64, P])):
+                 ("kda_linear_dgrad", [I, I, i64, i64, i64, P, i64, P, i64, P, i64, P, i64, P, P, S, P]),
+                 ("kda_linear_wgrad", [I, i64, i64, i64, P, i64, P, i64, P, i64, P, S, P]),
+                 ("kda_act_grad", [I, I, i64, i64, P, i64, P, i64, P, i64, P, P, S, P])):
         getattr(L, n).restype = I
         getattr(L, n).argtypes = a
 

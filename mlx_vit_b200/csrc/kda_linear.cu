@@ -3,7 +3,11 @@
 //
 //   forward   y  = act(x W^T + bias) + residual, and z = x W^T + bias kept for the backward
 //   dgrad     dx = dz W,  or  (dz W) * act'(z) where an activation lies below
-//   wgrad     dW = dz^T x,  db = the column sums of dz
+//   wgrad     dW = dz^T x
+//
+// and db, the column sums of dz, from the pass that makes dz (dgrad's epilogue, or the activation-gradient
+// pass).  (A product of dz^T with ones beside dW summed them without another pass, but each change
+// between the two accumulators cost the tensor cores some 100 ns: 90 us against 76 for dW of 4096 x 1024.)
 //
 // One kernel: C[m][n] = sum_k A[m][k] B[n][k] over tiles of 128 CG x BN, where each operand lies in
 // memory k-contiguous ("K-major") or m- / n-contiguous ("MN-major": the transposes are read in
@@ -35,7 +39,6 @@ constexpr int kEpiWarp = 4, kEpiWarps = 16;
 constexpr int kBlockK = 64;       // k per stage: 128 bytes, the swizzle's width
 constexpr int kStageA = 128 * 128;
 constexpr int kStaging = kEpiWarps * 4096;  // a 32 x 64 tile a warp
-constexpr int kOnesN = 32;        // columns of the product with ones that sums dz's columns
 constexpr int kSmemMax = 232448;
 constexpr int kPolls = 1 << 20;   // bound of a wait: some tens of milliseconds and more, against microseconds of work
 
@@ -47,23 +50,20 @@ struct alignas(64) Args {
   const void *bias, *in_ptr;
   void *out_ptr, *z_ptr;
   float *part;          // split: [splits][tiles_m 128 CG][ldp] partial products
-  float *sums;          // ONES: [splits tiles_n][m] partial column sums of A
+  float *sums;          // [32-row groups][n] column sums of what the epilogue writes, or null
   int m, n, k, tiles_m, tiles_n, splits, per_split;  // per_split: blocks of 64 k a part takes
-  uint32_t idesc, idesc_ones;
-  int act, in_kind, out_tma, in_tma, save_z, sum_first;
-  void *db;             // ONES, sum_first: where the sums go
+  uint32_t idesc;
+  int act, in_kind, out_tma, in_tma, save_z;
 };
 
-template <int CG, int BN, bool ONES>
+template <int CG, int BN>
 struct Shape {
   static constexpr int kStageB = BN / CG * 128;
   static constexpr int kStage = kStageA + kStageB;
-  static constexpr int kOnes = ONES ? kOnesN / CG * 128 : 0;
-  static constexpr int kFixed = kStaging + kOnes + kEpiWarps * 128 + 512;
+  static constexpr int kFixed = kStaging + kEpiWarps * 128 + 512;
   static constexpr int kStages = (kSmemMax - kFixed) / kStage < 8 ? (kSmemMax - kFixed) / kStage : 8;
-  static constexpr int kAcc = BN + (ONES ? kOnesN : 0);   // tensor-memory columns of one accumulator
-  static constexpr int kBufs = 2 * kAcc <= 512 ? 2 : 1;
-  static constexpr int kCols = kBufs * kAcc <= 128 ? 128 : kBufs * kAcc <= 256 ? 256 : 512;
+  static constexpr int kBufs = 2;           // accumulators of BN tensor-memory columns
+  static constexpr int kCols = kBufs * BN;  // 128, 256 or 512: a power of two, as allocations are
   static constexpr int kSmem = kStages * kStage + kFixed;
 };
 
@@ -287,10 +287,9 @@ __device__ __forceinline__ int2 place(int t, int tiles_m, int tiles_n) {
   return make_int2(group * kGroup + in % rows, in / rows);
 }
 
-template <typename T, int CG, int BN, bool A_MN, bool B_MN, bool ONES>
+template <typename T, int CG, int BN, bool A_MN, bool B_MN>
 __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant__ Args g) {
-  using S = Shape<CG, BN, ONES>;
-  using P = Pair<T>;
+  using S = Shape<CG, BN>;
   extern __shared__ __align__(1024) uint8_t sm[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0;
@@ -299,8 +298,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     if (tid == 0) atomicExch(&g_linear_status, KDA_ERR_MISALIGNED);
     return;
   }
-  uint8_t *staging = sm + S::kStages * S::kStage, *ones = staging + kStaging;
-  T *bias_sm = reinterpret_cast<T *>(ones + S::kOnes);
+  uint8_t *staging = sm + S::kStages * S::kStage;
+  T *bias_sm = reinterpret_cast<T *>(staging + kStaging);
   // barriers: full[stages], empty[stages], acc_full[2], acc_empty[2], in[epilogue warps]; then tensor memory's address
   const uint32_t bars = smem_u32(bias_sm) + kEpiWarps * 128;
   const uint32_t full = bars, empty = full + 8 * S::kStages, acc_full = empty + 8 * S::kStages,
@@ -320,8 +319,6 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     for (int w = 0; w < kEpiWarps; ++w) mbar_init(in_bar + 8 * w, 1);
     mbar_fence_init();
   }
-  if (ONES)
-    for (int i = tid; i < S::kOnes / 4; i += kThreads) reinterpret_cast<uint32_t *>(ones)[i] = P::pack(1.f, 1.f);
   if (warp == 2) alloc<CG>(tmem_at, S::kCols);
   fence_proxy_async_smem();
   tc_fence_before();
@@ -370,36 +367,25 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     if (rank == 0) {
       // ---- products ----
       const uint32_t a_low = desc_low<A_MN>(base), b_low = desc_low<B_MN>(base + kStageA);
-      const uint32_t ones_low = desc_low<false>(smem_u32(ones));
       uint32_t s = 0, ph = 0, n = 0;
       for (int u = first; ok && u < units; u += step, ++n) {
-        const int t = u % tiles, kb0 = u / tiles * g.per_split, kb1 = min(kblocks, kb0 + g.per_split);
+        const int kb0 = u / tiles * g.per_split, kb1 = min(kblocks, kb0 + g.per_split);
         const uint32_t buf = n % S::kBufs, use = n / S::kBufs;
-        const uint32_t d = tmem + buf * S::kAcc;
+        const uint32_t d = tmem + buf * BN;
         if (!(ok = wait(acc_empty + 8 * buf, (use & 1) ^ 1))) break;
         tc_fence_after();
-        const int tn = ONES ? place(t, g.tiles_m, g.tiles_n).y : 0;
-        bool summed = false;
         for (int kb = kb0; kb < kb1; ++kb) {
           if (!(ok = wait(full + 8 * s, ph))) break;
           tc_fence_after();
           const uint32_t al = a_low + s * (S::kStage >> 4), bl = b_low + s * (S::kStage >> 4);
-          // the column sums: the first column tile's, or each column tile's share
-          const bool sum = ONES && (g.sum_first ? tn == 0 : kb % g.tiles_n == tn);
           if (elect()) {
 #pragma unroll
             for (int k = 0; k < kBlockK / 16; ++k)
               mma<CG>(d, al + k * kDescStep<A_MN>, bl + k * kDescStep<B_MN>, g.idesc, kb > kb0 || k > 0);
-            if (sum) {
-#pragma unroll
-              for (int k = 0; k < kBlockK / 16; ++k)
-                mma<CG>(d + BN, al + k * kDescStep<A_MN>, ones_low, g.idesc_ones, summed || k > 0);
-            }
             commit<CG>(empty + 8 * s);
             if (kb + 1 == kb1) commit<CG>(acc_full + 8 * buf);
           }
           __syncwarp();
-          summed |= sum;
           if (++s == S::kStages) s = 0, ph ^= 1;
         }
       }
@@ -418,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       const int t = u % tiles, part = u / tiles;
       const uint32_t buf = n % S::kBufs, use = n / S::kBufs;
       const int2 at_tile = place(t, g.tiles_m, g.tiles_n);
-      const int tn = at_tile.y, row0 = at_tile.x * 128 * CG + (int)rank * 128 + 32 * q, col0 = tn * BN + 64 * c;
+      const int row0 = at_tile.x * 128 * CG + (int)rank * 128 + 32 * q, col0 = at_tile.y * BN + 64 * c;
       const bool mine = c < BN / 64 && row0 < g.m && col0 < g.n;
       const int rows = min(32, g.m - row0), cols = min(64, g.n - col0);
       auto fetch = [&] {  // residual or z into the staging tile (one lane)
@@ -446,22 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
         break;
       }
       tc_fence_after();
-      const uint32_t acc = tmem + buf * S::kAcc + ((uint32_t)(32 * q) << 16);
-      if (ONES && c == 0 && (!g.sum_first || tn == 0)) {
-        uint32_t v;
-        asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n" : "=r"(v) : "r"(acc + BN));
-        tmem_wait_ld();
-        const float f = __uint_as_float(v);
-        if (row0 + lane < g.m) {
-          if (g.sum_first) {
-            static_cast<T *>(g.db)[row0 + lane] = from_f<T>(f);
-          } else {
-            const int kb0 = part * g.per_split, kb1 = min(kblocks, kb0 + g.per_split);
-            const int some = kb0 + ((tn - kb0) % g.tiles_n + g.tiles_n) % g.tiles_n;  // first block this column tile sums
-            g.sums[((int64_t)part * g.tiles_n + tn) * g.m + row0 + lane] = some < kb1 ? f : 0.f;
-          }
-        }
-      }
+      const uint32_t acc = tmem + buf * BN + ((uint32_t)(32 * q) << 16);
       if (mine && g.splits > 1) {  // the float32 tile as it is, 32 columns a store
         const int prow = part * g.tiles_m * 128 * CG + row0;
 #pragma unroll
@@ -519,6 +490,15 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
         }
         fence_proxy_async_smem();
         __syncwarp();
+        if (B_MN && !A_MN && g.sums) {  // of columns 2 lane, 2 lane + 1 over the rows there are
+          float2 sum = both(0.f);
+#pragma unroll 8
+          for (int r = 0; r < rows; ++r)
+            sum = add2(sum, Pair<T>::unpack(*reinterpret_cast<const uint32_t *>(st + chunk_at(r, lane >> 2) + 4 * (lane & 3))));
+          float *to = g.sums + (int64_t)(row0 >> 5) * g.n + col0 + 2 * lane;
+          if (2 * lane < cols) to[0] = sum.x;
+          if (2 * lane + 1 < cols) to[1] = sum.y;
+        }
         if (g.out_tma) {
           if (lane == 0) {
             store_box(&g.out, st_at, col0, row0);
@@ -546,22 +526,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   if (warp == 2) dealloc<CG>(tmem, S::kCols);
 }
 
-// Adds the parts of a split product in their order and runs the epilogue; the blocks behind the
-// last row of blocks add the partial column sums.
+// Adds the parts of a split product in their order and runs the epilogue.
 constexpr int kJoinRows = 4;  // rows a block of 64 x 4 threads takes; a thread takes 8 columns
 template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args g, int64_t part_rows, int col_blocks,
-                                                   int64_t tile_blocks, int parts, T *db) {
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args g, int64_t part_rows, int col_blocks) {
   using P = Pair<T>;
   const int64_t blk = blockIdx.x;
-  if (blk >= tile_blocks) {  // db[j] = sum over the partials
-    const int64_t j = (blk - tile_blocks) * 256 + threadIdx.y * 64 + threadIdx.x;
-    if (j >= g.m) return;
-    float s = 0.f;
-    for (int i = 0; i < parts; ++i) s += g.sums[(int64_t)i * g.m + j];
-    db[j] = from_f<T>(s);
-    return;
-  }
   const int64_t row = blk / col_blocks * kJoinRows + threadIdx.y;
   const int col = (int)(blk % col_blocks) * 512 + threadIdx.x * 8;
   if (row >= g.m || col >= g.n) return;
@@ -745,11 +715,14 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) few_rows_kernel(const FewAr
   }
 }
 
-// dz = dy act'(z) over a [rows][cols] matrix (z null: a copy), any strides and alignments: a thread takes
-// 8 columns of a row, each matrix by 16 bytes where its rows allow it.  Bound by its bytes.
-template <typename T>
+// dz = dy act'(z) over a [rows][cols] matrix (z null: a copy; dz null: none), any strides and alignments, and
+// the column sums of dz.  A block takes 256 columns, 8 a thread (each matrix by 16 bytes where its
+// rows allow it), of a range of rows, 8 at a time; its sums meet in shared memory and go to its row of
+// partials.  Bound by its bytes.
+template <typename T, bool SUMS>
 __global__ void __launch_bounds__(256) act_grad_kernel(int act, int64_t rows, int cols, const T *dy, int64_t ldy, const T *z,
-                                                       int64_t ldz, T *dz, int64_t ldd, int vec_y, int vec_z, int vec_d) {
+                                                       int64_t ldz, T *dz, int64_t ldd, int vec_y, int vec_z, int vec_d,
+                                                       float *part, T *db) {
   using P = Pair<T>;
   auto load = [&](const T *p, bool vec, int k, float (&x)[8]) {
     if (vec) {
@@ -766,31 +739,71 @@ __global__ void __launch_bounds__(256) act_grad_kernel(int act, int64_t rows, in
       for (int j = 0; j < 8; ++j) x[j] = j < k ? to_f<T>(p[j]) : 0.f;
     }
   };
-  const int groups = (cols + 7) / 8;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < rows * groups; t += (int64_t)gridDim.x * 256) {
-    const int64_t r = t / groups;
-    const int c = (int)(t - r * groups) * 8, k = cols - c;
-    float x[8];
-    load(dy + r * ldy + c, vec_y && k >= 8, k, x);
-    if (z) {
-      float y[8];
-      load(z + r * ldz + c, vec_z && k >= 8, k, y);
+  const int c = blockIdx.x * 256 + threadIdx.x * 8, k = cols - c;
+  float sum[8] = {};
+  if (k > 0) {
+#pragma unroll 4
+    for (int64_t r = (int64_t)blockIdx.y * 8 + threadIdx.y; r < rows; r += (int64_t)gridDim.y * 8) {
+      float x[8];
+      load(dy + r * ldy + c, vec_y && k >= 8, k, x);
+      if (z) {
+        float y[8];
+        load(z + r * ldz + c, vec_z && k >= 8, k, y);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 g = activate_grad2(act, make_float2(y[2 * j], y[2 * j + 1]));
-        x[2 * j] *= g.x;
-        x[2 * j + 1] *= g.y;
+        for (int j = 0; j < 4; ++j) {
+          const float2 g = activate_grad2(act, make_float2(y[2 * j], y[2 * j + 1]));
+          x[2 * j] *= g.x;
+          x[2 * j + 1] *= g.y;
+        }
+      }
+      if (SUMS) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] += x[j];
+      }
+      if (dz) {
+        T *out = dz + r * ldd + c;
+        if (vec_d && k >= 8) {
+          *reinterpret_cast<uint4 *>(out) = make_uint4(P::pack(x[0], x[1]), P::pack(x[2], x[3]), P::pack(x[4], x[5]), P::pack(x[6], x[7]));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j < k) out[j] = from_f<T>(x[j]);
+        }
       }
     }
-    T *out = dz + r * ldd + c;
-    if (vec_d && k >= 8) {
-      *reinterpret_cast<uint4 *>(out) = make_uint4(P::pack(x[0], x[1]), P::pack(x[2], x[3]), P::pack(x[4], x[5]), P::pack(x[6], x[7]));
-    } else {
+  }
+  if (SUMS) {
+    __shared__ float red[8][256 + 8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < k) out[j] = from_f<T>(x[j]);
+    for (int j = 0; j < 8; ++j) red[threadIdx.y][threadIdx.x * 8 + j] = sum[j];
+    __syncthreads();
+    const int t = threadIdx.y * 32 + threadIdx.x, col = blockIdx.x * 256 + t;
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v += red[i][t];
+    if (col < cols) {
+      if (gridDim.y == 1) db[col] = from_f<T>(v);  // no other partials
+      else part[(int64_t)blockIdx.y * cols + col] = v;
     }
   }
+}
+// db[j] = sum over the partials, each thread row every 32nd of them, in their order
+template <typename T>
+__global__ void __launch_bounds__(1024) sums_kernel(const float *part, int parts, int cols, T *db) {
+  __shared__ float red[32][33];
+  const int j = blockIdx.x * 32 + threadIdx.x;
+  float s = 0.f;
+  if (j < cols) {
+#pragma unroll 4
+    for (int i = threadIdx.y; i < parts; i += 32) s += part[(int64_t)i * cols + j];
+  }
+  red[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  s = red[threadIdx.x][threadIdx.y];  // column 32 block + y, its partial sum x
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+  const int col = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && col < cols) db[col] = from_f<T>(s);
 }
 
 // ---- host side ----
@@ -842,23 +855,47 @@ static int64_t part_cols(const Plan &p, int64_t n) { return (n + p.bn - 1) / p.b
 static size_t part_bytes(const Plan &p, int64_t m, int64_t n) {
   return p.splits > 1 ? (size_t)p.splits * part_rows(p, m) * part_cols(p, n) * sizeof(float) : 0;
 }
-static size_t sums_bytes(const Plan &p, int64_t m, int64_t n) {
-  return ((size_t)p.splits * ((n + p.bn - 1) / p.bn) * m * sizeof(float) + 15) / 16 * 16;
+static size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+// partial column sums of an [m][n] result: a row for every 32 of its rows
+static size_t sums_bytes(int64_t m, int64_t n) { return round16((size_t)((m + 31) / 32) * n * sizeof(float)); }
+// ... and of the activation-gradient pass: a row for every block of rows
+static int row_blocks(int64_t rows, int64_t cols, int sms) {
+  const int64_t across = (cols + 255) / 256, most = (8ll * sms + across - 1) / across, need = (rows + 63) / 64;
+  return (int)(need < most ? need : most);
+}
+template <typename T>
+static int add_sums(const float *part, int parts, int cols, void *db, cudaStream_t st) {
+  sums_kernel<T><<<(cols + 31) / 32, dim3(32, 32), 0, st>>>(part, parts, cols, static_cast<T *>(db));
+  if (cudaGetLastError() != cudaSuccess) return KDA_ERR_CUDA;
+  count_launch();
+  return KDA_OK;
+}
+template <typename T>
+static int act_grad(int act, int64_t rows, int64_t cols, const void *dy, int64_t ldy, const void *z, int64_t ldz, void *dz,
+                    int64_t ldd, void *db, void *ws, int sms, cudaStream_t st) {
+  const int blocks = row_blocks(rows, cols, sms);
+  const dim3 grid((unsigned)((cols + 255) / 256), (unsigned)blocks), block(32, 8);
+  const T *y = static_cast<const T *>(dy), *zz = static_cast<const T *>(act ? z : nullptr);
+  T *out = static_cast<T *>(dz);
+  const int vy = tma_able(dy, ldy), vz = tma_able(z, ldz), vd = tma_able(dz, ldd);  // 16-byte rows
+  float *part = static_cast<float *>(ws);
+  if (db) act_grad_kernel<T, true><<<grid, block, 0, st>>>(act, rows, (int)cols, y, ldy, zz, ldz, out, ldd, vy, vz, vd, part,
+                                                            static_cast<T *>(db));
+  else act_grad_kernel<T, false><<<grid, block, 0, st>>>(act, rows, (int)cols, y, ldy, zz, ldz, out, ldd, vy, vz, vd, nullptr, nullptr);
+  if (cudaGetLastError() != cudaSuccess) return KDA_ERR_CUDA;
+  count_launch();
+  return db && blocks > 1 ? add_sums<T>(part, blocks, (int)cols, db, st) : KDA_OK;
 }
 
-template <typename T, int CG, int BN, bool A_MN, bool B_MN, bool ONES>
+template <typename T, int CG, int BN, bool A_MN, bool B_MN>
 static int launch(Args &g, int sms, cudaStream_t st) {
-  using S = Shape<CG, BN, ONES>;
-  auto kernel = gemm_kernel<T, CG, BN, A_MN, B_MN, ONES>;
+  using S = Shape<CG, BN>;
+  auto kernel = gemm_kernel<T, CG, BN, A_MN, B_MN>;
   g.tiles_m = (g.m + 128 * CG - 1) / (128 * CG);
   g.tiles_n = (g.n + BN - 1) / BN;
   constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-  auto idesc = [&](int n, bool b_mn) {
-    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)A_MN << 15) | ((uint32_t)b_mn << 16) |
-           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
-  };
-  g.idesc = idesc(BN, B_MN);
-  g.idesc_ones = idesc(kOnesN, false);
+  g.idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16) |
+            ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(128 * CG >> 4) << 24);
   static std::atomic<uint64_t> allowed{0};  // devices (of the first 64) where the kernel may use that much shared memory
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return KDA_ERR_CUDA;
@@ -886,8 +923,9 @@ static int launch(Args &g, int sms, cudaStream_t st) {
   return KDA_OK;
 }
 
-// One product: the tiles (and parts), then whatever of parts and column sums is left to add.
-template <typename T, bool A_MN, bool B_MN, bool ONES>
+// One product: the tiles (and parts), then whatever of parts and column sums is left to add.  The
+// workspace holds the column sums' partials, then the parts.
+template <typename T, bool A_MN, bool B_MN>
 static int run(Args &g, const Plan &p, const void *a, int64_t lda, const void *b, int64_t ldb, void *ws, void *db, int sms,
                cudaStream_t st) {
   int s;
@@ -896,33 +934,30 @@ static int run(Args &g, const Plan &p, const void *a, int64_t lda, const void *b
   g.splits = p.splits;
   g.per_split = p.per_split;
   char *at = static_cast<char *>(ws);
-  if (ONES) {
+  if (db) {
     g.sums = reinterpret_cast<float *>(at);
-    at += sums_bytes(p, g.m, g.n);
+    at += sums_bytes(g.m, g.n);
   }
-  // One CTA on a tile waits for its operands' copies, and the first column tile has the tensor cores'
-  // time for all sums; a pair is bound by them, so its column tiles share the sums and they are
-  // added afterwards (as they are where k is split).
-  g.sum_first = ONES && p.cg == 1 && p.splits == 1;
-  g.db = db;
   const int64_t rows = part_rows(p, g.m);
   if (p.splits > 1) {
     g.part = reinterpret_cast<float *>(at);
     g.ldp = part_cols(p, g.n);
     if ((s = tma_map_rows32(&g.out, at, p.splits * rows, g.ldp, g.ldp, 32))) return s;
   }
-  s = p.cg == 2    ? launch<T, 2, 256, A_MN, B_MN, ONES>(g, sms, st)
-      : p.bn == 128 ? launch<T, 1, 128, A_MN, B_MN, ONES>(g, sms, st)
-                    : launch<T, 1, 64, A_MN, B_MN, ONES>(g, sms, st);
-  if (s || (p.splits == 1 && (!ONES || g.sum_first))) return s;
-  const int col_blocks = (g.n + 511) / 512;
-  const int64_t tile_blocks = p.splits > 1 ? (int64_t)((g.m + kJoinRows - 1) / kJoinRows) * col_blocks : 0;
-  const int64_t blocks = tile_blocks + (ONES ? (g.m + 255) / 256 : 0);
-  join_kernel<T><<<(unsigned)blocks, dim3(64, 4), 0, st>>>(g, rows, col_blocks, tile_blocks, p.splits * g.tiles_n,
-                                                           static_cast<T *>(db));
-  if (cudaGetLastError() != cudaSuccess) return KDA_ERR_CUDA;
-  count_launch();
-  return KDA_OK;
+  s = p.cg == 2    ? launch<T, 2, 256, A_MN, B_MN>(g, sms, st)
+      : p.bn == 128 ? launch<T, 1, 128, A_MN, B_MN>(g, sms, st)
+                    : launch<T, 1, 64, A_MN, B_MN>(g, sms, st);
+  if (s) return s;
+  if (p.splits > 1) {
+    const int col_blocks = (g.n + 511) / 512;
+    join_kernel<T><<<(unsigned)((int64_t)((g.m + kJoinRows - 1) / kJoinRows) * col_blocks), dim3(64, 4), 0, st>>>(g, rows, col_blocks);
+    if (cudaGetLastError() != cudaSuccess) return KDA_ERR_CUDA;
+    count_launch();
+    // the joined result's sums: a pass over it
+    if (db)
+      return act_grad<T>(KDA_ACT_NONE, g.m, g.n, g.out_ptr, g.ldo, nullptr, 0, nullptr, 0, db, g.sums, sms, st);
+  }
+  return db ? add_sums<T>(g.sums, (g.m + 31) / 32, g.n, db, st) : KDA_OK;
 }
 
 template <typename T, int MT, int NB>
@@ -973,7 +1008,7 @@ static bool even(std::initializer_list<const void *> ps) {
 // The plan for a product, and whether the workspace holds it; without one k is not split.
 static int plan_in(Plan &p, int64_t m, int64_t n, int64_t k, int sms, bool sums, const void *ws, size_t ws_bytes) {
   p = plan_for(m, n, k, sms, ws != nullptr);
-  const size_t need = part_bytes(p, m, n) + (sums ? sums_bytes(p, m, n) : 0);
+  const size_t need = part_bytes(p, m, n) + (sums ? sums_bytes(m, n) : 0);
   return need && (!ws || (uintptr_t)ws % 16 || ws_bytes < need) ? KDA_ERR_WORKSPACE : KDA_OK;
 }
 
@@ -999,10 +1034,10 @@ size_t kda_linear_workspace_bytes(int op, int64_t M, int64_t N, int64_t K, int w
   int sms = device_sms();
   if (!sms) sms = 148;  // no device: the size on a B200
   if (op == KDA_LINEAR_FWD) return M <= kFewRows ? 0 : part_bytes(plan_for(M, N, K, sms, true), M, N);
-  if (op == KDA_LINEAR_DGRAD) return part_bytes(plan_for(M, K, N, sms, true), M, K);
-  if (op != KDA_LINEAR_WGRAD) return 0;
-  const Plan p = plan_for(N, K, M, sms, true);
-  return part_bytes(p, N, K) + (with_db ? sums_bytes(p, N, K) : 0);
+  if (op == KDA_LINEAR_DGRAD) return part_bytes(plan_for(M, K, N, sms, true), M, K) + (with_db ? sums_bytes(M, K) : 0);
+  if (op == KDA_LINEAR_WGRAD) return part_bytes(plan_for(N, K, M, sms, true), N, K);
+  if (op == KDA_LINEAR_ACT_GRAD) return with_db ? round16((size_t)row_blocks(M, N, sms) * N * sizeof(float)) : 0;
+  return 0;
 }
 
 int kda_linear_fwd(int dtype, int act, int64_t M, int64_t N, int64_t K, const void *x, int64_t ldx, const void *w,
@@ -1034,78 +1069,66 @@ int kda_linear_fwd(int dtype, int act, int64_t M, int64_t N, int64_t K, const vo
     g.ldz = ldz;
     if ((s = kda::tma_map_rows16(&g.z, z, M, N, ldz, 32))) return s;
   }
-  return dtype == KDA_BF16 ? run<__nv_bfloat16, false, false, false>(g, p, x, ldx, w, ldw, ws, nullptr, sms, st)
-                           : run<__half, false, false, false>(g, p, x, ldx, w, ldw, ws, nullptr, sms, st);
+  return dtype == KDA_BF16 ? run<__nv_bfloat16, false, false>(g, p, x, ldx, w, ldw, ws, nullptr, sms, st)
+                           : run<__half, false, false>(g, p, x, ldx, w, ldw, ws, nullptr, sms, st);
 }
 
 int kda_linear_dgrad(int dtype, int act, int64_t M, int64_t N, int64_t K, const void *dz, int64_t ldd, const void *w,
-                     int64_t ldw, const void *z, int64_t ldz, void *dx, int64_t ldx, void *ws, size_t ws_bytes,
-                     void *stream) {
+                     int64_t ldw, const void *z, int64_t ldz, void *dx, int64_t ldx, void *db, void *ws,
+                     size_t ws_bytes, void *stream) {
   int s = check(dtype, act, M, N, K);
   if (s) return s;
   if (!dz || !w || !dx || !ld_ok(ldd, N) || !ld_ok(ldw, K) || !ld_ok(ldx, K) || (z && !ld_ok(ldz, K)) ||
       (act != KDA_ACT_NONE && !z))
     return KDA_ERR_INVALID_ARG;
-  if (!tma_able(dz, ldd) || !tma_able(w, ldw) || !even({z, dx})) return KDA_ERR_MISALIGNED;
+  if (!tma_able(dz, ldd) || !tma_able(w, ldw) || !even({z, dx, db})) return KDA_ERR_MISALIGNED;
+  if (db && !ws) return KDA_ERR_WORKSPACE;
   const int sms = device_sms();
   if (!sms) return KDA_ERR_CUDA;
   Plan p;
-  if ((s = plan_in(p, M, K, N, sms, 0, ws, ws_bytes))) return s;
+  if ((s = plan_in(p, M, K, N, sms, db != nullptr, ws, ws_bytes))) return s;
   Args g = {};
   g.m = (int)M; g.n = (int)K; g.k = (int)N; g.act = act;
   if ((s = set_out(g, dx, ldx))) return s;
   if (act != KDA_ACT_NONE && (s = set_in(g, kInActGrad, z, ldz))) return s;
   cudaStream_t st = (cudaStream_t)stream;
-  return dtype == KDA_BF16 ? run<__nv_bfloat16, false, true, false>(g, p, dz, ldd, w, ldw, ws, nullptr, sms, st)
-                           : run<__half, false, true, false>(g, p, dz, ldd, w, ldw, ws, nullptr, sms, st);
+  return dtype == KDA_BF16 ? run<__nv_bfloat16, false, true>(g, p, dz, ldd, w, ldw, ws, db, sms, st)
+                           : run<__half, false, true>(g, p, dz, ldd, w, ldw, ws, db, sms, st);
 }
 
 int kda_linear_wgrad(int dtype, int64_t M, int64_t N, int64_t K, const void *dz, int64_t ldd, const void *x, int64_t ldx,
-                     void *dw, int64_t ldw, void *db, void *ws, size_t ws_bytes, void *stream) {
+                     void *dw, int64_t ldw, void *ws, size_t ws_bytes, void *stream) {
   int s = check(dtype, KDA_ACT_NONE, M, N, K);
   if (s) return s;
   if (!dz || !x || !dw || !ld_ok(ldd, N) || !ld_ok(ldx, K) || !ld_ok(ldw, K)) return KDA_ERR_INVALID_ARG;
-  if (!tma_able(dz, ldd) || !tma_able(x, ldx) || !even({dw, db})) return KDA_ERR_MISALIGNED;
+  if (!tma_able(dz, ldd) || !tma_able(x, ldx) || !even({dw})) return KDA_ERR_MISALIGNED;
   const int sms = device_sms();
-  if (db && !ws) return KDA_ERR_WORKSPACE;
   if (!sms) return KDA_ERR_CUDA;
   Plan p;
-  if ((s = plan_in(p, N, K, M, sms, db != nullptr, ws, ws_bytes))) return s;
+  if ((s = plan_in(p, N, K, M, sms, false, ws, ws_bytes))) return s;
   Args g = {};
   g.m = (int)N; g.n = (int)K; g.k = (int)M;
   if ((s = set_out(g, dw, ldw))) return s;
   cudaStream_t st = (cudaStream_t)stream;
-  if (db)
-    return dtype == KDA_BF16 ? run<__nv_bfloat16, true, true, true>(g, p, dz, ldd, x, ldx, ws, db, sms, st)
-                             : run<__half, true, true, true>(g, p, dz, ldd, x, ldx, ws, db, sms, st);
-  return dtype == KDA_BF16 ? run<__nv_bfloat16, true, true, false>(g, p, dz, ldd, x, ldx, ws, db, sms, st)
-                           : run<__half, true, true, false>(g, p, dz, ldd, x, ldx, ws, db, sms, st);
+  return dtype == KDA_BF16 ? run<__nv_bfloat16, true, true>(g, p, dz, ldd, x, ldx, ws, nullptr, sms, st)
+                           : run<__half, true, true>(g, p, dz, ldd, x, ldx, ws, nullptr, sms, st);
 }
 
 int kda_act_grad(int dtype, int act, int64_t rows, int64_t cols, const void *dy, int64_t ldy, const void *z, int64_t ldz,
-                 void *dz, int64_t ldd, void *stream) {
+                 void *dz, int64_t ldd, void *db, void *ws, size_t ws_bytes, void *stream) {
   int s = check(dtype, act, rows, cols, 1);
   if (s) return s;
-  if (!dy || !dz || !ld_ok(ldy, cols) || !ld_ok(ldd, cols) || (z && !ld_ok(ldz, cols)) || (act != KDA_ACT_NONE && !z))
+  if (!dy || (!dz && !db) || !ld_ok(ldy, cols) || (dz && !ld_ok(ldd, cols)) || (z && !ld_ok(ldz, cols)) ||
+      (act != KDA_ACT_NONE && !z))
     return KDA_ERR_INVALID_ARG;
-  if (!even({dy, z, dz})) return KDA_ERR_MISALIGNED;
+  if (!even({dy, z, dz, db})) return KDA_ERR_MISALIGNED;
+  if (db && (!ws || (uintptr_t)ws % 16)) return KDA_ERR_WORKSPACE;
   const int sms = device_sms();
   if (!sms) return KDA_ERR_CUDA;
-  const int64_t need = (rows * ((cols + 7) / 8) + 255) / 256, most = (int64_t)sms * 8;
-  const unsigned grid = (unsigned)(need < most ? need : most);
-  const int vy = tma_able(dy, ldy), vz = tma_able(z, ldz), vd = tma_able(dz, ldd);  // 16-byte rows
-  const void *zz = act ? z : nullptr;
+  if (db && ws_bytes < round16((size_t)row_blocks(rows, cols, sms) * cols * sizeof(float))) return KDA_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == KDA_BF16)
-    act_grad_kernel<<<grid, 256, 0, st>>>(act, rows, (int)cols, static_cast<const __nv_bfloat16 *>(dy), ldy,
-                                          static_cast<const __nv_bfloat16 *>(zz), ldz, static_cast<__nv_bfloat16 *>(dz), ldd,
-                                          vy, vz, vd);
-  else
-    act_grad_kernel<<<grid, 256, 0, st>>>(act, rows, (int)cols, static_cast<const __half *>(dy), ldy,
-                                          static_cast<const __half *>(zz), ldz, static_cast<__half *>(dz), ldd, vy, vz, vd);
-  if (cudaGetLastError() != cudaSuccess) return KDA_ERR_CUDA;
-  kda::count_launch();
-  return KDA_OK;
+  return dtype == KDA_BF16 ? act_grad<__nv_bfloat16>(act, rows, cols, dy, ldy, z, ldz, dz, ldd, db, ws, sms, st)
+                           : act_grad<__half>(act, rows, cols, dy, ldy, z, ldz, dz, ldd, db, ws, sms, st);
 }
 
 }  // extern "C"

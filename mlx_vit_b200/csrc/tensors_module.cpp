@@ -229,18 +229,6 @@ Tensor rows_of(const Tensor &x, int64_t cols) {
   if ((cols > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < cols)) t = t.contiguous();
   return t;
 }
-void act_grad(int act, const Tensor &dy, const Tensor &z, const Tensor &dz) {
-  done(kda_act_grad(dtype_of(dy), act, dy.size(0), dy.size(1), ptr(dy), pitch(dy), ptr(z), pitch(z), ptr(dz), pitch(dz),
-                    stream()),
-       "kda_act_grad");
-}
-// the matrix itself where the products can read it, else a copy with padded rows
-Tensor readable(const Tensor &t) {
-  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && pitch(t) % 8 == 0) return t;
-  Tensor out = matrix(t.size(0), t.size(1), t);
-  act_grad(KDA_ACT_NONE, t, Tensor(), out);
-  return out;
-}
 struct Workspace {
   Tensor t;
   size_t n;
@@ -248,26 +236,49 @@ struct Workspace {
     if (n) t = at::empty({(int64_t)n}, like.options().dtype(at::kByte));
   }
 };
+// dz (undefined: not wanted) = dy act'(z), and its column sums
+void act_grad(int act, const Tensor &dy, const Tensor &z, const Tensor &dz, const Tensor &db) {
+  const Workspace ws(KDA_LINEAR_ACT_GRAD, dy.size(0), dy.size(1), 1, db.defined(), dy);
+  done(kda_act_grad(dtype_of(dy), act, dy.size(0), dy.size(1), ptr(dy), pitch(dy), ptr(z), pitch(z), ptr(dz), pitch(dz), ptr(db),
+                    ptr(ws.t), ws.n, stream()),
+       "kda_act_grad");
+}
+bool is_readable(const Tensor &t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && pitch(t) % 8 == 0; }
+// the matrix itself where the products can read it, else a copy with padded rows
+Tensor readable(const Tensor &t) {
+  if (is_readable(t)) return t;
+  Tensor out = matrix(t.size(0), t.size(1), t);
+  act_grad(KDA_ACT_NONE, t, Tensor(), out, Tensor());
+  return out;
+}
+// the gradient at a layer's sum from the one at its result (z undefined: no activation), as the products
+// read it, and with want_db its column sums: in one pass, or none where neither is asked for
+Tensor gradient_at_sum(int act, const Tensor &dy, const Tensor &z, bool want_db, Tensor &db) {
+  const bool copy = act || !is_readable(dy);
+  if (want_db) db = at::empty({dy.size(1)}, dy.options());
+  const Tensor dz = copy ? matrix(dy.size(0), dy.size(1), dy) : Tensor();
+  if (copy || want_db) act_grad(act, dy, z, dz, db);
+  return copy ? dz : dy;
+}
 void product(int act, const Tensor &x, const Tensor &w, const Tensor &b, const Tensor &r, const Tensor &y, const Tensor &z) {
   const Workspace ws(KDA_LINEAR_FWD, x.size(0), w.size(0), w.size(1), false, x);
   done(kda_linear_fwd(dtype_of(x), act, x.size(0), w.size(0), w.size(1), ptr(x), pitch(x), ptr(w), pitch(w), ptr(b),
                       ptr(r), pitch(r), ptr(y), pitch(y), ptr(z), pitch(z), ptr(ws.t), ws.n, stream()),
        "kda_linear_fwd");
 }
-void dgrad(int act, const Tensor &dz, const Tensor &w, const Tensor &z, const Tensor &dx) {
-  const Workspace ws(KDA_LINEAR_DGRAD, dz.size(0), w.size(0), w.size(1), false, dz);
+void dgrad(int act, const Tensor &dz, const Tensor &w, const Tensor &z, const Tensor &dx, const Tensor &db) {
+  const Workspace ws(KDA_LINEAR_DGRAD, dz.size(0), w.size(0), w.size(1), db.defined(), dz);
   done(kda_linear_dgrad(dtype_of(dz), act, dz.size(0), w.size(0), w.size(1), ptr(dz), pitch(dz), ptr(w), pitch(w), ptr(z),
-                        pitch(z), ptr(dx), pitch(dx), ptr(ws.t), ws.n, stream()),
+                        pitch(z), ptr(dx), pitch(dx), ptr(db), ptr(ws.t), ws.n, stream()),
        "kda_linear_dgrad");
 }
-void wgrad(const Tensor &dz, const Tensor &x, bool want_db, Tensor &dw, Tensor &db) {
+Tensor wgrad(const Tensor &dz, const Tensor &x) {
   const int64_t m = dz.size(0), n = dz.size(1), k = x.size(1);
-  dw = at::empty({n, k}, x.options());
-  if (want_db) db = at::empty({n}, x.options());
-  const Workspace ws(KDA_LINEAR_WGRAD, m, n, k, want_db, x);
-  done(kda_linear_wgrad(dtype_of(x), m, n, k, ptr(dz), pitch(dz), ptr(x), pitch(x), ptr(dw), k, ptr(db), ptr(ws.t), ws.n,
-                        stream()),
+  Tensor dw = at::empty({n, k}, x.options());
+  const Workspace ws(KDA_LINEAR_WGRAD, m, n, k, false, x);
+  done(kda_linear_wgrad(dtype_of(x), m, n, k, ptr(dz), pitch(dz), ptr(x), pitch(x), ptr(dw), k, ptr(ws.t), ws.n, stream()),
        "kda_linear_wgrad");
+  return dw;
 }
 std::vector<int64_t> with_last(const Tensor &x, int64_t n) {
   std::vector<int64_t> s = x.sizes().vec();
@@ -335,20 +346,12 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
       if (need_b) g[2] = at::zeros({n}, w.options());
     } else if (need_x || need_w || need_b) {
       const c10::cuda::CUDAGuard guard(x.device());
-      Tensor dz = rows_of(dy, n);
-      if (act) {
-        const Tensor out = matrix(dz.size(0), n, dz);
-        act_grad(act, dz, z, out);
-        dz = out;
-      } else {
-        dz = readable(dz);
-      }
+      const Tensor dz = gradient_at_sum(act, rows_of(dy, n), z, need_b, g[2]);
       if (need_x) {
         g[0] = at::empty(sizes, x.options());
-        dgrad(KDA_ACT_NONE, dz, w, Tensor(), g[0].view({-1, k}));
+        dgrad(KDA_ACT_NONE, dz, w, Tensor(), g[0].view({-1, k}), Tensor());
       }
-      if (need_w || need_b) wgrad(dz, x, need_b, g[1], g[2]);
-      if (!need_w) g[1] = Tensor();
+      if (need_w) g[1] = wgrad(dz, x);
     }
     return once(g);
   }
@@ -401,19 +404,18 @@ struct Mlp : public torch::autograd::Function<Mlp> {
       if (need_b2) g[4] = at::zeros({out}, w2.options());
     } else if (need_x || need_w1 || need_b1 || need_w2 || need_b2) {
       const c10::cuda::CUDAGuard guard(x.device());
-      const Tensor dy2 = readable(rows_of(dy, out));
-      if (need_w2 || need_b2) wgrad(dy2, h, need_b2, g[3], g[4]);
+      const Tensor dy2 = gradient_at_sum(KDA_ACT_NONE, rows_of(dy, out), Tensor(), need_b2, g[4]);
+      if (need_w2) g[3] = wgrad(dy2, h);
       if (need_x || need_w1 || need_b1) {
         const Tensor dz = matrix(dy2.size(0), n, x);
-        dgrad(act, dy2, w2, z, dz);
+        if (need_b1) g[2] = at::empty({n}, x.options());
+        dgrad(act, dy2, w2, z, dz, g[2]);
         if (need_x) {
           g[0] = at::empty(sizes, x.options());
-          dgrad(KDA_ACT_NONE, dz, w1, Tensor(), g[0].view({-1, k}));
+          dgrad(KDA_ACT_NONE, dz, w1, Tensor(), g[0].view({-1, k}), Tensor());
         }
-        if (need_w1 || need_b1) wgrad(dz, x, need_b1, g[1], g[2]);
+        if (need_w1) g[1] = wgrad(dz, x);
       }
-      if (!need_w1) g[1] = Tensor();
-      if (!need_w2) g[3] = Tensor();
     }
     return once(g);
   }

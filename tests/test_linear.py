@@ -45,15 +45,21 @@ def test_backward_refusals():
     L, n = _lib.lib(), ctypes.c_void_p(None)
     st = lambda s: _lib.STATUS[s].replace("KDA_ERR_", "")  # noqa: E731
     bf = _lib.KDA_BF16
-    assert st(L.kda_linear_dgrad(bf, 3, 4, 8, 16, A, 8, A, 16, n, 0, A, 16, n, 0, n)) == "INVALID_ARG"  # no z
-    assert st(L.kda_linear_dgrad(bf, 0, 4, 8, 16, A, 12, A, 16, n, 0, A, 16, n, 0, n)) == "MISALIGNED"
-    assert st(L.kda_linear_wgrad(bf, 4, 8, 16, A, 8, A, 16, A, 16, A, n, 0, n)) == "WORKSPACE"
-    assert st(L.kda_linear_wgrad(bf, 4, 8, 16, A, 8, A, 16, A, 15, n, n, 0, n)) == "INVALID_ARG"
+    assert st(L.kda_linear_dgrad(bf, 3, 4, 8, 16, A, 8, A, 16, n, 0, A, 16, n, n, 0, n)) == "INVALID_ARG"  # no z
+    assert st(L.kda_linear_dgrad(bf, 0, 4, 8, 16, A, 12, A, 16, n, 0, A, 16, n, n, 0, n)) == "MISALIGNED"
+    assert st(L.kda_linear_dgrad(bf, 0, 4, 8, 16, A, 8, A, 16, n, 0, A, 16, A, n, 0, n)) == "WORKSPACE"
+    assert st(L.kda_linear_wgrad(bf, 4, 8, 16, A, 8, A, 16, A, 15, n, 0, n)) == "INVALID_ARG"
+    assert st(L.kda_linear_wgrad(bf, 4, 8, 16, A, 8, A, 12, A, 16, n, 0, n)) == "INVALID_ARG"
+    assert st(L.kda_linear_wgrad(bf, 4, 8, 16, A, 8, A + 2, 16, A, 16, n, 0, n)) == "MISALIGNED"
     for op in (_lib.KDA_LINEAR_FWD, _lib.KDA_LINEAR_DGRAD, _lib.KDA_LINEAR_WGRAD):
         assert L.kda_linear_workspace_bytes(op, 0, 8, 16, 1) == 0
         assert L.kda_linear_workspace_bytes(op, 1000, 8, 1 << 20, 1) >= 0
-    assert L.kda_linear_workspace_bytes(_lib.KDA_LINEAR_WGRAD, 4, 8, 16, 1) >= 8 * 4
+    assert L.kda_linear_workspace_bytes(_lib.KDA_LINEAR_DGRAD, 4, 8, 16, 1) >= 16 * 4
+    assert L.kda_linear_workspace_bytes(_lib.KDA_LINEAR_ACT_GRAD, 4, 8, 1, 1) >= 8 * 4
+    assert L.kda_linear_workspace_bytes(_lib.KDA_LINEAR_ACT_GRAD, 4, 8, 1, 0) == 0
     assert L.kda_linear_workspace_bytes(_lib.KDA_LINEAR_WGRAD, 12544, 2304, 768, 0) > 2304 * 768 * 4  # split
     assert L.kda_linear_workspace_bytes(7, 4, 8, 16, 1) == 0
-    assert st(L.kda_act_grad(bf, 1, 4, 8, A, 8, n, 0, A, 8, n)) == "INVALID_ARG"
-    assert st(L.kda_act_grad(bf, 0, 4, 8, A + 1, 8, n, 0, A, 8, n)) == "MISALIGNED"
+    assert st(L.kda_act_grad(bf, 1, 4, 8, A, 8, n, 0, A, 8, n, n, 0, n)) == "INVALID_ARG"
+    assert st(L.kda_act_grad(bf, 0, 4, 8, A, 8, n, 0, n, 0, n, n, 0, n)) == "INVALID_ARG"  # neither dz nor db
+    assert st(L.kda_act_grad(bf, 0, 4, 8, A + 1, 8, n, 0, A, 8, n, n, 0, n)) == "MISALIGNED"
+    assert st(L.kda_act_grad(bf, 0, 4, 8, A, 8, n, 0, n, 0, A, n, 0, n)) == "WORKSPACE"

@@ -276,6 +276,20 @@ def test_no_rows(cuda):
     assert y.shape == x.shape and (w.grad == 0).all() and (w2.grad == 0).all()
 
 
+def test_bias_gradient_with_infinite_weights(cuda):
+    """The hidden bias gradient sums the rows there are: those behind the last, zeros in the products, would
+    turn an infinite weight into NaN."""
+    x, dy = torch.ones(33, 16, dtype=torch.bfloat16, device=cuda), torch.ones(33, 8, dtype=torch.bfloat16, device=cuda)
+    w1 = torch.eye(16, dtype=torch.bfloat16, device=cuda)
+    w2 = torch.ones(8, 16, dtype=torch.bfloat16, device=cuda)
+    w2[3, 5] = float("inf")
+    b1 = torch.zeros(16, dtype=torch.bfloat16, device=cuda, requires_grad=True)
+    mlp(x, w1, b1, w2, None, "relu").backward(dy)
+    want = torch.full((16,), 33 * 8.0, device=cuda)
+    want[5] = float("inf")
+    assert torch.equal(b1.grad.float(), want)
+
+
 def test_values_that_are_not_finite_stay_in_their_rows(cuda):
     g = gen(8)
     x = rnd(g, 40, 72, dt=torch.bfloat16)
