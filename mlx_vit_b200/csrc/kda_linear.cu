@@ -19,6 +19,8 @@
 // to fill the GPU, k is split: each part writes its float32 tile to a workspace and a second kernel
 // adds the parts in order and runs the epilogue.  A few rows (M <= 32) take a kernel of their own
 // that streams the weights once through registers.
+#include <limits.h>
+
 #include <atomic>
 #include <initializer_list>
 
@@ -84,7 +86,9 @@ __device__ __forceinline__ void cluster_sync() {
 __device__ __forceinline__ void arrive_cluster(uint32_t addr) {  // addr: a shared::cluster address
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" :: "r"(addr) : "memory");
 }
-__device__ __forceinline__ bool wait(uint32_t mbar, uint32_t parity) { return mbar_wait(mbar, parity, kPolls); }
+__device__ __forceinline__ bool wait(uint32_t mbar, uint32_t parity, int polls = kPolls) {
+  return mbar_wait(mbar, parity, polls);
+}
 
 template <int CG>
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t mbar) {
@@ -399,6 +403,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
     T *bs = bias_sm + e * 64;
     const uint32_t empty_lead = CG == 2 ? map_rank(acc_empty, 0) : acc_empty;
     uint32_t n = 0, in_phase = 0;
+    // an accumulator's wait spans its whole sum: at least a microsecond's polls for each block of it
+    const int acc_polls = (int)min((int64_t)INT_MAX, (int64_t)kPolls + 128 * (int64_t)g.per_split);
     const bool in_tma = g.in_kind && g.in_tma && g.splits == 1, ahead = in_tma && !g.save_z;
     for (int u = first; ok && u < units; u += step, ++n) {
       const int t = u % tiles, part = u / tiles;
@@ -424,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
         }
         __syncwarp();
       }
-      if (lane == 0) ok = wait(acc_full + 8 * buf, use & 1);
+      if (lane == 0) ok = wait(acc_full + 8 * buf, use & 1, acc_polls);
       __syncwarp();
       if (!__all_sync(0xFFFFFFFFu, ok)) {
         ok = false;
@@ -819,24 +825,32 @@ static int device_sms() {
   return n;
 }
 
-// ---- which tiles, and into how many parts k is split ----
+// ---- which tiles, and into how many parts k is split: the least estimated time.  A pair of CTAs on
+// 256 x 256 moves the fewest bytes into shared memory for its products (64 KB for twice the work of
+// four 128 x 128 tiles' 128 KB) and wins where its tiles fill the GPU (12544 x 2304 x 768 forward: 37 us,
+// 49 on 128 x 128, 88 on 128 x 64); fewer rows or columns take smaller tiles (256 x 768 x 768: 10.4,
+// 8.1 and 7.7 us), and long sums over few tiles are split (dW of 768 x 768 from 12544 rows: 61 us whole,
+// 21 in eight parts; dW of 4096 x 1024, whose tiles nearly fill the GPU: 75 and 87 us in two).  Over 16
+// shapes the choice was within 5 % of the best of all tiles and 1 to 12 parts ----
 struct Plan {
   int cg, bn, splits, per_split;
 };
 static Plan plan_for(int64_t m, int64_t n, int64_t k, int sms, bool may_split) {
   struct Tile {
     int cg, bn;
-    double busy, alone, kb;  // us a block of 64 k where the GPU is full, and where it is not; KB it reads
+    double busy, alone;  // us a block of 64 k takes where the GPU is full, and on one tile alone (measured)
   };
-  static const Tile tiles[] = {{2, 256, 0.40, 0.30, 64}, {1, 128, 0.40, 0.20, 32}, {1, 64, 0.31, 0.16, 24}};
+  static const Tile tiles[] = {{2, 256, 0.40, 0.31}, {1, 128, 0.40, 0.26}, {1, 64, 0.31, 0.23}};
   const int64_t blocks = (k + kBlockK - 1) / kBlockK;
   Plan best = {};
   double best_us = 1e300;
   for (const Tile &t : tiles) {
     const int64_t count = ((m + 128 * t.cg - 1) / (128 * t.cg)) * ((n + t.bn - 1) / t.bn), units = sms / t.cg;
-    for (int64_t s = 1; s <= (may_split ? 16 : 1); ++s) {
-      const int64_t per = (blocks + s - 1) / s, parts = (blocks + per - 1) / per;
-      if (parts != s || (s > 1 && per < 4)) continue;
+    // tiles that fill the GPU are not split (measured: the joining costs more than an even last wave gains)
+    const int64_t most = may_split && count < units ? (blocks / 4 < 16 ? blocks / 4 : 16) : 1;
+    for (int64_t s = 1; s == 1 || s <= most; ++s) {
+      const int64_t per = (blocks + s - 1) / s;
+      if (s > 1 && (blocks + per - 1) / per != s) continue;  // an empty part
       const int64_t waves = (count * s + units - 1) / units;
       const double load = (double)(count * s < units ? count * s : units) / units;
       const double per_block = t.alone + (t.busy - t.alone) * load;

@@ -197,6 +197,8 @@ class AdamW(torch.optim.Optimizer):
             if not live:
                 continue
             capturing = live[0].is_cuda and torch.cuda.is_current_stream_capturing()
+            if capturing and not self.capturable:
+                raise ValueError("AdamW: a step is captured into a graph with capturable=True only")
             for p in live:
                 if not self.state[p]:
                     if capturing:

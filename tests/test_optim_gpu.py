@@ -413,6 +413,30 @@ def test_captured_step_replays(cuda, bits):
             assert torch.equal(o.ema_of(p), o2.ema_of(q))
 
 
+def test_capturable_state_round_trip(cuda):
+    """Step counter and learning rate of a capturable optimizer go through its state dict."""
+    def build():
+        torch.manual_seed(4)
+        ps = [torch.nn.Parameter(torch.randn(40, 9, device=cuda)), torch.nn.Parameter(torch.randn(3, device=cuda))]
+        for p in ps:
+            p.grad = torch.ones_like(p) * 0.1
+        return ps, optim.AdamW([dict(params=ps[:1]), dict(params=ps[1:], lr=3e-3)], lr=1e-2, state_bits=8, capturable=True)
+
+    ps, o = build()
+    for _ in range(3):
+        o.step()
+    o.param_groups[0]["lr"].fill_(5e-3)
+    qs, o2 = build()
+    o2.load_state_dict(copy.deepcopy(o.state_dict()))
+    with torch.no_grad():
+        for p, q in zip(ps, qs):
+            q.copy_(p)
+    o.step(), o2.step()
+    assert [int(g["step"]) for g in o2.param_groups] == [4, 4]
+    assert abs(float(o2.param_groups[0]["lr"]) - 5e-3) <= 2.0 ** -24 * 5e-3
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+
+
 def test_capture_refuses_frozen_numbers(cuda):
     ps = [torch.nn.Parameter(torch.randn(10, device=cuda))]
     ps[0].grad = torch.randn(10, device=cuda)
