@@ -1,6 +1,6 @@
 // mlx_vit_b200._tensors: the host side of the operators whose launches are shorter than Python's way
-// to them, in C++: the reading of a model's tensor lists for the optimizer, and the linear
-// products with their autograd functions.
+// to them, in C++: the optimizer's step over a model's tensor lists, and the linear products with
+// their autograd functions.
 //
 // An optimizer step over a model's parameters looks at some hundred tensors five times (parameter,
 // gradient, two states, shadow) before its one launch.  From Python that is about 0.1 us an
@@ -75,105 +75,75 @@ PyObject *guarded(F f) {
   return nullptr;
 }
 
-// adamw_table(params, grads, exp_avgs, exp_avg_sqs, emas or None, bits) -> (KdaAdamWTensor array as
-// bytes, device index).  ValueError for operands that the kernel does not take.  The versions
-// of what the step writes are advanced, as torch's own in-place operations do.
-PyObject *adamw_table(PyObject *, PyObject *args) {
-  PyObject *po, *go, *mo, *vo, *eo;
-  int bits;
-  if (!PyArg_ParseTuple(args, "OOOOOi", &po, &go, &mo, &vo, &eo, &bits)) return nullptr;
-  return guarded([&]() -> PyObject * {
-    const Items p(po, "params"), g(go, "grads"), m(mo, "exp_avgs"), v(vo, "exp_avg_sqs");
-    const bool ema = eo != Py_None;
-    const Items e(ema ? eo : po, "emas");
-    need(p.n > 0, "no parameters");
-    need(g.n == p.n && m.n == p.n && v.n == p.n && e.n == p.n, "every list must hold one entry a parameter");
-    const at::Device dev = tensor(p.p[0], "params").device();
-    need(dev.is_cuda(), "adamw_step takes CUDA tensors; there is no CPU path");
-    std::vector<KdaAdamWTensor> rows(p.n);
-    std::vector<const void *> written;
-    written.reserve(4 * p.n);
-    std::vector<const at::Tensor *> bump;
-    bump.reserve(4 * p.n);
-    for (Py_ssize_t i = 0; i < p.n; ++i) {
-      const at::Tensor &pt = tensor(p.p[i], "params"), &gt = tensor(g.p[i], "grads");
-      need(pt.device() == dev && gt.device() == dev,
-           "params and grads must all be on one CUDA device; there is no CPU path");
-      need(pt.layout() == at::kStrided && gt.layout() == at::kStrided, "params and grads must be dense tensors");
-      need(pt.sizes() == gt.sizes(), "grads: shapes do not match the parameters'");
-      need(pt.scalar_type() == gt.scalar_type(), "grads: dtypes do not match the parameters'");
-      need(pt.is_non_overlapping_and_dense(), "params must be dense in memory");
-      need((pt.is_contiguous() && gt.is_contiguous()) || pt.strides() == gt.strides(),
-           "grads: not laid out in memory as the parameters");
-      KdaAdamWTensor &r = rows[i];
-      r = {};
-      r.dtype = code_of(pt.scalar_type());
-      need(r.dtype >= 0, "params must be float32, bfloat16 or float16");
-      r.numel = pt.numel();
-      r.p = pt.data_ptr();
-      r.g = gt.data_ptr();
-      const at::Tensor *mt, *vt;
-      if (bits == 8) {
-        const int64_t blocks = (r.numel + 255) / 256;
-        const Items mp(m.p[i], "exp_avgs"), vp(v.p[i], "exp_avg_sqs");
-        need(mp.n == 2 && vp.n == 2, "8-bit states are (codes, exponents) pairs, all of them");
-        mt = &state_part(mp.p[0], "exp_avgs", at::kByte, dev, r.numel);
-        vt = &state_part(vp.p[0], "exp_avg_sqs", at::kByte, dev, r.numel);
-        const at::Tensor &me = state_part(mp.p[1], "exp_avgs' exponents", at::kByte, dev, blocks);
-        const at::Tensor &ve = state_part(vp.p[1], "exp_avg_sqs' exponents", at::kByte, dev, blocks);
-        r.m_exp = static_cast<uint8_t *>(me.data_ptr());
-        r.v_exp = static_cast<uint8_t *>(ve.data_ptr());
-        if (r.numel) written.insert(written.end(), {r.m_exp, r.v_exp});
-        bump.insert(bump.end(), {&me, &ve});
-      } else {
-        mt = &state_part(m.p[i], "exp_avgs", at::kFloat, dev, r.numel);
-        vt = &state_part(v.p[i], "exp_avg_sqs", at::kFloat, dev, r.numel);
-      }
-      r.m = mt->data_ptr();
-      r.v = vt->data_ptr();
-      bump.insert(bump.end(), {&pt, mt, vt});
-      if (ema) {
-        const at::Tensor &et = state_part(e.p[i], "emas", at::kFloat, dev, r.numel);
-        r.ema = static_cast<float *>(et.data_ptr());
-        bump.push_back(&et);
-      }
-      if (r.numel) {
-        written.insert(written.end(), {r.p, r.m, r.v});
-        if (ema) written.push_back(r.ema);
-      }
+// The KdaAdamWTensor array of a step's lists, after their checks, and their device.  The versions of
+// what the step writes are advanced, as torch's own in-place operations do.
+std::vector<KdaAdamWTensor> adamw_table(PyObject *po, PyObject *go, PyObject *mo, PyObject *vo, PyObject *eo, int &bits,
+                                        at::Device &dev) {
+  const Items p(po, "params"), g(go, "grads"), m(mo, "exp_avgs"), v(vo, "exp_avg_sqs");
+  const bool ema = eo != Py_None;
+  const Items e(ema ? eo : po, "emas");
+  need(p.n > 0, "no parameters");
+  need(g.n == p.n && m.n == p.n && v.n == p.n && e.n == p.n, "every list must hold one entry a parameter");
+  dev = tensor(p.p[0], "params").device();
+  bits = PyTuple_Check(m.p[0]) || PyList_Check(m.p[0]) ? 8 : 32;
+  need(dev.is_cuda(), "adamw_step takes CUDA tensors; there is no CPU path");
+  std::vector<KdaAdamWTensor> rows(p.n);
+  std::vector<const void *> written;
+  written.reserve(4 * p.n);
+  std::vector<const at::Tensor *> bump;
+  bump.reserve(4 * p.n);
+  for (Py_ssize_t i = 0; i < p.n; ++i) {
+    const at::Tensor &pt = tensor(p.p[i], "params"), &gt = tensor(g.p[i], "grads");
+    need(pt.device() == dev && gt.device() == dev,
+         "params and grads must all be on one CUDA device; there is no CPU path");
+    need(pt.layout() == at::kStrided && gt.layout() == at::kStrided, "params and grads must be dense tensors");
+    need(pt.sizes() == gt.sizes(), "grads: shapes do not match the parameters'");
+    need(pt.scalar_type() == gt.scalar_type(), "grads: dtypes do not match the parameters'");
+    need(pt.is_non_overlapping_and_dense(), "params must be dense in memory");
+    need((pt.is_contiguous() && gt.is_contiguous()) || pt.strides() == gt.strides(),
+         "grads: not laid out in memory as the parameters");
+    KdaAdamWTensor &r = rows[i];
+    r = {};
+    r.dtype = code_of(pt.scalar_type());
+    need(r.dtype >= 0, "params must be float32, bfloat16 or float16");
+    r.numel = pt.numel();
+    r.p = pt.data_ptr();
+    r.g = gt.data_ptr();
+    const at::Tensor *mt, *vt;
+    if (bits == 8) {
+      const int64_t blocks = (r.numel + 255) / 256;
+      const Items mp(m.p[i], "exp_avgs"), vp(v.p[i], "exp_avg_sqs");
+      need(mp.n == 2 && vp.n == 2, "8-bit states are (codes, exponents) pairs, all of them");
+      mt = &state_part(mp.p[0], "exp_avgs", at::kByte, dev, r.numel);
+      vt = &state_part(vp.p[0], "exp_avg_sqs", at::kByte, dev, r.numel);
+      const at::Tensor &me = state_part(mp.p[1], "exp_avgs' exponents", at::kByte, dev, blocks);
+      const at::Tensor &ve = state_part(vp.p[1], "exp_avg_sqs' exponents", at::kByte, dev, blocks);
+      r.m_exp = static_cast<uint8_t *>(me.data_ptr());
+      r.v_exp = static_cast<uint8_t *>(ve.data_ptr());
+      if (r.numel) written.insert(written.end(), {r.m_exp, r.v_exp});
+      bump.insert(bump.end(), {&me, &ve});
+    } else {
+      mt = &state_part(m.p[i], "exp_avgs", at::kFloat, dev, r.numel);
+      vt = &state_part(v.p[i], "exp_avg_sqs", at::kFloat, dev, r.numel);
     }
-    std::sort(written.begin(), written.end());
-    need(std::adjacent_find(written.begin(), written.end()) == written.end(), "the same tensor is passed twice");
-    for (const at::Tensor *t : bump)
-      if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
-    return Py_BuildValue("(y#i)", reinterpret_cast<const char *>(rows.data()),
-                         (Py_ssize_t)(rows.size() * sizeof(KdaAdamWTensor)), (int)dev.index());
-  });
-}
-
-// grad_table(grads) -> (KdaAdamWTensor array as bytes, device index), for the norm alone
-PyObject *grad_table(PyObject *, PyObject *args) {
-  PyObject *go;
-  if (!PyArg_ParseTuple(args, "O", &go)) return nullptr;
-  return guarded([&]() -> PyObject * {
-    const Items g(go, "grads");
-    need(g.n > 0, "no gradients");
-    const at::Device dev = tensor(g.p[0], "grads").device();
-    need(dev.is_cuda(), "grad_norm takes CUDA tensors; there is no CPU path");
-    std::vector<KdaAdamWTensor> rows(g.n);
-    for (Py_ssize_t i = 0; i < g.n; ++i) {
-      const at::Tensor &t = tensor(g.p[i], "grads");
-      need(t.device() == dev, "grads must all be on one CUDA device; there is no CPU path");
-      need(t.layout() == at::kStrided && t.is_non_overlapping_and_dense(), "grads must be dense in memory");
-      rows[i] = {};
-      rows[i].dtype = code_of(t.scalar_type());
-      need(rows[i].dtype >= 0, "grads must be float32, bfloat16 or float16");
-      rows[i].g = t.data_ptr();
-      rows[i].numel = t.numel();
+    r.m = mt->data_ptr();
+    r.v = vt->data_ptr();
+    bump.insert(bump.end(), {&pt, mt, vt});
+    if (ema) {
+      const at::Tensor &et = state_part(e.p[i], "emas", at::kFloat, dev, r.numel);
+      r.ema = static_cast<float *>(et.data_ptr());
+      bump.push_back(&et);
     }
-    return Py_BuildValue("(y#i)", reinterpret_cast<const char *>(rows.data()),
-                         (Py_ssize_t)(rows.size() * sizeof(KdaAdamWTensor)), (int)dev.index());
-  });
+    if (r.numel) {
+      written.insert(written.end(), {r.p, r.m, r.v});
+      if (ema) written.push_back(r.ema);
+    }
+  }
+  std::sort(written.begin(), written.end());
+  need(std::adjacent_find(written.begin(), written.end()) == written.end(), "the same tensor is passed twice");
+  for (const at::Tensor *t : bump)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  return rows;
 }
 
 // unlike(params, grads) -> indices of the strided gradients that lie in memory otherwise than their parameters
@@ -201,16 +171,114 @@ PyObject *unlike(PyObject *, PyObject *args) {
   });
 }
 
+void done(int status, const char *where) {
+  TORCH_CHECK(status == 0, where, ": ", kda_strerror(status));
+}
+void *stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
+bool capturing(void *st) {
+  cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
+  return cudaStreamIsCapturing(static_cast<cudaStream_t>(st), &s) == cudaSuccess && s != cudaStreamCaptureStatusNone;
+}
+at::Tensor adamw_workspace(int64_t count, const at::Device &dev) {
+  return at::empty({(int64_t)kda_adamw_workspace_bytes(count)}, at::TensorOptions().dtype(at::kByte).device(dev));
+}
+// a step, learning rate or norm that lies on the device
+const at::Tensor *scalar(PyObject *o, const char *name, at::ScalarType type, const at::Device &dev) {
+  if (!THPVariable_Check(o)) return nullptr;
+  const at::Tensor &t = THPVariable_Unpack(o);
+  if (t.device() != dev || t.scalar_type() != type || t.numel() != 1)
+    throw Refused{std::string(name) + " as a tensor must be one " + (type == at::kLong ? "int64" : "float32") +
+                  " value on the parameters' device"};
+  return &t;
+}
+
+// adamw_step(params, grads, exp_avgs, exp_avg_sqs, emas or None, step, lr, beta1, beta2, eps, weight_decay,
+//            bias_correction, max_grad_norm (0: none), ema_decay, seed, norm or None) -> norm or None.
+// ValueError for operands that the kernel does not take.
+PyObject *adamw_step(PyObject *, PyObject *args) {
+  PyObject *po, *go, *mo, *vo, *eo, *so, *lo, *no;
+  KdaAdamW a = {};
+  int bias;
+  unsigned int seed;
+  if (!PyArg_ParseTuple(args, "OOOOOOOddddpddIO", &po, &go, &mo, &vo, &eo, &so, &lo, &a.beta1, &a.beta2, &a.eps, &a.weight_decay,
+                        &bias, &a.max_grad_norm, &a.ema_decay, &seed, &no))
+    return nullptr;
+  return guarded([&]() -> PyObject * {
+    need(a.beta1 >= 0 && a.beta1 < 1 && a.beta2 >= 0 && a.beta2 < 1, "betas must lie in [0, 1)");
+    need(a.eps >= 0, "eps must not be negative");
+    need(a.ema_decay >= 0 && a.ema_decay <= 1, "ema_decay must lie in [0, 1]");
+    need(no == Py_None || a.max_grad_norm > 0, "norm is used with max_grad_norm only");
+    at::Device dev(at::kCPU);
+    const std::vector<KdaAdamWTensor> rows = adamw_table(po, go, mo, vo, eo, a.state_bits, dev);
+    need(a.state_bits == 32 || a.eps >= 1e-30, "8-bit states need an eps of at least 1e-30");
+    const at::Tensor *step = scalar(so, "step", at::kLong, dev), *lr = scalar(lo, "lr", at::kFloat, dev);
+    const at::Tensor *given = no == Py_None ? nullptr : scalar(no, "norm", at::kFloat, dev);
+    need(no == Py_None || given, "norm must be a tensor");
+    if (!step) {
+      a.step = PyLong_AsLongLong(so);
+      if (PyErr_Occurred()) return nullptr;
+      need(a.step >= 1, "step counts from 1");
+    }
+    if (!lr) {
+      a.lr = PyFloat_AsDouble(lo);
+      if (PyErr_Occurred()) return nullptr;
+    }
+    a.seed = seed;
+    a.bias_correction = bias;
+    a.use_ema = eo != Py_None;
+    a.norm_given = given != nullptr;
+    const c10::cuda::CUDAGuard guard(dev);
+    void *st = stream();
+    need((step && lr) || !capturing(st), "step and lr must be CUDA tensors while a graph is captured");
+    const bool clip = a.max_grad_norm > 0;
+    at::Tensor ws, norm;
+    if (clip || step || lr) ws = adamw_workspace((int64_t)rows.size(), dev);
+    if (clip) norm = given ? *given : at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
+    done(kda_adamw_step(&a, rows.data(), (int64_t)rows.size(), step ? step->data_ptr<int64_t>() : nullptr,
+                        lr ? lr->data_ptr<float>() : nullptr, clip ? norm.data_ptr<float>() : nullptr,
+                        ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0, st),
+         "kda_adamw_step");
+    if (step) step->unsafeGetTensorImpl()->bump_version();
+    if (clip) return THPVariable_Wrap(norm);
+    Py_RETURN_NONE;
+  });
+}
+
+// grad_norm(grads) -> their 2-norm, a float32 scalar on their device
+PyObject *grad_norm(PyObject *, PyObject *args) {
+  PyObject *go;
+  if (!PyArg_ParseTuple(args, "O", &go)) return nullptr;
+  return guarded([&]() -> PyObject * {
+    const Items g(go, "grads");
+    need(g.n > 0, "no gradients");
+    const at::Device dev = tensor(g.p[0], "grads").device();
+    need(dev.is_cuda(), "grad_norm takes CUDA tensors; there is no CPU path");
+    std::vector<KdaAdamWTensor> rows(g.n);
+    for (Py_ssize_t i = 0; i < g.n; ++i) {
+      const at::Tensor &t = tensor(g.p[i], "grads");
+      need(t.device() == dev, "grads must all be on one CUDA device; there is no CPU path");
+      need(t.layout() == at::kStrided && t.is_non_overlapping_and_dense(), "grads must be dense in memory");
+      rows[i] = {};
+      rows[i].dtype = code_of(t.scalar_type());
+      need(rows[i].dtype >= 0, "grads must be float32, bfloat16 or float16");
+      rows[i].g = t.data_ptr();
+      rows[i].numel = t.numel();
+    }
+    const c10::cuda::CUDAGuard guard(dev);
+    const at::Tensor ws = adamw_workspace((int64_t)rows.size(), dev);
+    const at::Tensor norm = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
+    done(kda_grad_norm(rows.data(), (int64_t)rows.size(), norm.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), stream()),
+         "kda_grad_norm");
+    return THPVariable_Wrap(norm);
+  });
+}
+
 // ---- linear products ----
 using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::Variable;
 using torch::autograd::variable_list;
 
-void done(int status, const char *where) {
-  TORCH_CHECK(status == 0, where, ": ", kda_strerror(status));
-}
-void *stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 int dtype_of(const Tensor &t) { return t.scalar_type() == at::kBFloat16 ? KDA_BF16 : KDA_F16; }
 void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 // elements from row to row of a matrix with contiguous rows
@@ -488,8 +556,8 @@ PyObject *mlp(PyObject *, PyObject *args) {
   });
 }
 
-PyMethodDef methods[] = {{"adamw_table", adamw_table, METH_VARARGS, nullptr},
-                         {"grad_table", grad_table, METH_VARARGS, nullptr},
+PyMethodDef methods[] = {{"adamw_step", adamw_step, METH_VARARGS, nullptr},
+                         {"grad_norm", grad_norm, METH_VARARGS, nullptr},
                          {"unlike", unlike, METH_VARARGS, nullptr},
                          {"linear_act", linear_act, METH_VARARGS, nullptr},
                          {"mlp", mlp, METH_VARARGS, nullptr},

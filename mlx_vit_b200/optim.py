@@ -24,7 +24,6 @@ holds a value that is not finite reads back as NaN.
 """
 from __future__ import annotations
 
-import ctypes
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -62,25 +61,11 @@ def _need(ok, msg):
         raise ValueError(msg)
 
 
-def _workspace(count, dev):
-    n = _lib.lib().kda_adamw_workspace_bytes(count)
-    return torch.empty(n, dtype=torch.uint8, device=torch.device("cuda", dev)), n
-
-
-@torch.no_grad()
 def grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     """The 2-norm of all gradients together, a float32 scalar on their device (sums in 64 bits)."""
-    grads = list(grads)
-    rows, dev = _lib.tensors().grad_table(grads)
-    with torch.cuda.device(dev):
-        out = torch.empty((), dtype=torch.float32, device=grads[0].device)
-        ws, nws = _workspace(len(grads), dev)
-        _lib.check(_lib.lib().kda_grad_norm(rows, len(grads), out.data_ptr(), ws.data_ptr(), nws,
-                                            torch.cuda.current_stream().cuda_stream), "kda_grad_norm")
-    return out
+    return _lib.tensors().grad_norm(list(grads))
 
 
-@torch.no_grad()
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
                exp_avgs: Sequence[Union[torch.Tensor, State8]], exp_avg_sqs: Sequence[Union[torch.Tensor, State8]], *,
                step: Union[int, torch.Tensor], lr: Union[float, torch.Tensor], betas=(0.9, 0.999), eps: float = 1e-8,
@@ -99,41 +84,11 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     (float32) follow the parameters with ``ema_decay``.  Tensors must not overlap one another.
     Returns the gradients' norm (float32 scalar) with ``max_grad_norm``, else None.
     """
-    params, grads, exp_avgs, exp_avg_sqs = list(params), list(grads), list(exp_avgs), list(exp_avg_sqs)
-    bits = 8 if exp_avgs and isinstance(exp_avgs[0], (tuple, list)) else 32
     _need((emas is None) == (ema_decay is None), "emas and ema_decay go together")
-    _need(ema_decay is None or 0.0 <= ema_decay <= 1.0, f"ema_decay must lie in [0, 1], got {ema_decay}")
-    _need(0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0, f"betas must lie in [0, 1), got {betas}")
-    _need(eps >= 0.0, f"eps must not be negative, got {eps}")
-    _need(bits == 32 or eps >= 1e-30, f"8-bit states need an eps of at least 1e-30, got {eps}")
-    _need(max_grad_norm is None or max_grad_norm > 0.0, f"max_grad_norm must be positive, got {max_grad_norm}")
-    _need(norm is None or max_grad_norm is not None, "norm is used with max_grad_norm only")
-    rows, dev = _lib.tensors().adamw_table(params, grads, exp_avgs, exp_avg_sqs, None if emas is None else list(emas),
-                                           bits)
-    step_t = step if isinstance(step, torch.Tensor) else None
-    lr_t = lr if isinstance(lr, torch.Tensor) else None
-    for n, t, dt in (("step", step_t, torch.int64), ("lr", lr_t, torch.float32), ("norm", norm, torch.float32)):
-        _need(t is None or (t.get_device() == dev and t.dtype == dt and t.numel() == 1),
-              f"{n} as a tensor must be one {dt} value on the parameters' device")
-    if step_t is None:
-        _need(step >= 1, f"step counts from 1, got {step}")
-    with torch.cuda.device(dev):
-        if (step_t is None or lr_t is None) and torch.cuda.is_current_stream_capturing():
-            raise ValueError("adamw_step: step and lr must be CUDA tensors while a graph is captured")
-        out = norm
-        ws, nws = None, 0
-        if max_grad_norm is not None or step_t is not None or lr_t is not None:
-            ws, nws = _workspace(len(params), dev)
-            if max_grad_norm is not None and norm is None:
-                out = torch.empty((), dtype=torch.float32, device=params[0].device)
-        args = _lib.KdaAdamW(0.0 if lr_t is not None else float(lr), betas[0], betas[1], eps, weight_decay,
-                             max_grad_norm or 0.0, ema_decay or 0.0, 0 if step_t is not None else step,
-                             seed & 0xFFFFFFFF, bits, bool(bias_correction), emas is not None, norm is not None, 0)
-        _lib.check(_lib.lib().kda_adamw_step(
-            ctypes.byref(args), rows, len(params), None if step_t is None else step_t.data_ptr(),
-            None if lr_t is None else lr_t.data_ptr(), None if out is None else out.data_ptr(),
-            None if ws is None else ws.data_ptr(), nws, torch.cuda.current_stream().cuda_stream), "kda_adamw_step")
-    return out
+    _need(max_grad_norm is None or max_grad_norm > 0.0, "max_grad_norm must be positive")
+    return _lib.tensors().adamw_step(list(params), list(grads), list(exp_avgs), list(exp_avg_sqs),
+                                     None if emas is None else list(emas), step, lr, betas[0], betas[1], eps, weight_decay,
+                                     bias_correction, max_grad_norm or 0.0, ema_decay or 0.0, seed & 0xFFFFFFFF, norm)
 
 
 class AdamW(torch.optim.Optimizer):
