@@ -197,10 +197,38 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """As torch's, but the states keep their own dtypes (torch casts them to the parameters')."""
-        super().load_state_dict(state_dict)
+        """As torch's, but the states keep their own dtypes (torch casts them to the parameters').  The
+        float32 states of a ``torch.optim.AdamW`` can be loaded into one of 32 bits."""
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i in ids:
+            held = state_dict["state"].get(i)
+            _need(not held or ("exp_avg_exp" in held) == (self.state_bits == 8),
+                  f"the loaded states are not those of an optimizer with state_bits={self.state_bits}")
+        super().load_state_dict(state_dict)
         for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
             if i in state_dict["state"]:
-                self.state[p] = {k: v.to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
-                                 for k, v in state_dict["state"][i].items()}
+                self.state[p] = {k: self._own(k, v, p) for k, v in state_dict["state"][i].items()}
+        for group in self.param_groups:
+            for name, value in self.defaults.items():
+                group.setdefault(name, value)
+            held = [self.state[p] for p in group["params"] if self.state[p]]
+            # the step's number: a group's where it is capturable, else a parameter's
+            if self.capturable:
+                steps = [st.pop("step") for st in held if "step" in st]
+                if "step" not in group and steps:
+                    group["step"] = max(steps)
+            elif "step" in group:
+                n = int(group.pop("step"))
+                group["lr"] = float(group["lr"])
+                for st in held:
+                    st["step"] = n
+
+    def _own(self, name, v, p):
+        """A loaded state entry as this optimizer holds it: tensors flat, in the parameter's order in memory."""
+        if name == "step":
+            return int(v)
+        if not isinstance(v, torch.Tensor):
+            return v
+        if v.dtype != torch.uint8 and v.dim() != 1 and v.shape == p.shape:
+            return torch.empty_like(p, dtype=torch.float32).copy_(v).as_strided((p.numel(),), (1,))
+        return v.to(p.device, copy=True)

@@ -373,6 +373,30 @@ def test_optimizer_state_round_trip(cuda, bits):
                 assert torch.equal(s1[k], s2[k]) if torch.is_tensor(s1[k]) else s1[k] == s2[k]
 
 
+def test_states_of_torch_adamw_load(cuda):
+    """A run that torch.optim.AdamW began goes on: the next step moves every parameter as torch's would,
+    a channels-last one among them, within float32's roundings of the update (see above)."""
+    a, b = params_of(cuda), params_of(cuda)
+    old = torch.optim.AdamW(a.parameters(), lr=1e-2)
+    for t in range(3):
+        old.zero_grad()
+        backward(a, t)
+        old.step()
+    b.load_state_dict(a.state_dict())
+    b[0].to(memory_format=torch.channels_last)
+    new = optim.AdamW(b.parameters(), lr=1e-2)
+    new.load_state_dict(old.state_dict())
+    for p, q in zip(a.parameters(), b.parameters()):
+        g = torch.randn(p.shape, generator=torch.Generator(device="cuda").manual_seed(5), device=cuda)
+        p.grad, q.grad = g, g.clone()
+    old.step(), new.step()
+    assert all(new.state[p]["step"] == 4 for p in b.parameters())
+    for p, q in zip(a.parameters(), b.parameters()):
+        assert ((p - q).abs() <= 16 * 2.0 ** -24 * (q.abs() + 1) + 1e-2 * 2.0 ** -16).all()
+    with pytest.raises(ValueError, match="state_bits"):
+        optim.AdamW(b.parameters(), state_bits=8).load_state_dict(new.state_dict())
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_captured_step_replays(cuda, bits):
     """A captured step advances its own counter and reads the learning rate that is set between
@@ -435,6 +459,25 @@ def test_capturable_state_round_trip(cuda):
     assert [int(g["step"]) for g in o2.param_groups] == [4, 4]
     assert abs(float(o2.param_groups[0]["lr"]) - 5e-3) <= 2.0 ** -24 * 5e-3
     assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+
+
+@pytest.mark.parametrize("first", [False, True])
+def test_state_between_capturable_and_not(cuda, first):
+    """The step's number goes along whichever of the two saved it: the next step is the same."""
+    w = torch.nn.Parameter(torch.randn(500, device=cuda))
+    w.grad = torch.randn_like(w)
+    a = optim.AdamW([w], lr=1e-2, capturable=first)
+    for _ in range(3):
+        a.step()
+    v = torch.nn.Parameter(w.detach().clone())
+    v.grad = w.grad.clone()
+    b = optim.AdamW([v], lr=1e-2, capturable=not first)
+    b.load_state_dict(a.state_dict())
+    a.step(), b.step()
+    # the constants of the step come from lr as float32 on one side: one rounding of the update
+    assert ((w - v).abs() <= 4 * 2.0 ** -24 * (w.abs() + 1)).all()
+    n = b.param_groups[0]["step"] if not first else b.state[v]["step"]
+    assert int(n) == 4
 
 
 def test_capture_refuses_frozen_numbers(cuda):
