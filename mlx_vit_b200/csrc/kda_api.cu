@@ -81,10 +81,10 @@ const char *kda_strerror(int s) {
   switch (s) {
     case KDA_OK: return "ok";
     case KDA_ERR_INVALID_ARG: return "invalid argument (null pointer, non-positive size or bad descriptor)";
-    case KDA_ERR_UNSUPPORTED: return "unsupported shape: needs Dk == Dv, chunk <= 64, D <= 128";
+    case KDA_ERR_UNSUPPORTED: return "unsupported shape or option (the recurrence needs Dk == Dv, chunk <= 64, D <= 128)";
     case KDA_ERR_DTYPE: return "unsupported dtype code";
-    case KDA_ERR_MISALIGNED: return "pointer not 16-byte aligned";
-    case KDA_ERR_WORKSPACE: return "workspace missing or too small (see kda_workspace_bytes)";
+    case KDA_ERR_MISALIGNED: return "pointer or row pitch not aligned as the call needs it";
+    case KDA_ERR_WORKSPACE: return "workspace missing or too small (see the call's workspace query)";
     case KDA_ERR_CUDA: return "CUDA launch or runtime error";
     case KDA_ERR_TIMEOUT: return "a bounded device-side wait timed out";
     case KDA_ERR_SCRATCH_LIMIT: return "problem needs more workspace than kda_bwd_noalloc's static scratch (KDA_NOALLOC_SCRATCH_BYTES)";

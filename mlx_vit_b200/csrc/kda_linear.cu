@@ -13,7 +13,7 @@
 // memory k-contiguous ("K-major") or m- / n-contiguous ("MN-major": the transposes are read in
 // place).  Each persistent CTA (or pair of CTAs, CG = 2, whose tensor cores work on one tile and read
 // half of B each) walks its tiles with one thread copying operand blocks of 64 k by TMA into a
-// ring of stages, one thread issuing the products, and eight warps taking finished accumulators
+// ring of stages, one thread issuing the products, and sixteen warps taking finished accumulators
 // from tensor memory through the epilogue while the next tile's products run (two accumulators).
 // Rows, columns and k past the end are TMA's zero fill and clipped stores.  Where the tiles are too few
 // to fill the GPU, k is split: each part writes its float32 tile to a workspace and a second kernel
@@ -88,6 +88,10 @@ __device__ __forceinline__ void arrive_cluster(uint32_t addr) {  // addr: a shar
 }
 __device__ __forceinline__ bool wait(uint32_t mbar, uint32_t parity, int polls = kPolls) {
   return mbar_wait(mbar, parity, polls);
+}
+// by a whole warp, with one answer for it: a warp that elects threads must not part
+__device__ __forceinline__ bool wait_warp(uint32_t mbar, uint32_t parity) {
+  return __all_sync(0xFFFFFFFFu, wait(mbar, parity));
 }
 
 template <int CG>
@@ -304,10 +308,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   }
   uint8_t *staging = sm + S::kStages * S::kStage;
   T *bias_sm = reinterpret_cast<T *>(staging + kStaging);
-  // barriers: full[stages], empty[stages], acc_full[2], acc_empty[2], in[epilogue warps]; then tensor memory's address
+  // barriers: full[stages], empty[stages], acc_full[2], acc_empty[2], in[epilogue warps], idle; then tensor memory's address
   const uint32_t bars = smem_u32(bias_sm) + kEpiWarps * 128;
   const uint32_t full = bars, empty = full + 8 * S::kStages, acc_full = empty + 8 * S::kStages,
-                 acc_empty = acc_full + 16, in_bar = acc_empty + 16, tmem_at = in_bar + 8 * kEpiWarps;
+                 acc_empty = acc_full + 16, in_bar = acc_empty + 16, idle = in_bar + 8 * kEpiWarps, tmem_at = idle + 8;
   const int kblocks = (g.k + kBlockK - 1) / kBlockK;
   const int tiles = g.tiles_m * g.tiles_n, units = tiles * g.splits, first = blockIdx.x / CG, step = gridDim.x / CG;
 
@@ -321,6 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       mbar_init(acc_empty + 8 * i, kEpiWarps * CG);
     }
     for (int w = 0; w < kEpiWarps; ++w) mbar_init(in_bar + 8 * w, 1);
+    mbar_init(idle, 1);
     mbar_fence_init();
   }
   if (warp == 2) alloc<CG>(tmem_at, S::kCols);
@@ -341,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
       const int2 at_tile = place(t, g.tiles_m, g.tiles_n);
       const int m0 = at_tile.x * 128 * CG + (int)rank * 128, n0 = at_tile.y * BN + (int)rank * (BN / CG);
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!(ok = wait(empty + 8 * s, ph))) break;
+        if (!(ok = wait_warp(empty + 8 * s, ph))) break;
         const uint32_t at = base + s * S::kStage, bt = at + kStageA, fb = full_lead + 8 * s;
         if (elect()) {
           if (rank == 0) mbar_expect_tx(full + 8 * s, S::kStage * CG);
@@ -376,10 +381,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
         const int kb0 = u / tiles * g.per_split, kb1 = min(kblocks, kb0 + g.per_split);
         const uint32_t buf = n % S::kBufs, use = n / S::kBufs;
         const uint32_t d = tmem + buf * BN;
-        if (!(ok = wait(acc_empty + 8 * buf, (use & 1) ^ 1))) break;
+        if (!(ok = wait_warp(acc_empty + 8 * buf, (use & 1) ^ 1))) break;
         tc_fence_after();
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!(ok = wait(full + 8 * s, ph))) break;
+          if (!(ok = wait_warp(full + 8 * s, ph))) break;
           tc_fence_after();
           const uint32_t al = a_low + s * (S::kStage >> 4), bl = b_low + s * (S::kStage >> 4);
           if (elect()) {
@@ -392,6 +397,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
           __syncwarp();
           if (++s == S::kStages) s = 0, ph ^= 1;
         }
+      }
+      if (!ok) {  // gave up: let the products in flight end before tensor memory is freed
+        if (elect()) commit<CG>(idle);
+        __syncwarp();
+        mbar_wait(idle, 0, 1 << 16);
       }
     }
   } else if (warp >= kEpiWarp) {

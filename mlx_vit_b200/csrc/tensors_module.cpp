@@ -177,7 +177,9 @@ void done(int status, const char *where) {
 void *stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 bool capturing(void *st) {
   cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
-  return cudaStreamIsCapturing(static_cast<cudaStream_t>(st), &s) == cudaSuccess && s != cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(static_cast<cudaStream_t>(st), &s) == cudaSuccess) return s != cudaStreamCaptureStatusNone;
+  (void)cudaGetLastError();  // not a question for this stream now: the launch will say
+  return false;
 }
 at::Tensor adamw_workspace(int64_t count, const at::Device &dev) {
   return at::empty({(int64_t)kda_adamw_workspace_bytes(count)}, at::TensorOptions().dtype(at::kByte).device(dev));
