@@ -735,56 +735,78 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) few_rows_kernel(const FewAr
 // the column sums of dz.  A block takes 256 columns, 8 a thread (each matrix by 16 bytes where its
 // rows allow it), of a range of rows, 8 at a time; its sums meet in shared memory and go to its row of
 // partials.  Bound by its bytes.
-template <typename T, bool SUMS>
-__global__ void __launch_bounds__(256) act_grad_kernel(int act, int64_t rows, int cols, const T *dy, int64_t ldy, const T *z,
-                                                       int64_t ldz, T *dz, int64_t ldd, int vec_y, int vec_z, int vec_d,
-                                                       float *part, T *db) {
+template <typename T, int ACT, bool SUMS>
+__global__ void __launch_bounds__(256) act_grad_kernel(int64_t rows, int cols, const T *dy, int64_t ldy, const T *z, int64_t ldz,
+                                                       T *dz, int64_t ldd, int vec_y, int vec_z, int vec_d, float *part, T *db) {
   using P = Pair<T>;
-  auto load = [&](const T *p, bool vec, int k, float (&x)[8]) {
-    if (vec) {
-      const uint4 u = *reinterpret_cast<const uint4 *>(p);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  auto unpack = [](const uint4 &u, float (&x)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = P::unpack(w[j]);
-        x[2 * j] = f.x;
-        x[2 * j + 1] = f.y;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = j < k ? to_f<T>(p[j]) : 0.f;
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = P::unpack(w[j]);
+      x[2 * j] = f.x;
+      x[2 * j + 1] = f.y;
     }
   };
   const int c = blockIdx.x * 256 + threadIdx.x * 8, k = cols - c;
   float sum[8] = {};
-  if (k > 0) {
-#pragma unroll 4
-    for (int64_t r = (int64_t)blockIdx.y * 8 + threadIdx.y; r < rows; r += (int64_t)gridDim.y * 8) {
-      float x[8];
-      load(dy + r * ldy + c, vec_y && k >= 8, k, x);
-      if (z) {
-        float y[8];
-        load(z + r * ldz + c, vec_z && k >= 8, k, y);
+  auto finish = [&](float (&x)[8], const float (&y)[8]) {
+    if (ACT != KDA_ACT_NONE) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 g = activate_grad2(act, make_float2(y[2 * j], y[2 * j + 1]));
-          x[2 * j] *= g.x;
-          x[2 * j + 1] *= g.y;
-        }
+      for (int j = 0; j < 4; ++j) {
+        const float2 g = activate_grad2(ACT, make_float2(y[2 * j], y[2 * j + 1]));
+        x[2 * j] *= g.x;
+        x[2 * j + 1] *= g.y;
       }
-      if (SUMS) {
+    }
+    if (SUMS) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum[j] += x[j];
+      for (int j = 0; j < 8; ++j) sum[j] += x[j];
+    }
+  };
+  const int64_t step = (int64_t)gridDim.y * 8;
+  int64_t r = (int64_t)blockIdx.y * 8 + threadIdx.y;
+  if (k >= 8 && vec_y && (ACT == KDA_ACT_NONE || vec_z) && (!dz || vec_d)) {
+    constexpr int R = 4;  // rows whose loads are in flight together
+    for (; r < rows; r += R * step) {
+      uint4 a[R], b[R];
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        if (r + i * step >= rows) break;
+        a[i] = *reinterpret_cast<const uint4 *>(dy + (r + i * step) * ldy + c);
+        if (ACT != KDA_ACT_NONE) b[i] = *reinterpret_cast<const uint4 *>(z + (r + i * step) * ldz + c);
       }
-      if (dz) {
-        T *out = dz + r * ldd + c;
-        if (vec_d && k >= 8) {
-          *reinterpret_cast<uint4 *>(out) = make_uint4(P::pack(x[0], x[1]), P::pack(x[2], x[3]), P::pack(x[4], x[5]), P::pack(x[6], x[7]));
-        } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (j < k) out[j] = from_f<T>(x[j]);
-        }
+      for (int i = 0; i < R; ++i) {
+        if (r + i * step >= rows) break;
+        float x[8], y[8] = {};
+        unpack(a[i], x);
+        if (ACT != KDA_ACT_NONE) unpack(b[i], y);
+        finish(x, y);
+        if (dz)
+          *reinterpret_cast<uint4 *>(dz + (r + i * step) * ldd + c) =
+              make_uint4(P::pack(x[0], x[1]), P::pack(x[2], x[3]), P::pack(x[4], x[5]), P::pack(x[6], x[7]));
+      }
+    }
+  } else if (k > 0) {
+#pragma unroll 2
+    for (; r < rows; r += step) {
+      float x[8], y[8] = {};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = j < k ? to_f<T>(dy[r * ldy + c + j]) : 0.f;
+      if (ACT != KDA_ACT_NONE) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = j < k ? to_f<T>(z[r * ldz + c + j]) : 0.f;
+      }
+      finish(x, y);
+      if (!dz) continue;
+      T *out = dz + r * ldd + c;
+      if (vec_d && k >= 8) {
+        *reinterpret_cast<uint4 *>(out) = make_uint4(P::pack(x[0], x[1]), P::pack(x[2], x[3]), P::pack(x[4], x[5]), P::pack(x[6], x[7]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j < k) out[j] = from_f<T>(x[j]);
       }
     }
   }
@@ -882,9 +904,10 @@ static size_t part_bytes(const Plan &p, int64_t m, int64_t n) {
 static size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 // partial column sums of an [m][n] result: a row for every 32 of its rows
 static size_t sums_bytes(int64_t m, int64_t n) { return round16((size_t)((m + 31) / 32) * n * sizeof(float)); }
-// ... and of the activation-gradient pass: a row for every block of rows
+// ... and of the activation-gradient pass: a row for every block of rows.  Two turns of 8 rows a block while
+// that does not fill the GPU; few rows in one block, whose sums need no adding
 static int row_blocks(int64_t rows, int64_t cols, int sms) {
-  const int64_t across = (cols + 255) / 256, most = (8ll * sms + across - 1) / across, need = (rows + 63) / 64;
+  const int64_t across = (cols + 255) / 256, most = (8ll * sms + across - 1) / across, need = rows <= 64 ? 1 : (rows + 15) / 16;
   return (int)(need < most ? need : most);
 }
 template <typename T>
@@ -894,21 +917,34 @@ static int add_sums(const float *part, int parts, int cols, void *db, cudaStream
   count_launch();
   return KDA_OK;
 }
-template <typename T>
-static int act_grad(int act, int64_t rows, int64_t cols, const void *dy, int64_t ldy, const void *z, int64_t ldz, void *dz,
-                    int64_t ldd, void *db, void *ws, int sms, cudaStream_t st) {
+template <typename T, int ACT>
+static int act_grad(int64_t rows, int64_t cols, const void *dy, int64_t ldy, const void *z, int64_t ldz, void *dz, int64_t ldd,
+                    void *db, void *ws, int sms, cudaStream_t st) {
   const int blocks = row_blocks(rows, cols, sms);
   const dim3 grid((unsigned)((cols + 255) / 256), (unsigned)blocks), block(32, 8);
-  const T *y = static_cast<const T *>(dy), *zz = static_cast<const T *>(act ? z : nullptr);
+  const T *y = static_cast<const T *>(dy), *zz = static_cast<const T *>(z);
   T *out = static_cast<T *>(dz);
   const int vy = tma_able(dy, ldy), vz = tma_able(z, ldz), vd = tma_able(dz, ldd);  // 16-byte rows
   float *part = static_cast<float *>(ws);
-  if (db) act_grad_kernel<T, true><<<grid, block, 0, st>>>(act, rows, (int)cols, y, ldy, zz, ldz, out, ldd, vy, vz, vd, part,
-                                                            static_cast<T *>(db));
-  else act_grad_kernel<T, false><<<grid, block, 0, st>>>(act, rows, (int)cols, y, ldy, zz, ldz, out, ldd, vy, vz, vd, nullptr, nullptr);
+  if (db)
+    act_grad_kernel<T, ACT, true><<<grid, block, 0, st>>>(rows, (int)cols, y, ldy, zz, ldz, out, ldd, vy, vz, vd, part,
+                                                          static_cast<T *>(db));
+  else
+    act_grad_kernel<T, ACT, false><<<grid, block, 0, st>>>(rows, (int)cols, y, ldy, zz, ldz, out, ldd, vy, vz, vd, nullptr, nullptr);
   if (cudaGetLastError() != cudaSuccess) return KDA_ERR_CUDA;
   count_launch();
   return db && blocks > 1 ? add_sums<T>(part, blocks, (int)cols, db, st) : KDA_OK;
+}
+template <typename T>
+static int act_grad(int act, int64_t rows, int64_t cols, const void *dy, int64_t ldy, const void *z, int64_t ldz, void *dz,
+                    int64_t ldd, void *db, void *ws, int sms, cudaStream_t st) {
+  switch (act) {
+    case KDA_ACT_RELU: return act_grad<T, KDA_ACT_RELU>(rows, cols, dy, ldy, z, ldz, dz, ldd, db, ws, sms, st);
+    case KDA_ACT_SILU: return act_grad<T, KDA_ACT_SILU>(rows, cols, dy, ldy, z, ldz, dz, ldd, db, ws, sms, st);
+    case KDA_ACT_GELU: return act_grad<T, KDA_ACT_GELU>(rows, cols, dy, ldy, z, ldz, dz, ldd, db, ws, sms, st);
+    case KDA_ACT_GELU_TANH: return act_grad<T, KDA_ACT_GELU_TANH>(rows, cols, dy, ldy, z, ldz, dz, ldd, db, ws, sms, st);
+    default: return act_grad<T, KDA_ACT_NONE>(rows, cols, dy, ldy, z, ldz, dz, ldd, db, ws, sms, st);
+  }
 }
 
 template <typename T, int CG, int BN, bool A_MN, bool B_MN>
