@@ -256,9 +256,24 @@ __device__ __forceinline__ void finish8(float (&v)[8], uint4 *slot, bool add) {
     }
   }
 }
-// `keep`: the accumulator with its bias as it is (z), else finished.  bs: the chunk's bias.
+// Column lane % 8 of eight columns' sums over the warp's lanes: halves are exchanged while columns are
+// left, then the four groups of lanes are added.
+__device__ __forceinline__ float column_sum(const float (&v)[8], int lane) {
+  float a[4], b[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    a[i] = (lane & 4 ? v[i + 4] : v[i]) + __shfl_xor_sync(0xFFFFFFFFu, lane & 4 ? v[i] : v[i + 4], 4);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) b[i] = (lane & 2 ? a[i + 2] : a[i]) + __shfl_xor_sync(0xFFFFFFFFu, lane & 2 ? a[i] : a[i + 2], 2);
+  float s = (lane & 1 ? b[1] : b[0]) + __shfl_xor_sync(0xFFFFFFFFu, lane & 1 ? b[0] : b[1], 1);
+  s += __shfl_xor_sync(0xFFFFFFFFu, s, 8);
+  return s + __shfl_xor_sync(0xFFFFFFFFu, s, 16);
+}
+// `keep`: the accumulator with its bias as it is (z), else finished.  bs: the chunk's bias.  sums (kGrad, or
+// null): where the column sums of the warp's `rows` rows go, before they are rounded.
 template <typename T, int KIND, int ACT>
-__device__ __forceinline__ void chunk(const Args &g, uint32_t acc, uint8_t *so, const T *bs, int lane, bool keep) {
+__device__ __forceinline__ void chunk(const Args &g, uint32_t acc, uint8_t *so, const T *bs, int lane, bool keep,
+                                      float *sums = nullptr, int rows = 0, int cols = 0) {
   using P = Pair<T>;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -282,6 +297,14 @@ __device__ __forceinline__ void chunk(const Args &g, uint32_t acc, uint8_t *so, 
       }
       uint4 *slot = reinterpret_cast<uint4 *>(so + chunk_at(lane, 4 * h + u));
       if (!keep) finish8<T, KIND, ACT>(v, slot, g.in_kind == kInAdd);
+      if (KIND == kGrad && sums) {
+        float w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = lane < rows ? v[j] : 0.f;
+        const float s = column_sum(w, lane);
+        const int j = 32 * h + 8 * u + lane;
+        if (lane < 8 && j < cols) sums[j] = s;
+      }
       *slot = make_uint4(P::pack(v[0], v[1]), P::pack(v[2], v[3]), P::pack(v[4], v[5]), P::pack(v[6], v[7]));
     }
   }
@@ -496,25 +519,18 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
           chunk<T, kPlain, KDA_ACT_NONE>(g, acc + 64 * c, st, bs, lane, false);
         } else {
           constexpr int kind = B_MN ? kGrad : kForward;
+          float *sums = B_MN && g.sums ? g.sums + (int64_t)(row0 >> 5) * g.n + col0 : nullptr;
+          const uint32_t from = acc + 64 * c;
           switch (g.act) {
-            case KDA_ACT_RELU: chunk<T, kind, KDA_ACT_RELU>(g, acc + 64 * c, st, bs, lane, false); break;
-            case KDA_ACT_SILU: chunk<T, kind, KDA_ACT_SILU>(g, acc + 64 * c, st, bs, lane, false); break;
-            case KDA_ACT_GELU: chunk<T, kind, KDA_ACT_GELU>(g, acc + 64 * c, st, bs, lane, false); break;
-            case KDA_ACT_GELU_TANH: chunk<T, kind, KDA_ACT_GELU_TANH>(g, acc + 64 * c, st, bs, lane, false); break;
-            default: chunk<T, kind, KDA_ACT_NONE>(g, acc + 64 * c, st, bs, lane, false);
+            case KDA_ACT_RELU: chunk<T, kind, KDA_ACT_RELU>(g, from, st, bs, lane, false, sums, rows, cols); break;
+            case KDA_ACT_SILU: chunk<T, kind, KDA_ACT_SILU>(g, from, st, bs, lane, false, sums, rows, cols); break;
+            case KDA_ACT_GELU: chunk<T, kind, KDA_ACT_GELU>(g, from, st, bs, lane, false, sums, rows, cols); break;
+            case KDA_ACT_GELU_TANH: chunk<T, kind, KDA_ACT_GELU_TANH>(g, from, st, bs, lane, false, sums, rows, cols); break;
+            default: chunk<T, kind, KDA_ACT_NONE>(g, from, st, bs, lane, false, sums, rows, cols);
           }
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (B_MN && !A_MN && g.sums) {  // of columns 2 lane, 2 lane + 1 over the rows there are
-          float2 sum = both(0.f);
-#pragma unroll 8
-          for (int r = 0; r < rows; ++r)
-            sum = add2(sum, Pair<T>::unpack(*reinterpret_cast<const uint32_t *>(st + chunk_at(r, lane >> 2) + 4 * (lane & 3))));
-          float *to = g.sums + (int64_t)(row0 >> 5) * g.n + col0 + 2 * lane;
-          if (2 * lane < cols) to[0] = sum.x;
-          if (2 * lane + 1 < cols) to[1] = sum.y;
-        }
         if (g.out_tma) {
           if (lane == 0) {
             store_box(&g.out, st_at, col0, row0);
@@ -542,52 +558,65 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   if (warp == 2) dealloc<CG>(tmem, S::kCols);
 }
 
-// Adds the parts of a split product in their order and runs the epilogue.
-constexpr int kJoinRows = 4;  // rows a block of 64 x 4 threads takes; a thread takes 8 columns
-template <typename T>
+// Adds the parts of a split product in their order and runs the epilogue, with SUMS on 32 rows a block
+// whose column sums are its row of partials.
+constexpr int kJoinRows = 4;  // rows a block of 64 x 4 threads takes at once; a thread takes 8 columns
+template <typename T, bool SUMS>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args g, int64_t part_rows, int col_blocks) {
   using P = Pair<T>;
-  const int64_t blk = blockIdx.x;
-  const int64_t row = blk / col_blocks * kJoinRows + threadIdx.y;
-  const int col = (int)(blk % col_blocks) * 512 + threadIdx.x * 8;
-  if (row >= g.m || col >= g.n) return;
-  float v[8] = {};
-  for (int p = 0; p < g.splits; ++p) {  // whole vectors: the workspace's columns are padded to tiles
-    const float4 *src = reinterpret_cast<const float4 *>(g.part + (p * part_rows + row) * g.ldp + col);
-    const float4 a = src[0], b = src[1];
-    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-    v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
-  }
-  const int k = min(8, g.n - col);
-  if (g.bias) {
+  constexpr int kRows = SUMS ? 32 : kJoinRows;
+  const int64_t blk = blockIdx.x, row0 = blk / col_blocks * kRows;
+  const int col = (int)(blk % col_blocks) * 512 + threadIdx.x * 8, k = min(8, g.n - col);
+  float sum[8] = {};
+  for (int64_t row = row0 + threadIdx.y; k > 0 && row < min(row0 + kRows, (int64_t)g.m); row += kJoinRows) {
+    float v[8] = {};
+    for (int p = 0; p < g.splits; ++p) {  // whole vectors: the workspace's columns are padded to tiles
+      const float4 *src = reinterpret_cast<const float4 *>(g.part + (p * part_rows + row) * g.ldp + col);
+      const float4 a = src[0], b = src[1];
+      v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+      v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+    }
+    if (g.bias) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < k) v[j] += to_f<T>(static_cast<const T *>(g.bias)[col + j]);
-  }
-  if (g.save_z) {
-    T *z = static_cast<T *>(g.z_ptr) + row * g.ldz + col;
+      for (int j = 0; j < 8; ++j)
+        if (j < k) v[j] += to_f<T>(static_cast<const T *>(g.bias)[col + j]);
+    }
+    if (g.save_z) {
+      T *z = static_cast<T *>(g.z_ptr) + row * g.ldz + col;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < k) z[j] = from_f<T>(v[j]);
-  }
-  float x[8];
-  if (g.in_kind) {
-    const T *in = static_cast<const T *>(g.in_ptr) + row * g.ldi + col;
+      for (int j = 0; j < 8; ++j)
+        if (j < k) z[j] = from_f<T>(v[j]);
+    }
+    float x[8];
+    if (g.in_kind) {
+      const T *in = static_cast<const T *>(g.in_ptr) + row * g.ldi + col;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = j < k ? to_f<T>(in[j]) : 0.f;
-  }
+      for (int j = 0; j < 8; ++j) x[j] = j < k ? to_f<T>(in[j]) : 0.f;
+    }
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (g.in_kind == kInActGrad) v[j] *= activate_grad(g.act, x[j]);
-    else v[j] = activate(g.act, v[j]) + (g.in_kind == kInAdd ? x[j] : 0.f);
-  }
-  T *out = static_cast<T *>(g.out_ptr) + row * g.ldo + col;
-  if (k == 8 && g.out_tma) {
-    *reinterpret_cast<uint4 *>(out) = make_uint4(P::pack(v[0], v[1]), P::pack(v[2], v[3]), P::pack(v[4], v[5]), P::pack(v[6], v[7]));
-  } else {
+    for (int j = 0; j < 8; ++j) {
+      if (g.in_kind == kInActGrad) v[j] *= activate_grad(g.act, x[j]);
+      else v[j] = activate(g.act, v[j]) + (g.in_kind == kInAdd ? x[j] : 0.f);
+      if (SUMS) sum[j] += v[j];
+    }
+    T *out = static_cast<T *>(g.out_ptr) + row * g.ldo + col;
+    if (k == 8 && g.out_tma) {
+      *reinterpret_cast<uint4 *>(out) = make_uint4(P::pack(v[0], v[1]), P::pack(v[2], v[3]), P::pack(v[4], v[5]), P::pack(v[6], v[7]));
+    } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < k) out[j] = from_f<T>(v[j]);
+      for (int j = 0; j < 8; ++j)
+        if (j < k) out[j] = from_f<T>(v[j]);
+    }
+  }
+  if (SUMS) {
+    __shared__ float red[kJoinRows][512 + 8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) red[threadIdx.y][threadIdx.x * 8 + j] = sum[j];
+    __syncthreads();
+    for (int t = threadIdx.y * 64 + threadIdx.x; t < 512; t += 256) {
+      const int c = (int)(blk % col_blocks) * 512 + t;
+      if (c < g.n) g.sums[(row0 >> 5) * g.n + c] = red[0][t] + red[1][t] + red[2][t] + red[3][t];
+    }
   }
 }
 
@@ -1010,12 +1039,12 @@ static int run(Args &g, const Plan &p, const void *a, int64_t lda, const void *b
   if (s) return s;
   if (p.splits > 1) {
     const int col_blocks = (g.n + 511) / 512;
-    join_kernel<T><<<(unsigned)((int64_t)((g.m + kJoinRows - 1) / kJoinRows) * col_blocks), dim3(64, 4), 0, st>>>(g, rows, col_blocks);
+    const int per = db ? 32 : kJoinRows;
+    const unsigned blocks = (unsigned)((int64_t)((g.m + per - 1) / per) * col_blocks);
+    if (db) join_kernel<T, true><<<blocks, dim3(64, 4), 0, st>>>(g, rows, col_blocks);
+    else join_kernel<T, false><<<blocks, dim3(64, 4), 0, st>>>(g, rows, col_blocks);
     if (cudaGetLastError() != cudaSuccess) return KDA_ERR_CUDA;
     count_launch();
-    // the joined result's sums: a pass over it
-    if (db)
-      return act_grad<T>(KDA_ACT_NONE, g.m, g.n, g.out_ptr, g.ldo, nullptr, 0, nullptr, 0, db, g.sums, sms, st);
   }
   return db ? add_sums<T>(g.sums, (g.m + 31) / 32, g.n, db, st) : KDA_OK;
 }

@@ -276,6 +276,23 @@ def test_no_rows(cuda):
     assert y.shape == x.shape and (w.grad == 0).all() and (w2.grad == 0).all()
 
 
+@pytest.mark.parametrize("m,k,n,out", [(3000, 64, 1024, 512), (700, 40, 1001, 96), (300, 64, 136, 5000)])
+def test_bias_gradients_are_sums_of_unrounded_values(cuda, m, k, n, out):
+    """db1 and db2 are rounded once: what they sum, the gradient at z before it is stored, carries only
+    z's rounding (through act'') and the accumulation's; last case: the product below is split."""
+    g = gen(16)
+    x, dy = rnd(g, m, k, dt=torch.bfloat16), rnd(g, m, out, dt=torch.bfloat16)
+    w1, w2 = rnd(g, n, k, dt=torch.bfloat16, scale=k ** -0.5), rnd(g, out, n, dt=torch.bfloat16, scale=n ** -0.5)
+    b1 = rnd(g, n, dt=torch.bfloat16, scale=0.5).requires_grad_()
+    b2 = rnd(g, out, dt=torch.bfloat16).requires_grad_()
+    d1, d2 = torch.autograd.grad(mlp(x, w1, b1, w2, b2, "none"), (b1, b2), dy)
+    want = dy.double().sum(0)
+    near(d2, want, (m + 2) * U * dy.double().abs().sum(0) + 2.0 ** -8 * 1.01 * want.abs(), "db2")
+    dh, e = product(dy.double(), w2.double().t())
+    want = dh.sum(0)
+    near(d1, want, e.sum(0) + (m + 2) * U * dh.abs().sum(0) + 2.0 ** -8 * 1.01 * want.abs(), "db1")
+
+
 def test_bias_gradient_with_infinite_weights(cuda):
     """The hidden bias gradient sums the rows there are: those behind the last, zeros in the products, would
     turn an infinite weight into NaN."""
