@@ -190,6 +190,7 @@ def check_mlp(m, k, n, out, dtype, act, bias, residual, seed=0):
     ey = e * 1.01 + ea @ W2.abs().t()
     if bias:
         want = want + b2.detach().double()
+        ey = ey + U * want.abs()  # the sum with the bias is rounded before the residual may cancel it
     if residual:
         want = want + r.detach().double()
     near(y, want, ey + 2 * U * want.abs() + h * want.abs() * 1.01 + tiny, "y")

@@ -461,6 +461,28 @@ def test_capturable_state_round_trip(cuda):
     assert all(torch.equal(p, q) for p, q in zip(ps, qs))
 
 
+def test_captured_step_of_many_tensors(cuda):
+    """More tensors than the small table holds: the captured launch carries the whole table itself."""
+    def build():
+        torch.manual_seed(8)
+        ps = [torch.nn.Parameter(torch.randn(30 + i, device=cuda)) for i in range(500)]
+        for p in ps:
+            p.grad = torch.randn_like(p)
+        return ps, optim.AdamW(ps, lr=1e-2, max_grad_norm=3.0, capturable=True)
+
+    (ps, o), (qs, o2) = build(), build()
+    o.step(), o2.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o.step()
+    junk = [torch.randn(1 << 16, device=cuda) for _ in range(8)]  # memory that the host's lists might have held
+    for _ in range(3):
+        graph.replay()
+        o2.step()
+    del junk
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs)) and int(o.param_groups[0]["step"]) == 4
+
+
 @pytest.mark.parametrize("first", [False, True])
 def test_state_between_capturable_and_not(cuda, first):
     """The step's number goes along whichever of the two saved it: the next step is the same."""
