@@ -542,7 +542,9 @@ PyObject *linear_act(PyObject *, PyObject *args) {
     const Tensor x = operand(xo, "x", false), w = operand(wo, "weight", false), b = operand(bo, "bias", true),
                  r = operand(ro, "residual", true);
     check_operands(x, r, {{"weight", w, b}});
-    return THPVariable_Wrap(LinearAct::apply(x, w, maybe(b), maybe(r), (int64_t)act, grads_wanted(x, w, b, r)));
+    // nothing to record: the computation alone
+    if (!grads_wanted(x, w, b, r)) return THPVariable_Wrap(LinearAct::forward(nullptr, x, w, maybe(b), maybe(r), act, false));
+    return THPVariable_Wrap(LinearAct::apply(x, w, maybe(b), maybe(r), (int64_t)act, true));
   });
 }
 // mlp(x, w1, b1 or None, w2, b2 or None, act, residual or None) -> y
@@ -554,7 +556,9 @@ PyObject *mlp(PyObject *, PyObject *args) {
     const Tensor x = operand(xo, "x", false), w1 = operand(w1o, "w1", false), b1 = operand(b1o, "b1", true),
                  w2 = operand(w2o, "w2", false), b2 = operand(b2o, "b2", true), r = operand(ro, "residual", true);
     check_operands(x, r, {{"w1", w1, b1}, {"w2", w2, b2}});
-    return THPVariable_Wrap(Mlp::apply(x, w1, maybe(b1), w2, maybe(b2), maybe(r), (int64_t)act, grads_wanted(x, w1, b1, w2, b2, r)));
+    if (!grads_wanted(x, w1, b1, w2, b2, r))
+      return THPVariable_Wrap(Mlp::forward(nullptr, x, w1, maybe(b1), w2, maybe(b2), maybe(r), act, false));
+    return THPVariable_Wrap(Mlp::apply(x, w1, maybe(b1), w2, maybe(b2), maybe(r), (int64_t)act, true));
   });
 }
 
