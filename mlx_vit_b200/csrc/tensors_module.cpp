@@ -14,6 +14,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -371,6 +372,25 @@ variable_list once(variable_list grads) {
 using Maybe = std::optional<Tensor>;
 Maybe maybe(const Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); }
 Tensor plain(const Maybe &t) { return t ? *t : Tensor(); }
+// A leaf's accumulating node keeps the stream on which the leaf first entered a graph that still lives.  Where
+// that is the default stream, a backward pass that is being captured would have to wait on it, which invalidates
+// the capture inside torch's engine and ends the process: refused before.
+void refuse_uncapturable_leaves(const at::Device &dev) {
+  const c10::cuda::CUDAGuard guard(dev);
+  const c10::cuda::CUDAStream now = c10::cuda::getCurrentCUDAStream();
+  if (!capturing(now.stream())) return;
+  const std::shared_ptr<torch::autograd::Node> node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (size_t i = 0; i < node->num_outputs(); ++i) {
+    const torch::autograd::Edge &e = node->next_edge(i);
+    if (!e.function || !node->task_should_compute_output(i) || !dynamic_cast<torch::autograd::AccumulateGrad *>(e.function.get()))
+      continue;
+    const std::optional<c10::Stream> s = e.function->stream();
+    TORCH_CHECK(!s || *s != c10::cuda::getDefaultCUDAStream(now.device_index()).unwrap(),
+                "linear products: an operand entered a graph on the default stream that is still alive, so that its gradient "
+                "cannot be captured; release that graph's results, or run it on another stream");
+  }
+}
 // which of the tensor arguments need a gradient; an absent one has no edge in the graph
 struct Needs {
   const AutogradContext *ctx;
@@ -401,6 +421,7 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
     return y;
   }
   static variable_list backward(AutogradContext *ctx, variable_list dys) {
+    refuse_uncapturable_leaves(dys[0].device());
     const variable_list saved = ctx->get_saved_variables();
     const Tensor x = saved[0].detach(), w = saved[1].detach(), z = saved[2], dy = dys[0].detach();
     const int64_t n = w.size(0), k = w.size(1);
@@ -455,6 +476,7 @@ struct Mlp : public torch::autograd::Function<Mlp> {
     return y;
   }
   static variable_list backward(AutogradContext *ctx, variable_list dys) {
+    refuse_uncapturable_leaves(dys[0].device());
     const variable_list saved = ctx->get_saved_variables();
     const Tensor x = saved[0].detach(), w1 = saved[1].detach(), w2 = saved[2].detach(), h = saved[3], z = saved[4],
                  dy = dys[0].detach();

@@ -6,6 +6,7 @@ far under h at these sizes but carried along.  y: that error times the activatio
 most 1.13), the activation's own error (3.0e-5 relative of the normal tail, which is at most that of the
 result, and 2e-9 where the tail is cut; a few u else), and h of the result.  z and the gradient at z are stored in 16 bits: h of each, through the
 second derivative (at most 0.8) and the next product."""
+import gc
 import math
 
 import pytest
@@ -404,6 +405,52 @@ def test_capture_and_two_streams(cuda):
     torch.cuda.synchronize()
     for o, want in zip(got, eager):
         assert all(torch.equal(a, b) for a, b in zip(o, want))
+    assert _lib.lib().kda_device_status(0) == 0
+
+
+@pytest.mark.parametrize("which", ["linear_act", "mlp", "residual"])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_capture_beside_an_eager_graph_is_refused(cuda, which, accumulate):
+    """A leaf whose eager graph on the default stream is alive: its captured backward raises, nothing is left
+    invalid, and once that graph is gone the same step is captured and replays as eager."""
+    g = gen(12)
+    x, w = rnd(g, 70, 64, dt=torch.bfloat16), rnd(g, 64, 64, dt=torch.bfloat16, scale=0.1)
+    r = rnd(g, 70, 64, dt=torch.bfloat16)
+    leaves = [r] if which == "residual" else [x, w]
+    for t in leaves:
+        t.requires_grad_()
+
+    def forward():
+        return linear_act(x, w, None, "silu", r) if which != "mlp" else mlp(x, w, None, w, None, "silu", r)
+
+    def step():
+        y = forward()
+        if accumulate:
+            y.backward(torch.ones_like(y))
+            return [t.grad for t in leaves]
+        return torch.autograd.grad(y, leaves, torch.ones_like(y))
+
+    def captured():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        return graph, out
+
+    alive = forward()
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        captured()
+    torch.cuda.synchronize()
+    want = [t.clone() for t in torch.autograd.grad(alive, leaves, torch.ones_like(alive))]
+    del alive
+    gc.collect()
+    for t in leaves:
+        t.grad = None
+    graph, out = captured()
+    for t in out:
+        t.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
     assert _lib.lib().kda_device_status(0) == 0
 
 
