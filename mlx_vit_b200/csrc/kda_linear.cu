@@ -639,11 +639,11 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
 // The weights' bytes bound it: each is read once, straight into the fragments of m16n8k16 products
 // whose 16 rows are rows of x and whose 8 columns are 8 outputs.  k may be summed in any order, so a
 // lane's share of two products is 8 consecutive k (one 16-byte load of W, one of each row of x)
-// instead of the layout's pairs.  `kw` warps share 8 outputs, each with its range of k, and the next eight
+// instead of the layout's pairs.  `kw` warps share 8 or 16 outputs, each with its range of k, and the next eight
 // loads of W a lane (4 KB a warp) are in flight while the last eight are multiplied; x comes
 // through the first-level cache, which W's loads pass by.  The warps' sums meet in shared memory.
-// Measured from memory, a call in a graph: 1 x 2048 x 8192 8.9 us (3.8 TB/s), 16 rows 9.9 us, 1 x 768 x 768
-// 3.4 us; with the loads not in flight during the products 10.8, 13.4 and 5.0 us.
+// Measured from memory, a call in a graph: 1 x 8192 x 2048 7.9 us (4.2 TB/s), 16 rows 9.8 us, 1 x 768 x 768
+// 3.4 us, 1 x 50000 x 1024 21.3 us (4.8 TB/s).  Bound by the loads in flight while a wave starts and ends.
 template <typename T>
 __device__ __forceinline__ void mma_m16n8k16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                              uint32_t b1) {
@@ -681,8 +681,7 @@ struct FewArgs {
   int m, n, k, act;
 };
 constexpr int kFewRows = 32, kFewWarps = 8;
-// MT groups of 8 rows of x (1, 2 or 4) by NB groups of 8 outputs a warp: with more rows of x two, so that a
-// load of x serves two products
+// MT groups of 8 rows of x (1, 2 or 4) by NB groups of 8 outputs a warp; with two a load of x serves two products
 template <typename T, int MT, int NB>
 __global__ void __launch_bounds__(32 * kFewWarps, 2) few_rows_kernel(const FewArgs a, int kw, int range) {
   __shared__ float red[kFewWarps][8 * MT][8 * NB + 1];
@@ -1068,10 +1067,13 @@ static int run(Args &g, const Plan &p, const void *a, int64_t lda, const void *b
 
 template <typename T, int MT, int NB>
 static int few_rows(const FewArgs &a, int sms, cudaStream_t st) {
-  // warps per group of outputs: enough that some 12 warps an SM stream weights, at most a CTA's
+  // warps per group of outputs: the fewest within a tenth of the least time, waves of CTAs by a warp's share of k
+  // (16 x 11008 x 4096: two warps 25.0 us, four, whose CTAs leave a second wave of 48, 28.0)
   const int groups = (a.n + 8 * NB - 1) / (8 * NB);
   int kw = 1;
-  while (kw < kFewWarps && (int64_t)groups * kw < 12ll * sms) kw *= 2;
+  auto time = [&](int w) { return (double)(((int64_t)groups * w + 2 * kFewWarps * sms - 1) / (2 * kFewWarps * sms)) / w; };
+  for (int w = 2; w <= kFewWarps; w *= 2)
+    if (time(w) < 0.9 * time(kw)) kw = w;
   const int range = ((a.k + 31) / 32 + kw - 1) / kw * 32, per = kFewWarps / kw;
   few_rows_kernel<T, MT, NB><<<(groups + per - 1) / per, 32 * kFewWarps, 0, st>>>(a, kw, range);
   if (cudaGetLastError() != cudaSuccess) return KDA_ERR_CUDA;
@@ -1080,7 +1082,12 @@ static int few_rows(const FewArgs &a, int sms, cudaStream_t st) {
 }
 template <typename T>
 static int few_rows(const FewArgs &a, int sms, cudaStream_t st) {
-  return a.m <= 8 ? few_rows<T, 1, 1>(a, sms, st) : a.m <= 16 ? few_rows<T, 2, 2>(a, sms, st) : few_rows<T, 4, 2>(a, sms, st);
+  // eight outputs a warp where their CTAs, eight warps for each, are resident at once (with more than 16 rows: one an
+  // SM), sixteen where they are not: 16 x 512 x 2048 3.6 us by eight, 4.6 by sixteen, 16 x 2048 x 8192 10.9
+  // and 12.0, 16 x 8192 x 2048 11.2 and 9.8, 1 x 8192 x 2048 8.9 and 7.9, 32 x 1024 x 4096 7.2 and 8.5
+  const bool narrow = (a.n + 7) / 8 <= (a.m <= 16 ? 2 : 1) * sms;
+  if (narrow) return a.m <= 8 ? few_rows<T, 1, 1>(a, sms, st) : a.m <= 16 ? few_rows<T, 2, 1>(a, sms, st) : few_rows<T, 4, 1>(a, sms, st);
+  return a.m <= 8 ? few_rows<T, 1, 2>(a, sms, st) : a.m <= 16 ? few_rows<T, 2, 2>(a, sms, st) : few_rows<T, 4, 2>(a, sms, st);
 }
 
 static int set_out(Args &g, void *p, int64_t ld) {

@@ -168,6 +168,13 @@ def test_few_rows(cuda, m):
     check_linear(m, 130, 4097, "fp16", "silu", True, True, seed=m, train=False)
 
 
+@pytest.mark.parametrize("n,k", [(1185, 264), (2369, 104), (3001, 40), (9001, 72), (11008, 520), (40003, 136)])
+@pytest.mark.parametrize("m", [1, 9, 16, 17, 32])
+def test_few_rows_by_many_outputs(cuda, m, n, k):
+    """Every split of k over the warps of a CTA, 8 and 16 outputs a warp."""
+    check_linear(m, n, k, "bf16", "silu", True, True, seed=m, train=False)
+
+
 def check_mlp(m, k, n, out, dtype, act, bias, residual, seed=0):
     dt, h = DT[dtype], torch.finfo(DT[dtype]).eps / 2
     tiny = float(torch.finfo(dt).tiny) * torch.finfo(dt).eps
