@@ -17,7 +17,7 @@
 // from tensor memory through the epilogue while the next tile's products run (two accumulators).
 // Rows, columns and k past the end are TMA's zero fill and clipped stores.  Where the tiles are too few
 // to fill the GPU, k is split: each part writes its float32 tile to a workspace and a second kernel
-// adds the parts in order and runs the epilogue.  A few rows (M <= 32) take a kernel of their own
+// adds the parts in order and runs the epilogue.  A few rows (M <= 16, <= 32 of fewer outputs) take a kernel of their own
 // that streams the weights once through registers.
 //
 // Bound by the tensor cores where the tiles fill the GPU: 4096 x 2048 x 8192 in bf16 92-98 us (1400-1490
@@ -681,6 +681,10 @@ struct FewArgs {
   int m, n, k, act;
 };
 constexpr int kFewRows = 32, kFewWarps = 8;
+// With more than 16 rows x's way through the first-level cache bounds it; from 64 outputs an SM on the tiled kernel's
+// tile for each is as fast or faster: 32 x 11008 x 4096 32.8 us here, 27.0 in tiles, 32 x 20000 x 512 18.3 and
+// 11.5, 32 x 9473 x 2048 (one tile more than SMs) 19.7 and 18.8, 17 rows 17.9 and 21.5
+static bool is_few(int64_t m, int64_t n, int sms) { return m <= 16 || (m <= kFewRows && n <= 64ll * sms); }
 // MT groups of 8 rows of x (1, 2 or 4) by NB groups of 8 outputs a warp; with two a load of x serves two products
 template <typename T, int MT, int NB>
 __global__ void __launch_bounds__(32 * kFewWarps, 2) few_rows_kernel(const FewArgs a, int kw, int range) {
@@ -1146,7 +1150,7 @@ size_t kda_linear_workspace_bytes(int op, int64_t M, int64_t N, int64_t K, int w
   if (check(KDA_BF16, KDA_ACT_NONE, M, N, K)) return 0;
   int sms = device_sms();
   if (!sms) sms = 148;  // no device: the size on a B200
-  if (op == KDA_LINEAR_FWD) return M <= kFewRows ? 0 : part_bytes(plan_for(M, N, K, sms, true), M, N);
+  if (op == KDA_LINEAR_FWD) return is_few(M, N, sms) ? 0 : part_bytes(plan_for(M, N, K, sms, true), M, N);
   if (op == KDA_LINEAR_DGRAD) return part_bytes(plan_for(M, K, N, sms, true), M, K) + (with_db ? sums_bytes(M, K) : 0);
   if (op == KDA_LINEAR_WGRAD) return part_bytes(plan_for(N, K, M, sms, true), N, K);
   if (op == KDA_LINEAR_ACT_GRAD) return with_db ? round16((size_t)row_blocks(M, N, sms) * N * sizeof(float)) : 0;
@@ -1166,7 +1170,7 @@ int kda_linear_fwd(int dtype, int act, int64_t M, int64_t N, int64_t K, const vo
   const int sms = device_sms();
   if (!sms) return KDA_ERR_CUDA;
   cudaStream_t st = (cudaStream_t)stream;
-  if (M <= kFewRows) {
+  if (is_few(M, N, sms)) {
     const FewArgs a = {x, w, bias, residual, y, z, ldx, ldw, ldr, ldy, ldz, (int)M, (int)N, (int)K, act};
     return dtype == KDA_BF16 ? few_rows<__nv_bfloat16>(a, sms, st) : few_rows<__half>(a, sms, st);
   }
