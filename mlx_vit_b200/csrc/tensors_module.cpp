@@ -430,7 +430,9 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
     Needs needs{ctx};
     const bool need_x = needs(true), need_w = needs(true), need_b = needs(ctx->saved_data["bias"].toBool());
     variable_list g(6);
-    if (needs(ctx->saved_data["residual"].toBool())) g[3] = dy;
+    // dys[0] itself, whose owners torch counts before it keeps a gradient: dy, a tensor of its own over the same
+    // memory, would be kept as it is and then written to
+    if (needs(ctx->saved_data["residual"].toBool())) g[3] = dys[0];
     if (x.numel() == 0) {
       if (need_x) g[0] = at::zeros(sizes, x.options());
       if (need_w) g[1] = at::zeros_like(w);
@@ -487,7 +489,8 @@ struct Mlp : public torch::autograd::Function<Mlp> {
     const bool need_x = needs(true), need_w1 = needs(true), need_b1 = needs(ctx->saved_data["bias1"].toBool()),
                need_w2 = needs(true), need_b2 = needs(ctx->saved_data["bias2"].toBool());
     variable_list g(8);
-    if (needs(ctx->saved_data["residual"].toBool())) g[5] = dy;
+    // as in LinearAct
+    if (needs(ctx->saved_data["residual"].toBool())) g[5] = dys[0];
     if (x.numel() == 0) {
       if (need_x) g[0] = at::zeros(sizes, x.options());
       if (need_w1) g[1] = at::zeros_like(w1);

@@ -491,3 +491,31 @@ def test_gradient_against_differences(cuda, act):
         d = grad.double() / grad.double().norm()
         diff = (move(1e-4, d) - move(-1e-4, d)) / 2e-4
         assert abs(diff - float((grad.double() * d).sum())) <= 4e-3 * abs(diff)
+
+
+@pytest.mark.parametrize("which", ["linear_act", "mlp"])
+def test_residual_gradient_is_its_own(cuda, which):
+    """A leaf residual's gradient accumulates in memory of its own, beside the dy that the caller keeps and
+    beside the gradient of another leaf that the same dy reaches."""
+    g = gen(17)
+    x, w = rnd(g, 40, 64, dt=torch.bfloat16), rnd(g, 64, 64, dt=torch.bfloat16, scale=0.1)
+    r, other = (torch.zeros(40, 64, dtype=torch.bfloat16, device=cuda, requires_grad=True) for _ in range(2))
+
+    def forward():
+        return linear_act(x, w, None, "none", r) if which == "linear_act" else mlp(x, w, None, w, None, "relu", r)
+
+    dy = torch.ones(40, 64, dtype=torch.bfloat16, device=cuda)
+    for n in (1, 2, 3):
+        forward().backward(dy)
+        assert (r.grad == n).all() and (dy == 1).all()
+    r.grad.zero_()
+    assert (dy == 1).all()
+    for y in (lambda: forward() + other, lambda: other + forward()):
+        r.grad = other.grad = None
+        y().sum().backward()
+        r.grad.mul_(5)
+        assert (other.grad == 1).all()
+        y().backward(dy)
+        assert (other.grad == 2).all() and (r.grad == 6).all() and (dy == 1).all()
+    gr, = torch.autograd.grad(forward(), r, dy)
+    assert torch.equal(gr, dy)
