@@ -530,7 +530,17 @@ struct Layer {
   const char *name;
   const Tensor &w, &b;
 };
+// a tangent is not carried along, and a result without one would count as constant
+void refuse_tangent(const Tensor &t) {
+  TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "linear products: no forward-mode derivatives");
+}
 void check_operands(const Tensor &x, const Tensor &r, std::initializer_list<Layer> layers) {
+  refuse_tangent(x);
+  refuse_tangent(r);
+  for (const Layer &l : layers) {
+    refuse_tangent(l.w);
+    refuse_tangent(l.b);
+  }
   need(x.is_cuda(), "linear products take CUDA tensors; there is no CPU path");
   need(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, "linear products take bfloat16 or float16");
   need(x.dim() >= 1, "x must have at least one dimension");

@@ -11,6 +11,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd_ad
 
 from mlx_vit_b200 import _lib
 from mlx_vit_b200.linear import ACTIVATIONS, linear_act, mlp
@@ -519,3 +520,26 @@ def test_residual_gradient_is_its_own(cuda, which):
         assert (other.grad == 2).all() and (r.grad == 6).all() and (dy == 1).all()
     gr, = torch.autograd.grad(forward(), r, dy)
     assert torch.equal(gr, dy)
+
+
+def test_forward_mode_is_refused(cuda):
+    """A tangent at any operand is refused, whether gradients are recorded or not: no result without one."""
+    g = gen(18)
+    x, w, b, r = (rnd(g, *s, dt=torch.bfloat16) for s in ((40, 64), (64, 64), (64,), (40, 64)))
+    with fwd_ad.dual_level():
+        for i in range(4):
+            ops = [fwd_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate((x, w, b, r))]
+            calls = [lambda: linear_act(*ops[:3], "gelu", ops[3]), lambda: mlp(ops[0], w, None, ops[1], ops[2], "gelu", ops[3]),
+                     lambda: mlp(ops[0], ops[1], ops[2], w, None, "gelu", ops[3])]
+            for call in calls:
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+                with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+        assert fwd_ad.unpack_dual(linear_act(x, w, b, "gelu", r)).tangent is None
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: linear_act(t, w), (x,), (torch.ones_like(x),))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: linear_act(t, w))(x.view(4, 10, 64))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: linear_act(t, w).float().sum())(x)
