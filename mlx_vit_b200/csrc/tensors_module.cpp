@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/cuda/CUDAContextLight.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -17,6 +18,7 @@
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <cstdint>
@@ -535,6 +537,10 @@ void refuse_tangent(const Tensor &t) {
   TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "linear products: no forward-mode derivatives");
 }
 void check_operands(const Tensor &x, const Tensor &r, std::initializer_list<Layer> layers) {
+  // a tracer (torch.jit.trace, make_fx) would record the results' allocation and not what fills them
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  TORCH_CHECK(!torch::jit::tracer::isTracing() && !Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY),
+              "linear products cannot be traced");
   refuse_tangent(x);
   refuse_tangent(r);
   for (const Layer &l : layers) {

@@ -32,8 +32,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     x is (..., in_features), weight (out_features, in_features), bias (out_features,), residual
     (..., out_features); all bf16 or all fp16, on one device, any strides.  ``activation`` is "none",
     "relu", "silu", "gelu" (exact) or "gelu_tanh".  Sizes or strides that 16 bytes do not divide are
-    taken through padded copies.  Differentiable once in every tensor, in reverse mode (forward-mode
-    tangents raise)."""
+    taken through padded copies.  Differentiable once in every tensor, in reverse mode; forward-mode
+    tangents, ``torch.func``'s transforms and tracers raise."""
     return _lib.tensors().linear_act(x, weight, bias, _act(activation), residual)
 
 

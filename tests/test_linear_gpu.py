@@ -543,3 +543,22 @@ def test_forward_mode_is_refused(cuda):
         torch.func.vmap(lambda t: linear_act(t, w))(x.view(4, 10, 64))
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda t: linear_act(t, w).float().sum())(x)
+
+
+def test_tracers_are_refused(cuda):
+    """A tracer sees the allocation of the result and not the kernels that fill it: what it recorded would return
+    memory that no one wrote."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    g = gen(19)
+    x, w = rnd(g, 40, 64, dt=torch.bfloat16), rnd(g, 64, 64, dt=torch.bfloat16)
+    for f in (lambda t: linear_act(t, w), lambda t: mlp(t, w, None, w, None, "relu", t)):
+        for leaf in (x, x.clone().requires_grad_()):
+            with pytest.raises(RuntimeError, match="traced"):
+                torch.jit.trace(f, (leaf,))
+            with pytest.raises(RuntimeError, match="traced"):
+                make_fx(f)(leaf)
+            with pytest.raises(RuntimeError):
+                make_fx(f, tracing_mode="fake")(leaf)
+        compiled = torch.compile(f, backend="eager")  # leaves the graph around the call
+        assert torch.equal(compiled(x), f(x))
