@@ -198,7 +198,13 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, but the states keep their own dtypes (torch casts them to the parameters').  The
-        float32 states of a ``torch.optim.AdamW`` can be loaded into one of 32 bits."""
+        float32 states of a ``torch.optim.AdamW`` can be loaded into one of 32 bits, unless its groups ask
+        for another rule than this one's (``maximize``, ``amsgrad``, decay that is not decoupled)."""
+        for g in state_dict["param_groups"]:
+            for name in ("maximize", "amsgrad"):
+                _need(not g.get(name), f"the loaded states are of an optimizer with {name}, which this one has not")
+            _need(g.get("decoupled_weight_decay", True) or not g.get("weight_decay"),
+                  "the loaded states are of an optimizer whose weight decay is not decoupled")
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i in ids:
             held = state_dict["state"].get(i)

@@ -100,3 +100,28 @@ def test_hash_spreads():
     h = mix(np.arange(1 << 16, dtype=np.uint64))
     assert len(set(h.tolist())) == 1 << 16
     assert abs((h & np.uint64(0xFFFF)).mean() / 65535 - 0.5) < 0.01
+
+
+def torch_states(opt, *ps, **kw):
+    """The state dict of a torch optimizer after one step over parameters like these."""
+    qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+    for q in qs:
+        q.grad = torch.ones_like(q)
+    old = opt(qs, **kw)
+    old.step()
+    return old.state_dict()
+
+
+@pytest.mark.parametrize("opt,kw,name", [(torch.optim.AdamW, dict(maximize=True), "maximize"),
+                                         (torch.optim.AdamW, dict(amsgrad=True), "amsgrad"),
+                                         (torch.optim.Adam, dict(weight_decay=0.1), "decoupled")])
+def test_states_of_another_rule_are_refused(opt, kw, name):
+    """What a loaded group asks for and the step does not do; nothing is loaded."""
+    p = torch.nn.Parameter(torch.randn(6))
+    new = optim.AdamW([p], lr=0.5)
+    with pytest.raises(ValueError, match=name):
+        new.load_state_dict(torch_states(opt, p, **kw))
+    assert not new.state and new.param_groups[0]["lr"] == 0.5
+    new.load_state_dict(torch_states(torch.optim.AdamW, p, lr=0.25))
+    new.load_state_dict(torch_states(torch.optim.Adam, p, lr=0.25))  # without decay the two are one rule
+    assert new.state[p]["step"] == 1 and new.param_groups[0]["lr"] == 0.25
