@@ -96,9 +96,9 @@ class AdamW(torch.optim.Optimizer):
 
     ``state_bits`` 32 or 8; ``max_grad_norm`` clips the global norm over all groups (the last
     step's norm is ``self.grad_norm``); ``ema_decay`` keeps a float32 shadow of every parameter
-    (``ema_of``), started at the parameter's first step.  ``capturable`` keeps the step's number
-    and the learning rate on the device, so that ``step`` can be captured into a CUDA graph
-    after one eager step; the parameters of a group then share one step number and all need
+    (``ema_of``), started at the parameter's first step, or the first after states without a shadow
+    were loaded.  ``capturable`` keeps the step's number and the learning rate on the device, so that
+    ``step`` can be captured into a CUDA graph after one eager step; the parameters of a group then share one step number and all need
     gradients, and ``lr`` is the tensor ``group["lr"]`` (fill it to change it).
     """
 
@@ -122,15 +122,21 @@ class AdamW(torch.optim.Optimizer):
         """The shadow average of a parameter, in its shape (float32)."""
         return self.state[p]["ema"].as_strided(p.shape, p.stride())
 
-    def _init_state(self, p):
+    def _lacks_state(self, p):
         st = self.state[p]
-        if not self.capturable:
-            st["step"] = 0
-        for name in ("exp_avg", "exp_avg_sq"):
-            if self.state_bits == 8:
-                st[name], st[name + "_exp"] = zeros_state8(p)
-            else:
-                st[name] = torch.zeros(p.numel(), dtype=torch.float32, device=p.device)
+        return not st or (self.ema_decay is not None and "ema" not in st)
+
+    def _init_state(self, p):
+        """The state of a parameter that has none, and the shadow of one whose loaded state has none."""
+        st = self.state[p]
+        if not st:
+            if not self.capturable:
+                st["step"] = 0
+            for name in ("exp_avg", "exp_avg_sq"):
+                if self.state_bits == 8:
+                    st[name], st[name + "_exp"] = zeros_state8(p)
+                else:
+                    st[name] = torch.zeros(p.numel(), dtype=torch.float32, device=p.device)
         if self.ema_decay is not None:  # in the parameter's order in memory, as every state
             st["ema"] = p.detach().as_strided((p.numel(),), (1,)).float().clone()
         return st
@@ -155,7 +161,7 @@ class AdamW(torch.optim.Optimizer):
             if capturing and not self.capturable:
                 raise ValueError("AdamW: a step is captured into a graph with capturable=True only")
             for p in live:
-                if not self.state[p]:
+                if self._lacks_state(p):
                     if capturing:
                         raise ValueError("AdamW: take one step before a step is captured into a graph")
                     self._init_state(p)

@@ -125,3 +125,15 @@ def test_states_of_another_rule_are_refused(opt, kw, name):
     new.load_state_dict(torch_states(torch.optim.AdamW, p, lr=0.25))
     new.load_state_dict(torch_states(torch.optim.Adam, p, lr=0.25))  # without decay the two are one rule
     assert new.state[p]["step"] == 1 and new.param_groups[0]["lr"] == 0.25
+
+
+def test_a_loaded_state_without_a_shadow_starts_one():
+    """The shadow starts at the parameter's next step, from what the parameter is then."""
+    p = torch.nn.Parameter(torch.randn(6))
+    new = optim.AdamW([p], ema_decay=0.9)
+    new.load_state_dict(torch_states(torch.optim.AdamW, p))
+    p.data.fill_(2.0)  # a model's weights may be loaded after its optimizer's states
+    p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError, match="no CPU path"):
+        new.step()
+    assert (new.ema_of(p) == 2).all() and new.state[p]["step"] == 1 and (new.state[p]["exp_avg"] != 0).all()

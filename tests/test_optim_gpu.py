@@ -555,3 +555,30 @@ def test_offsets_past_32_bits(cuda):
     want, _, _ = adamw64(np.zeros(1000), np64(g[-1000:]), 0.0, 0.0, 1, 3e-3, 0.9, 0.999, 1e-8, 0.1)
     assert (np.abs(np64(p[-1000:]) - want) <= 1.01 * 2.0 ** -8 * np.abs(want)).all()
     assert int(m[0][:-1000].max()) == 0 and int(v[1][:-4].max()) == 0
+
+
+def test_a_torch_state_gets_a_shadow(cuda):
+    """A run that torch.optim.AdamW began goes on with a shadow average, which starts at its next step; a captured step
+    wants that start behind it."""
+    a, b = params_of(cuda), params_of(cuda)
+    old = torch.optim.AdamW(a.parameters(), lr=1e-2)
+    backward(a, 0)
+    old.step()
+    b.load_state_dict(a.state_dict())
+    for capturable in (False, True):
+        new = optim.AdamW(b.parameters(), lr=1e-2, ema_decay=0.9, capturable=capturable)
+        new.load_state_dict(old.state_dict())
+        before = [p.detach().clone() for p in b.parameters()]
+        b.zero_grad()
+        backward(b, 1)
+        if capturable:
+            for g in new.param_groups:
+                g["step"], g["lr"] = torch.tensor(g["step"], device=cuda), torch.tensor(g["lr"], device=cuda)
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                with pytest.raises(ValueError, match="captured"):
+                    new.step()
+                next(b.parameters()).grad.mul_(1.0)
+        new.step()
+        for p, q in zip(b.parameters(), before):
+            want = 0.9 * q.double() + 0.1 * p.detach().double()
+            assert ((new.ema_of(p).double() - want).abs() <= 4 * 2.0 ** -24 * (p.detach().abs() + q.abs())).all()
