@@ -203,9 +203,10 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """As torch's, but the states keep their own dtypes (torch casts them to the parameters').  The
-        float32 states of a ``torch.optim.AdamW`` can be loaded into one of 32 bits, unless its groups ask
-        for another rule than this one's (``maximize``, ``amsgrad``, decay that is not decoupled)."""
+        """As torch's, but the states are not cast to the parameters' dtypes.  The states of a
+        ``torch.optim.AdamW`` can be loaded into one of 32 bits (in float32, whatever they were), unless
+        its groups ask for another rule than this one's (``maximize``, ``amsgrad``, decay that is not
+        decoupled)."""
         for g in state_dict["param_groups"]:
             for name in ("maximize", "amsgrad"):
                 _need(not g.get(name), f"the loaded states are of an optimizer with {name}, which this one has not")
@@ -236,11 +237,14 @@ class AdamW(torch.optim.Optimizer):
                     st["step"] = n
 
     def _own(self, name, v, p):
-        """A loaded state entry as this optimizer holds it: tensors flat, in the parameter's order in memory."""
+        """A loaded state entry as this optimizer holds it: tensors flat, in the parameter's order in memory,
+        codes and exponents as they are, others in float32."""
         if name == "step":
             return int(v)
         if not isinstance(v, torch.Tensor):
             return v
-        if v.dtype != torch.uint8 and v.dim() != 1 and v.shape == p.shape:
+        if v.dtype == torch.uint8:
+            return v.to(p.device, copy=True)
+        if v.dim() != 1 and v.shape == p.shape:
             return torch.empty_like(p, dtype=torch.float32).copy_(v).as_strided((p.numel(),), (1,))
-        return v.to(p.device, copy=True)
+        return v.to(p.device, torch.float32, copy=True)

@@ -137,3 +137,21 @@ def test_a_loaded_state_without_a_shadow_starts_one():
     with pytest.raises(ValueError, match="no CPU path"):
         new.step()
     assert (new.ema_of(p) == 2).all() and new.state[p]["step"] == 1 and (new.state[p]["exp_avg"] != 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_loaded_states_are_float32(dtype):
+    """torch holds a 16-bit parameter's states in 16 bits, those of biases and norms, of one dimension, too."""
+    ps = [torch.nn.Parameter(torch.randn(s).to(dtype)) for s in ((6,), (3, 4), (), (2, 1, 5))]
+    states = torch_states(torch.optim.AdamW, *ps)
+    assert states["state"][0]["exp_avg"].dtype == dtype
+    new = optim.AdamW(ps)
+    new.load_state_dict(states)
+    for i, p in enumerate(ps):
+        for name in ("exp_avg", "exp_avg_sq"):
+            held = new.state[p][name]
+            assert held.dtype == torch.float32 and held.shape == (p.numel(),)
+            assert torch.equal(held, states["state"][i][name].float().reshape(-1))
+    again = optim.AdamW(ps)
+    again.load_state_dict(new.state_dict())
+    assert all(torch.equal(again.state[p][n], new.state[p][n]) for p in ps for n in ("exp_avg", "exp_avg_sq"))

@@ -582,3 +582,24 @@ def test_a_torch_state_gets_a_shadow(cuda):
         for p, q in zip(b.parameters(), before):
             want = 0.9 * q.double() + 0.1 * p.detach().double()
             assert ((new.ema_of(p).double() - want).abs() <= 4 * 2.0 ** -24 * (p.detach().abs() + q.abs())).all()
+
+
+
+def test_torch_states_in_16_bits_load(cuda):
+    """States that torch keeps in the parameter's 16 bits, biases' among them, are taken on in float32."""
+    a, b = params_of(cuda, torch.bfloat16), params_of(cuda, torch.bfloat16)
+    old = torch.optim.AdamW(a.parameters(), lr=1e-2)
+    backward(a, 0)
+    old.step()
+    b.load_state_dict(a.state_dict())
+    new = optim.AdamW(b.parameters(), lr=1e-2)
+    new.load_state_dict(old.state_dict())
+    backward(b, 1)
+    want = []
+    for p, q in zip(b.parameters(), a.parameters()):
+        st = old.state[q]
+        want.append(adamw64(np64(p), np64(p.grad), np64(st["exp_avg"]), np64(st["exp_avg_sq"]), 2, 1e-2, 0.9, 0.999, 1e-8, 1e-2)[0])
+    new.step()
+    for p, x in zip(b.parameters(), want):
+        # half a step of bf16; m, v, the update and the sum some roundings of float32 (the update is below 1)
+        assert (np.abs(np64(p) - x) <= 2.0 ** -8 * 1.01 * np.abs(x) + 32 * 2.0 ** -24 * (1 + np.abs(x))).all()
