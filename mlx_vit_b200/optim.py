@@ -206,7 +206,7 @@ class AdamW(torch.optim.Optimizer):
         """As torch's, but the states are not cast to the parameters' dtypes.  The states of a
         ``torch.optim.AdamW`` can be loaded into one of 32 bits (in float32, whatever they were), unless
         its groups ask for another rule than this one's (``maximize``, ``amsgrad``, decay that is not
-        decoupled)."""
+        decoupled).  A capturable group takes states of one step number only."""
         for g in state_dict["param_groups"]:
             for name in ("maximize", "amsgrad"):
                 _need(not g.get(name), f"the loaded states are of an optimizer with {name}, which this one has not")
@@ -217,6 +217,10 @@ class AdamW(torch.optim.Optimizer):
             held = state_dict["state"].get(i)
             _need(not held or ("exp_avg_exp" in held) == (self.state_bits == 8),
                   f"the loaded states are not those of an optimizer with state_bits={self.state_bits}")
+        for g in state_dict["param_groups"] if self.capturable else ():
+            steps = {int(state_dict["state"][i]["step"]) for i in g["params"] if "step" in state_dict["state"].get(i, ())}
+            _need(len(steps) <= 1 or "step" in g, "the parameters of a capturable group have one step number, those loaded "
+                  f"have {len(steps)}: {sorted(steps)}")
         super().load_state_dict(state_dict)
         for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
             if i in state_dict["state"]:
@@ -229,7 +233,7 @@ class AdamW(torch.optim.Optimizer):
             if self.capturable:
                 steps = [st.pop("step") for st in held if "step" in st]
                 if "step" not in group and steps:
-                    group["step"] = max(steps)
+                    group["step"] = steps[0]
             elif "step" in group:
                 n = int(group.pop("step"))
                 group["lr"] = float(group["lr"])

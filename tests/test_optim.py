@@ -1,4 +1,5 @@
 """CPU: the optimizer's argument checks and its 8-bit state format (restated)."""
+import copy
 import ctypes
 
 import numpy as np
@@ -155,3 +156,26 @@ def test_loaded_states_are_float32(dtype):
     again = optim.AdamW(ps)
     again.load_state_dict(new.state_dict())
     assert all(torch.equal(again.state[p][n], new.state[p][n]) for p in ps for n in ("exp_avg", "exp_avg_sq"))
+
+
+def test_capturable_refuses_states_of_several_steps():
+    """A capturable group has one step number: parameters that have taken 1 and 2 steps would be corrected by one."""
+    a, b = (torch.nn.Parameter(torch.randn(6)) for _ in range(2))
+    old = torch.optim.AdamW([a, b])
+    a.grad = torch.ones_like(a)
+    old.step()
+    b.grad = torch.ones_like(b)
+    old.step()
+    new = optim.AdamW([a, b], capturable=True)
+    with pytest.raises(ValueError, match="step"):
+        new.load_state_dict(old.state_dict())
+    assert not new.state
+    plain = optim.AdamW([a, b])
+    plain.load_state_dict(old.state_dict())
+    assert [plain.state[p]["step"] for p in (a, b)] == [2, 1]
+    apart = optim.AdamW([dict(params=[a]), dict(params=[b])], capturable=True)
+    states = old.state_dict()
+    g = states["param_groups"][0]
+    states["param_groups"] = [dict(g, params=[0]), dict(g, params=[1])]
+    apart.load_state_dict(states)
+    assert [int(g["step"]) for g in apart.param_groups] == [2, 1]
