@@ -61,6 +61,11 @@ def _need(ok, msg):
         raise ValueError(msg)
 
 
+def _same_order(p, stride):
+    """Whether a dense tensor of p's shape with these strides lies in memory as p does."""
+    return all(a == b for a, b, n in zip(p.stride(), stride, p.shape) if n > 1)
+
+
 def grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     """The 2-norm of all gradients together, a float32 scalar on their device (sums in 64 bits)."""
     return _lib.tensors().grad_norm(list(grads))
@@ -130,6 +135,7 @@ class AdamW(torch.optim.Optimizer):
         """The state of a parameter that has none, and the shadow of one whose loaded state has none."""
         st = self.state[p]
         if not st:
+            st["stride"] = tuple(p.stride())  # the order in memory that the states lie in
             if not self.capturable:
                 st["step"] = 0
             for name in ("exp_avg", "exp_avg_sq"):
@@ -206,17 +212,21 @@ class AdamW(torch.optim.Optimizer):
         """As torch's, but the states are not cast to the parameters' dtypes.  The states of a
         ``torch.optim.AdamW`` can be loaded into one of 32 bits (in float32, whatever they were), unless
         its groups ask for another rule than this one's (``maximize``, ``amsgrad``, decay that is not
-        decoupled).  A capturable group takes states of one step number only."""
+        decoupled).  A capturable group takes states of one step number only.  States lie in their
+        parameter's order in memory: float32 ones are reordered for a parameter that lies otherwise,
+        8-bit ones refused."""
         for g in state_dict["param_groups"]:
             for name in ("maximize", "amsgrad"):
                 _need(not g.get(name), f"the loaded states are of an optimizer with {name}, which this one has not")
             _need(g.get("decoupled_weight_decay", True) or not g.get("weight_decay"),
                   "the loaded states are of an optimizer whose weight decay is not decoupled")
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        for i in ids:
+        for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
             held = state_dict["state"].get(i)
             _need(not held or ("exp_avg_exp" in held) == (self.state_bits == 8),
                   f"the loaded states are not those of an optimizer with state_bits={self.state_bits}")
+            _need(self.state_bits == 32 or not held or _same_order(p, held.get("stride", p.stride())),
+                  "8-bit states cannot be loaded into a parameter that lies otherwise in memory than theirs")
         for g in state_dict["param_groups"] if self.capturable else ():
             steps = {int(state_dict["state"][i]["step"]) for i in g["params"] if "step" in state_dict["state"].get(i, ())}
             _need(len(steps) <= 1 or "step" in g, "the parameters of a capturable group have one step number, those loaded "
@@ -224,7 +234,10 @@ class AdamW(torch.optim.Optimizer):
         super().load_state_dict(state_dict)
         for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
             if i in state_dict["state"]:
-                self.state[p] = {k: self._own(k, v, p) for k, v in state_dict["state"][i].items()}
+                held = state_dict["state"][i]
+                self.state[p] = {k: self._own(k, v, p, held.get("stride", p.stride())) for k, v in held.items()}
+                if held:
+                    self.state[p]["stride"] = tuple(p.stride())
         for group in self.param_groups:
             for name, value in self.defaults.items():
                 group.setdefault(name, value)
@@ -240,9 +253,9 @@ class AdamW(torch.optim.Optimizer):
                 for st in held:
                     st["step"] = n
 
-    def _own(self, name, v, p):
-        """A loaded state entry as this optimizer holds it: tensors flat, in the parameter's order in memory,
-        codes and exponents as they are, others in float32."""
+    def _own(self, name, v, p, stride):
+        """A loaded state entry as this optimizer holds it: tensors flat, in the parameter's order in memory
+        (``stride``: the order of those that came flat), codes and exponents as they are, others in float32."""
         if name == "step":
             return int(v)
         if not isinstance(v, torch.Tensor):
@@ -251,4 +264,6 @@ class AdamW(torch.optim.Optimizer):
             return v.to(p.device, copy=True)
         if v.dim() != 1 and v.shape == p.shape:
             return torch.empty_like(p, dtype=torch.float32).copy_(v).as_strided((p.numel(),), (1,))
+        if v.shape == (p.numel(),) and not _same_order(p, stride):
+            return self._own(name, v.as_strided(p.shape, stride), p, stride)
         return v.to(p.device, torch.float32, copy=True)

@@ -179,3 +179,44 @@ def test_capturable_refuses_states_of_several_steps():
     states["param_groups"] = [dict(g, params=[0]), dict(g, params=[1])]
     apart.load_state_dict(states)
     assert [int(g["step"]) for g in apart.param_groups] == [2, 1]
+
+
+@pytest.mark.parametrize("swap", [False, True])
+def test_states_follow_the_parameter_s_layout(swap):
+    """States lie in their parameter's order in memory: loaded into a parameter laid out otherwise, float32 ones are
+    reordered and 8-bit ones, whose blocks are of that order, refused."""
+    a, b = (torch.nn.Parameter(torch.randn(2, 3, 4, 5).to(memory_format=f))
+            for f in (torch.contiguous_format, torch.channels_last)[::-1 if swap else 1])
+    g = torch.randn(2, 3, 4, 5)
+    old = torch.optim.AdamW([a])
+    a.grad = g.clone()
+    old.step()
+    one, two, same = optim.AdamW([a], ema_decay=0.5), optim.AdamW([b], ema_decay=0.5), optim.AdamW([a], ema_decay=0.5)
+    one.load_state_dict(old.state_dict())
+    one._init_state(a)
+    states = copy.deepcopy(one.state_dict())
+    two.load_state_dict(states)
+    same.load_state_dict(states)
+    for name, want in (("exp_avg", old.state[a]["exp_avg"]), ("exp_avg_sq", old.state[a]["exp_avg_sq"]), ("ema", a.detach())):
+        for o, p in ((one, a), (two, b), (same, a)):
+            held = o.state[p][name]
+            assert held.shape == (120,) and torch.equal(held.as_strided(p.shape, p.stride()), want)
+    assert torch.equal(two.ema_of(b), a.detach())
+    for st in states["state"].values():  # states from before the layout was kept: the parameter's own
+        del st["stride"]
+    two.load_state_dict(states)
+    assert torch.equal(two.state[b]["exp_avg"], one.state[a]["exp_avg"])
+    codes = optim.AdamW([a], state_bits=8)
+    codes._init_state(a)
+    optim.AdamW([a], state_bits=8).load_state_dict(codes.state_dict())
+    with pytest.raises(ValueError, match="memory"):
+        optim.AdamW([b], state_bits=8).load_state_dict(codes.state_dict())
+
+
+def test_layouts_that_differ_in_name_only():
+    """Strides of dimensions of one element say nothing."""
+    a = torch.nn.Parameter(torch.randn(4, 1, 3))
+    b = torch.nn.Parameter(a.detach().as_strided((4, 1, 3), (3, 7, 1)))
+    codes = optim.AdamW([a], state_bits=8)
+    codes._init_state(a)
+    optim.AdamW([b], state_bits=8).load_state_dict(codes.state_dict())
