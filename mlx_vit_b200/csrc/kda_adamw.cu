@@ -707,6 +707,7 @@ int kda_adamw_step(const KdaAdamW *a, const KdaAdamWTensor *x, int64_t count, in
       !(a->max_grad_norm >= 0) || !(a->ema_decay >= 0 && a->ema_decay <= 1) || (!step_dev && a->step < 1) ||
       !isfinite(a->lr) || !isfinite(a->weight_decay) || (eight && a->eps < 1e-30))
     return KDA_ERR_INVALID_ARG;
+  if (!multiple(step_dev, 8) || !multiple(lr_dev, 4) || !multiple(grad_norm, 4)) return KDA_ERR_MISALIGNED;
   int s = check_tensors(x, count);
   if (s) return s;
   for (int64_t i = 0; i < count; ++i) {

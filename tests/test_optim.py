@@ -220,3 +220,17 @@ def test_layouts_that_differ_in_name_only():
     codes = optim.AdamW([a], state_bits=8)
     codes._init_state(a)
     optim.AdamW([b], state_bits=8).load_state_dict(codes.state_dict())
+
+
+def test_c_entries_refuse_misaligned_scalars():
+    a = 1 << 20
+    row = (a, a, a, a, 0, 0, 0, 16, _lib.KDA_F32)
+    L = _lib.lib()
+
+    def status(step=None, lr=None, norm=None):
+        args = _lib.KdaAdamW(lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, max_grad_norm=1.0, step=1, state_bits=32)
+        return _lib.STATUS[L.kda_adamw_step(ctypes.byref(args), (ctypes.c_int64 * 9)(*row), 1, step, lr, norm, a, 1 << 20, None)]
+
+    assert status(step=a + 4) == "KDA_ERR_MISALIGNED"
+    assert status(lr=a + 2) == "KDA_ERR_MISALIGNED"
+    assert status(norm=a + 2) == "KDA_ERR_MISALIGNED"
