@@ -312,8 +312,9 @@ typedef struct KdaAdamW {
  * device counter, advanced by the call before it is used) and lr_dev (a device float) replace step
  * and lr.  grad_norm (device float, may be NULL) receives ||g|| over all tensors before
  * clipping.  The three need their types' alignment (KDA_ERR_MISALIGNED).  The workspace
- * (kda_adamw_workspace_bytes) is needed with clipping, grad_norm, step_dev or lr_dev.  Results do
- * not depend on the order in which blocks run.
+ * (kda_adamw_workspace_bytes) is needed with clipping, grad_norm, step_dev or lr_dev, but not with
+ * count 0, where step_dev is advanced and grad_norm is 0.  Results do not depend on the order in
+ * which blocks run.
  * Counterpart: the trainers' AdamW, gradient clipping and ModelEMA (train_mlx_k400.py:176-222,
  * :379-408). */
 KDA_API size_t kda_adamw_workspace_bytes(int64_t count);

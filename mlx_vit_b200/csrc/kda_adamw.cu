@@ -539,14 +539,14 @@ __global__ void __launch_bounds__(kThreads) prep_kernel(Prep a, const double *pa
   if (threadIdx.x) return;
   const double n = a.norm_given ? (double)*norm : sqrt(s);
   if (norm && !a.norm_given) *norm = (float)n;
+  int64_t step = a.host_step;
+  if (a.step) *a.step = step = *a.step + 1;
   if (!dyn) return;
   double coef = 1;
   if (a.max_norm > 0) {
     coef = a.max_norm / (n + 1e-6);
     if (coef > 1) coef = 1;  // a NaN stays one
   }
-  int64_t step = a.host_step;
-  if (a.step) *a.step = step = *a.step + 1;
   const double lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
   dyn->coef = (float)coef;
   dyn->c1 = (float)(a.bias ? lr / (1 - pow(a.b1, (double)step)) : lr);
@@ -729,11 +729,12 @@ int kda_adamw_step(const KdaAdamW *a, const KdaAdamWTensor *x, int64_t count, in
   double *partial = nullptr;
   int parts = 0;
   if (dynamic || grad_norm) {
-    const bool sum = (clip || grad_norm) && !given;
+    const bool sum = (clip || grad_norm) && !given && count;
     const int64_t most = sum ? max_parts(count, sms) : 0;
-    if (!ws || !multiple(ws, 16) || ws_bytes < kDynBytes + (size_t)most * sizeof(double)) return KDA_ERR_WORKSPACE;
-    dyn = dynamic ? static_cast<Dyn *>(ws) : nullptr;
-    partial = reinterpret_cast<double *>(static_cast<char *>(ws) + kDynBytes);
+    // without tensors the step's number and the norm alone are written, and no workspace is used
+    if (count && (!ws || !multiple(ws, 16) || ws_bytes < kDynBytes + (size_t)most * sizeof(double))) return KDA_ERR_WORKSPACE;
+    dyn = dynamic && count ? static_cast<Dyn *>(ws) : nullptr;
+    partial = count ? reinterpret_cast<double *>(static_cast<char *>(ws) + kDynBytes) : nullptr;
     if (sum) {
       s = count <= kCapSmall ? launch_squares<kCapSmall>(x, count, partial, (int)most, parts, sms, st)
                              : launch_squares<kCap>(x, count, partial, (int)most, parts, sms, st);
@@ -767,8 +768,8 @@ int kda_grad_norm(const KdaAdamWTensor *x, int64_t count, float *norm, void *ws,
   const int sms = sm_count();
   if (!sms) return KDA_ERR_CUDA;
   const int64_t most = max_parts(count, sms);
-  if (!ws || !multiple(ws, 16) || ws_bytes < kDynBytes + (size_t)most * sizeof(double)) return KDA_ERR_WORKSPACE;
-  double *partial = reinterpret_cast<double *>(static_cast<char *>(ws) + kDynBytes);
+  if (count && (!ws || !multiple(ws, 16) || ws_bytes < kDynBytes + (size_t)most * sizeof(double))) return KDA_ERR_WORKSPACE;
+  double *partial = count ? reinterpret_cast<double *>(static_cast<char *>(ws) + kDynBytes) : nullptr;
   cudaStream_t st = (cudaStream_t)stream;
   int parts = 0;
   s = count <= kCapSmall ? launch_squares<kCapSmall>(x, count, partial, (int)most, parts, sms, st)

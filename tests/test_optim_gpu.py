@@ -1,12 +1,13 @@
 """GPU: the AdamW step against its formulas in 64 bits and, for the 8-bit states, code by code
 against a restatement of the format."""
 import copy
+import ctypes
 
 import numpy as np
 import pytest
 import torch
 
-from mlx_vit_b200 import optim
+from mlx_vit_b200 import _lib, optim
 from optim_testutil import BLOCK, adamw64, decode, encode, moments32, random_bits
 
 pytestmark = pytest.mark.gpu
@@ -603,3 +604,20 @@ def test_torch_states_in_16_bits_load(cuda):
     for p, x in zip(b.parameters(), want):
         # half a step of bf16; m, v, the update and the sum some roundings of float32 (the update is below 1)
         assert (np.abs(np64(p) - x) <= 2.0 ** -8 * 1.01 * np.abs(x) + 32 * 2.0 ** -24 * (1 + np.abs(x))).all()
+
+
+def test_c_calls_of_no_tensors(cuda):
+    """The size query asks for no workspace and the calls take none: the device's step number is advanced, and the
+    norm of nothing is zero."""
+    L = _lib.lib()
+    nws = L.kda_adamw_workspace_bytes(0)
+    assert nws == 0
+    step, norm = torch.full((), 4, dtype=torch.int64, device=cuda), torch.full((2,), 7.0, device=cuda)
+    a = _lib.KdaAdamW(lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, max_grad_norm=1.0, state_bits=32)
+    s = torch.cuda.current_stream().cuda_stream
+    _lib.check(L.kda_adamw_step(ctypes.byref(a), None, 0, step.data_ptr(), None, norm.data_ptr(), None, nws, s), "step")
+    _lib.check(L.kda_grad_norm(None, 0, norm[1:].data_ptr(), None, nws, s), "norm")
+    assert int(step) == 5 and norm.tolist() == [0.0, 0.0]
+    a.max_grad_norm = 0.0
+    _lib.check(L.kda_adamw_step(ctypes.byref(a), None, 0, step.data_ptr(), None, None, None, 0, s), "step")
+    assert int(step) == 6
