@@ -78,10 +78,10 @@ PyObject *guarded(F f) {
   return nullptr;
 }
 
-// The KdaAdamWTensor array of a step's lists, after their checks, and their device.  The versions of
-// what the step writes are advanced, as torch's own in-place operations do.
+// The KdaAdamWTensor array of a step's lists, after their checks, their device, and the tensors that the
+// step writes.
 std::vector<KdaAdamWTensor> adamw_table(PyObject *po, PyObject *go, PyObject *mo, PyObject *vo, PyObject *eo, int &bits,
-                                        at::Device &dev) {
+                                        at::Device &dev, std::vector<const at::Tensor *> &bump) {
   const Items p(po, "params"), g(go, "grads"), m(mo, "exp_avgs"), v(vo, "exp_avg_sqs");
   const bool ema = eo != Py_None;
   const Items e(ema ? eo : po, "emas");
@@ -93,8 +93,7 @@ std::vector<KdaAdamWTensor> adamw_table(PyObject *po, PyObject *go, PyObject *mo
   std::vector<KdaAdamWTensor> rows(p.n);
   std::vector<const void *> written;
   written.reserve(4 * p.n);
-  std::vector<const at::Tensor *> bump;
-  bump.reserve(4 * p.n);
+  bump.reserve(4 * p.n + 1);
   for (Py_ssize_t i = 0; i < p.n; ++i) {
     const at::Tensor &pt = tensor(p.p[i], "params"), &gt = tensor(g.p[i], "grads");
     need(pt.device() == dev && gt.device() == dev,
@@ -144,8 +143,6 @@ std::vector<KdaAdamWTensor> adamw_table(PyObject *po, PyObject *go, PyObject *mo
   }
   std::sort(written.begin(), written.end());
   need(std::adjacent_find(written.begin(), written.end()) == written.end(), "the same tensor is passed twice");
-  for (const at::Tensor *t : bump)
-    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
   return rows;
 }
 
@@ -214,7 +211,8 @@ PyObject *adamw_step(PyObject *, PyObject *args) {
     need(a.ema_decay >= 0 && a.ema_decay <= 1, "ema_decay must lie in [0, 1]");
     need(no == Py_None || a.max_grad_norm > 0, "norm is used with max_grad_norm only");
     at::Device dev(at::kCPU);
-    const std::vector<KdaAdamWTensor> rows = adamw_table(po, go, mo, vo, eo, a.state_bits, dev);
+    std::vector<const at::Tensor *> written;
+    const std::vector<KdaAdamWTensor> rows = adamw_table(po, go, mo, vo, eo, a.state_bits, dev, written);
     need(a.state_bits == 32 || a.eps >= 1e-30, "8-bit states need an eps of at least 1e-30");
     const at::Tensor *step = scalar(so, "step", at::kLong, dev), *lr = scalar(lo, "lr", at::kFloat, dev);
     const at::Tensor *given = no == Py_None ? nullptr : scalar(no, "norm", at::kFloat, dev);
@@ -243,7 +241,10 @@ PyObject *adamw_step(PyObject *, PyObject *args) {
                         lr ? lr->data_ptr<float>() : nullptr, clip ? norm.data_ptr<float>() : nullptr,
                         ws.defined() ? ws.data_ptr() : nullptr, ws.defined() ? (size_t)ws.numel() : 0, st),
          "kda_adamw_step");
-    if (step) step->unsafeGetTensorImpl()->bump_version();
+    // the versions of what was written advance, as under torch's own in-place operations
+    if (step) written.push_back(step);
+    for (const at::Tensor *t : written)
+      if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
     if (clip) return THPVariable_Wrap(norm);
     Py_RETURN_NONE;
   });

@@ -621,3 +621,21 @@ def test_c_calls_of_no_tensors(cuda):
     a.max_grad_norm = 0.0
     _lib.check(L.kda_adamw_step(ctypes.byref(a), None, 0, step.data_ptr(), None, None, None, 0, s), "step")
     assert int(step) == 6
+
+
+def test_a_refused_step_leaves_versions_alone(cuda):
+    """A call that writes nothing does not tell autograd that something changed: a living graph's backward runs."""
+    p = torch.randn(64, device=cuda, requires_grad=True)
+    g, m, v, e = (torch.zeros(64, device=cuda) for _ in range(4))
+    y = (p * p).sum()
+    was = [t._version for t in (p, m, v, e)]
+    kw = dict(emas=[e], ema_decay=0.9)
+    for bad in (dict(step=0, lr=1e-3), dict(step=1, lr=float("inf")), dict(step=torch.ones((), device=cuda), lr=1e-3),
+                dict(step=1, lr=1e-3, max_grad_norm=1.0, norm=m[:2]), dict(step=1, lr=m), dict(step="1", lr=1e-3)):
+        with pytest.raises((ValueError, RuntimeError, TypeError)):
+            optim.adamw_step([p], [g], [m], [v], **bad, **kw)
+    assert [t._version for t in (p, m, v, e)] == was
+    y.backward()
+    assert torch.equal(p.grad, 2 * p.detach())
+    optim.adamw_step([p], [g], [m], [v], step=1, lr=1e-3, **kw)
+    assert all(t._version > n for t, n in zip((p, m, v, e), was))
