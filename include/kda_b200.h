@@ -51,7 +51,7 @@
 extern "C" {
 #endif
 
-#define KDA_ABI_VERSION 7
+#define KDA_ABI_VERSION 8
 
 enum kda_dtype { KDA_F32 = 0, KDA_BF16 = 1, KDA_F16 = 2 };
 
@@ -300,7 +300,8 @@ typedef struct KdaAdamW {
   int32_t use_ema;
   int32_t norm_given;     /* with clipping: grad_norm holds ||g|| already (kda_grad_norm), read instead
                              of computed: how several calls clip by one norm */
-  int32_t reserved;
+  uint32_t first_tensor;  /* the first tensor's number in the step, where several calls make one: the 8-bit
+                             states are rounded by bits of (seed, step, tensor's number, element) */
 } KdaAdamW;
 
 /* One AdamW step over `count` tensors (a host array, read before the call returns):

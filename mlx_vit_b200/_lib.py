@@ -12,7 +12,7 @@ import threading
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libkda_b200.so")
 
-KDA_ABI_VERSION = 7
+KDA_ABI_VERSION = 8
 KDA_F32, KDA_BF16, KDA_F16 = 0, 1, 2
 KDA_ACT_NONE, KDA_ACT_RELU, KDA_ACT_SILU, KDA_ACT_GELU, KDA_ACT_GELU_TANH = range(5)
 KDA_LINEAR_FWD, KDA_LINEAR_DGRAD, KDA_LINEAR_WGRAD, KDA_LINEAR_ACT_GRAD = range(4)
@@ -64,7 +64,7 @@ class KdaAdamW(ctypes.Structure):
                 ("max_grad_norm", ctypes.c_double), ("ema_decay", ctypes.c_double),
                 ("step", ctypes.c_int64), ("seed", ctypes.c_uint32), ("state_bits", ctypes.c_int32),
                 ("bias_correction", ctypes.c_int32), ("use_ema", ctypes.c_int32),
-                ("norm_given", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+                ("norm_given", ctypes.c_int32), ("first_tensor", ctypes.c_uint32)]
 
 
 class KdaError(RuntimeError):

@@ -602,13 +602,13 @@ static int launched() {
 constexpr size_t kDynBytes = 256;
 
 template <int CAP, typename F>
-static int for_tables(const KdaAdamWTensor *x, int64_t count, bool grads_only, bool eight, F launch) {
+static int for_tables(const KdaAdamWTensor *x, int64_t count, uint32_t first, bool grads_only, bool eight, F launch) {
   static thread_local Table<CAP> t;
   int64_t at = 0;
   while (at < count) {
     t.count = 0;
     t.chunks = 0;
-    t.index0 = (uint32_t)at;
+    t.index0 = first + (uint32_t)at;
     uint64_t chunks = 0;
     for (; at < count && t.count < CAP; ++at) {
       const KdaAdamWTensor &a = x[at];
@@ -645,7 +645,7 @@ static int grid_for(uint32_t chunks, int sms, int per_sm) {
 template <int CAP>
 static int launch_squares(const KdaAdamWTensor *x, int64_t count, double *partial, int most, int &parts, int sms,
                           cudaStream_t st) {
-  return for_tables<CAP>(x, count, true, false, [&](const Table<CAP> &t) {
+  return for_tables<CAP>(x, count, 0, true, false, [&](const Table<CAP> &t) {
     const int grid = grid_for(t.chunks, sms, kCtasPerSmRead);
     if (parts + grid > most) return (int)KDA_ERR_WORKSPACE;
     squares_kernel<CAP><<<grid, kThreads, 0, st>>>(t, partial + parts);
@@ -654,20 +654,21 @@ static int launch_squares(const KdaAdamWTensor *x, int64_t count, double *partia
   });
 }
 template <bool EIGHT, bool EMA, int CAP>
-static int launch_update(const KdaAdamWTensor *x, int64_t count, const Hyper &h, const Dyn *dyn, int sms, cudaStream_t st) {
-  return for_tables<CAP>(x, count, false, EIGHT, [&](const Table<CAP> &t) {
+static int launch_update(const KdaAdamWTensor *x, int64_t count, uint32_t first, const Hyper &h, const Dyn *dyn, int sms,
+                         cudaStream_t st) {
+  return for_tables<CAP>(x, count, first, false, EIGHT, [&](const Table<CAP> &t) {
     adamw_kernel<EIGHT, EMA, CAP><<<grid_for(t.chunks, sms, kCtasPerSm), kThreads, 0, st>>>(t, h, dyn);
     return launched();
   });
 }
 template <int CAP>
-static int launch_update(const KdaAdamWTensor *x, int64_t count, const Hyper &h, const Dyn *dyn, bool eight, bool ema,
-                         int sms, cudaStream_t st) {
+static int launch_update(const KdaAdamWTensor *x, int64_t count, uint32_t first, const Hyper &h, const Dyn *dyn, bool eight,
+                         bool ema, int sms, cudaStream_t st) {
   if (eight)
-    return ema ? launch_update<true, true, CAP>(x, count, h, dyn, sms, st)
-               : launch_update<true, false, CAP>(x, count, h, dyn, sms, st);
-  return ema ? launch_update<false, true, CAP>(x, count, h, dyn, sms, st)
-             : launch_update<false, false, CAP>(x, count, h, dyn, sms, st);
+    return ema ? launch_update<true, true, CAP>(x, count, first, h, dyn, sms, st)
+               : launch_update<true, false, CAP>(x, count, first, h, dyn, sms, st);
+  return ema ? launch_update<false, true, CAP>(x, count, first, h, dyn, sms, st)
+             : launch_update<false, false, CAP>(x, count, first, h, dyn, sms, st);
 }
 
 static int64_t max_parts(int64_t count, int sms) {
@@ -757,8 +758,8 @@ int kda_adamw_step(const KdaAdamW *a, const KdaAdamWTensor *x, int64_t count, in
     h.decay = (float)(1 - a->lr * a->weight_decay);
     h.key = mix(a->seed + (uint32_t)a->step * 0x9E3779B9u);
   }
-  return count <= kCapSmall ? launch_update<kCapSmall>(x, count, h, dyn, eight, a->use_ema != 0, sms, st)
-                            : launch_update<kCap>(x, count, h, dyn, eight, a->use_ema != 0, sms, st);
+  return count <= kCapSmall ? launch_update<kCapSmall>(x, count, a->first_tensor, h, dyn, eight, a->use_ema != 0, sms, st)
+                            : launch_update<kCap>(x, count, a->first_tensor, h, dyn, eight, a->use_ema != 0, sms, st);
 }
 
 int kda_grad_norm(const KdaAdamWTensor *x, int64_t count, float *norm, void *ws, size_t ws_bytes, void *stream) {

@@ -195,15 +195,15 @@ const at::Tensor *scalar(PyObject *o, const char *name, at::ScalarType type, con
 }
 
 // adamw_step(params, grads, exp_avgs, exp_avg_sqs, emas or None, step, lr, beta1, beta2, eps, weight_decay,
-//            bias_correction, max_grad_norm (0: none), ema_decay, seed, norm or None) -> norm or None.
+//            bias_correction, max_grad_norm (0: none), ema_decay, seed, norm or None, first_tensor) -> norm or None.
 // ValueError for operands that the kernel does not take.
 PyObject *adamw_step(PyObject *, PyObject *args) {
   PyObject *po, *go, *mo, *vo, *eo, *so, *lo, *no;
   KdaAdamW a = {};
   int bias;
-  unsigned int seed;
-  if (!PyArg_ParseTuple(args, "OOOOOOOddddpddIO", &po, &go, &mo, &vo, &eo, &so, &lo, &a.beta1, &a.beta2, &a.eps, &a.weight_decay,
-                        &bias, &a.max_grad_norm, &a.ema_decay, &seed, &no))
+  unsigned int seed, first;
+  if (!PyArg_ParseTuple(args, "OOOOOOOddddpddIOI", &po, &go, &mo, &vo, &eo, &so, &lo, &a.beta1, &a.beta2, &a.eps, &a.weight_decay,
+                        &bias, &a.max_grad_norm, &a.ema_decay, &seed, &no, &first))
     return nullptr;
   return guarded([&]() -> PyObject * {
     need(a.beta1 >= 0 && a.beta1 < 1 && a.beta2 >= 0 && a.beta2 < 1, "betas must lie in [0, 1)");
@@ -227,6 +227,7 @@ PyObject *adamw_step(PyObject *, PyObject *args) {
       if (PyErr_Occurred()) return nullptr;
     }
     a.seed = seed;
+    a.first_tensor = first;
     a.bias_correction = bias;
     a.use_ema = eo != Py_None;
     a.norm_given = given != nullptr;

@@ -18,9 +18,9 @@ With ``state_bits=8`` m and v are held as one byte an element plus one exponent 
 magnitude plus one, and a code's magnitude 8 k + f stands for (1 + f / 8) 2^(k - L + e - 127),
 zero for zero; m has a sign in bit 7 and L = 15, v has L = 31.  Values are rounded to their three
 bits of mantissa stochastically (to nearest, v could never decay by beta2 = 0.999 a step), by bits
-that a hash of (seed, step, tensor, element) gives: the same call gives the same states.  Magnitudes
-below the least code become it or zero for m, unbiased, and the least code for v.  A block that
-holds a value that is not finite reads back as NaN.
+that a hash of (seed, step, the tensor's number in the step, element) gives: the same call gives the
+same states.  Magnitudes below the least code become it or zero for m, unbiased, and the least code
+for v.  A block that holds a value that is not finite reads back as NaN.
 """
 from __future__ import annotations
 
@@ -76,7 +76,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
                step: Union[int, torch.Tensor], lr: Union[float, torch.Tensor], betas=(0.9, 0.999), eps: float = 1e-8,
                weight_decay: float = 1e-2, bias_correction: bool = True, max_grad_norm: Optional[float] = None,
                emas: Optional[Sequence[torch.Tensor]] = None, ema_decay: Optional[float] = None, seed: int = 0,
-               norm: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+               norm: Optional[torch.Tensor] = None, first_tensor: int = 0) -> Optional[torch.Tensor]:
     """One AdamW step over lists of CUDA tensors, in place.
 
     ``params`` and ``grads`` are float32, bfloat16 or float16, dense in memory and each pair laid
@@ -87,13 +87,16 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     With ``max_grad_norm`` the gradients are scaled as they are read (``grads`` keep their values)
     by their global norm, or by ``norm``, a float32 CUDA scalar, where that is given.  ``emas``
     (float32) follow the parameters with ``ema_decay``.  Tensors must not overlap one another.
+    ``first_tensor`` numbers the lists' first tensor where several calls make one step, so that 8-bit
+    states in different calls are rounded by different bits.
     Returns the gradients' norm (float32 scalar) with ``max_grad_norm``, else None.
     """
     _need((emas is None) == (ema_decay is None), "emas and ema_decay go together")
     _need(max_grad_norm is None or max_grad_norm > 0.0, "max_grad_norm must be positive")
+    _need(0 <= first_tensor < 1 << 31, "first_tensor counts from 0")
     return _lib.tensors().adamw_step(list(params), list(grads), list(exp_avgs), list(exp_avg_sqs),
                                      None if emas is None else list(emas), step, lr, betas[0], betas[1], eps, weight_decay,
-                                     bias_correction, max_grad_norm or 0.0, ema_decay or 0.0, seed & 0xFFFFFFFF, norm)
+                                     bias_correction, max_grad_norm or 0.0, ema_decay or 0.0, seed & 0xFFFFFFFF, norm, first_tensor)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -194,6 +197,7 @@ class AdamW(torch.optim.Optimizer):
         norm = None
         if self.max_grad_norm is not None and len(calls) > 1:
             norm = grad_norm([g for c in calls for g in c[2]])
+        first = 0  # tensors of the calls before
         for group, ps, gs, n in calls:
             out = adamw_step(ps, gs, self._states(ps, "exp_avg"),
                              self._states(ps, "exp_avg_sq"), step=n,
@@ -201,8 +205,9 @@ class AdamW(torch.optim.Optimizer):
                              eps=group["eps"], weight_decay=group["weight_decay"],
                              bias_correction=group["bias_correction"], max_grad_norm=self.max_grad_norm,
                              emas=None if self.ema_decay is None else [self.state[p]["ema"] for p in ps],
-                             ema_decay=self.ema_decay, seed=self.seed, norm=norm)
+                             ema_decay=self.ema_decay, seed=self.seed, norm=norm, first_tensor=first)
             self.grad_norm = out
+            first += len(ps)
             if not self.capturable:
                 for p in ps:
                     self.state[p]["step"] = n

@@ -639,3 +639,59 @@ def test_a_refused_step_leaves_versions_alone(cuda):
     assert torch.equal(p.grad, 2 * p.detach())
     optim.adamw_step([p], [g], [m], [v], step=1, lr=1e-3, **kw)
     assert all(t._version > n for t, n in zip((p, m, v, e), was))
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_groups_round_by_bits_of_their_own(cuda, capturable):
+    """Equal tensors with equal gradients in two groups, and in two subsets of one group with step numbers of their
+    own, are rounded apart; the codes are the restated ones of the tensor's place in the whole step."""
+    torch.manual_seed(9)
+    w, grad = torch.randn(40, 50, device=cuda), torch.randn(40, 50, device=cuda)
+
+    def run(groups, late=None):
+        ps = [torch.nn.Parameter(w.clone()) for _ in range(4)]
+        o = optim.AdamW([dict(params=[ps[i] for i in g]) for g in groups], lr=1e-3, state_bits=8, seed=3, capturable=capturable)
+        for t in range(2):
+            for i, p in enumerate(ps):
+                p.grad = None if t == 0 and i == late else grad.clone()
+            o.step()
+        return ps, [o.state[p] for p in ps]
+
+    m32, v32 = moments32(grad.cpu().numpy().reshape(-1), np.zeros(2000), np.zeros(2000), 0.9, 0.999)
+
+    def first_codes(tensor):  # both states after a first step from zero
+        r = random_bits(3, 1, tensor, 2000)
+        return encode(m32, r & np.uint64(0xFFFF), 15, True), encode(v32, r >> np.uint64(16), 31, False)
+
+    ps = [torch.nn.Parameter(w.clone()) for _ in range(4)]
+    o = optim.AdamW([dict(params=ps[:1]), dict(params=ps[1:3]), dict(params=ps[3:])], lr=1e-3, state_bits=8, seed=3,
+                    capturable=capturable)
+    for p in ps:
+        p.grad = grad.clone()
+    o.step()
+    for i, p in enumerate(ps):
+        for name, (code, exp) in zip(("exp_avg", "exp_avg_sq"), first_codes(i)):
+            assert np.array_equal(o.state[p][name].cpu().numpy(), code), (i, name)
+            assert np.array_equal(o.state[p][name + "_exp"].cpu().numpy(), exp), (i, name)
+    _, one = run([[0, 1, 2, 3]])
+    _, two = run([[0, 1], [2, 3]])
+    for a, b in zip(one, two):  # how the parameters are grouped changes nothing
+        assert torch.equal(a["exp_avg"], b["exp_avg"]) and torch.equal(a["exp_avg_sq"], b["exp_avg_sq"])
+    assert all(not torch.equal(two[i]["exp_avg"], two[j]["exp_avg"]) for i in range(4) for j in range(i))
+    if not capturable:
+        _, st = run([[0, 1, 2, 3]], late=1)  # 1 is at its first step while the others are at their second
+        assert [s["step"] for s in st] == [2, 1, 2, 2]
+
+
+def test_first_tensor_of_a_call(cuda):
+    """Lists stepped in two calls with ``first_tensor`` give the codes of one call."""
+    outs = []
+    for cut in (None, 4):
+        p, g, m, v = make(cuda, "bf16", 8)
+        for part in ([slice(None)] if cut is None else [slice(0, cut), slice(cut, None)]):
+            optim.adamw_step(p[part], g[part], m[part], v[part], step=2, seed=5, first_tensor=part.start or 0, **HYP)
+        outs.append([x.clone() for x in p] + [c.clone() for c, _ in m] + [c.clone() for c, _ in v])
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    for bad in (-1, 1 << 31):
+        with pytest.raises((ValueError, OverflowError)):
+            optim.adamw_step(p, g, m, v, step=2, first_tensor=bad, **HYP)
