@@ -87,7 +87,8 @@ __device__ __forceinline__ float activate_grad(int act, float z) {
     case KDA_ACT_GELU: return gelu_grad2(both(z)).x;
     case KDA_ACT_GELU_TANH: {
       const float s = logistic(kTanhA * z * fmaf(kTanhB, z * z, 1.f));
-      return fmaf(z * s * (1.f - s), kTanhA * fmaf(3.f * kTanhB, z * z, 1.f), s);
+      // s (1 - s) is zero from |z| = 11 on, where z^2 may be infinite: cut far behind that
+      return fmaf(z * s * (1.f - s), kTanhA * fmaf(3.f * kTanhB, fminf(z * z, 1e6f), 1.f), s);
     }
     default: return 1.f;
   }

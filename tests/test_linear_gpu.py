@@ -562,3 +562,34 @@ def test_tracers_are_refused(cuda):
                 make_fx(f, tracing_mode="fake")(leaf)
         compiled = torch.compile(f, backend="eager")  # leaves the graph around the call
         assert torch.equal(compiled(x), f(x))
+
+
+@pytest.mark.parametrize("act", list(ACTIVATIONS))
+@pytest.mark.parametrize("m,n", [(9, 8), (100, 8), (100, 13)])
+def test_far_from_zero(cuda, act, m, n):
+    """Results and gradients at pre-activations up to 2^122, where z^2 and z^3 are past float32: z is a power of
+    two, exact in every form.  dz is stored in 16 bits; each product below is of powers of two."""
+    g = gen(20)
+    h = 2.0 ** -8
+    x = torch.zeros(m, 16, dtype=torch.bfloat16, device=cuda)
+    x[:, 0] = torch.exp2(torch.arange(m, device=cuda) % 9 * 7.0) * torch.where(torch.arange(m, device=cuda) % 2 == 0, 1.0, -1.0)
+    w1 = torch.zeros(n, 16, dtype=torch.bfloat16, device=cuda)
+    w1[:, 0] = torch.exp2(torch.arange(n, device=cuda) % 8 * 9.5).log2().round().exp2()
+    eye = torch.eye(n, dtype=torch.bfloat16, device=cuda)
+    z = x.double() @ w1.double().t()
+    assert z.abs().max() > 2.0 ** 100
+    s = grad64(z, act)
+    want_y, dy = act64(z, act), rnd(g, m, n, dt=torch.bfloat16)
+    dz = dy.double() * s
+    for which in ("linear_act", "mlp"):
+        a, b = x.clone().requires_grad_(), w1.clone().requires_grad_()
+        bias = torch.zeros(n, dtype=torch.bfloat16, device=cuda, requires_grad=True)
+        y = linear_act(a, b, bias, act) if which == "linear_act" else mlp(a, b, bias, eye, None, act)
+        near(y, want_y, (h + 3.1e-5) * 1.01 * want_y.abs() + 2e-9, "y")
+        dx, dw, db = torch.autograd.grad(y, (a, b, bias), dy)
+        edz = 1.01 * h * dz.abs() + 2e-5 * dy.double().abs()
+        for got, left, right, name in ((dx, dz, w1.double(), "dx"), (dw, dz.t(), x.double(), "dw")):
+            want = left @ right
+            e = edz if name == "dx" else edz.t()
+            near(got, want, e @ right.abs() + (m + n + 2) * U * (left.abs() @ right.abs()) + 1.01 * h * want.abs(), name)
+        near(db, dz.sum(0), edz.sum(0) + (m + 2) * U * dz.abs().sum(0) + 1.01 * h * dz.sum(0).abs(), "db")
