@@ -243,7 +243,8 @@ KDA_API int kda_bwd_noalloc(const KdaDesc *desc, const void *q, const void *k, c
  * (KDA_ERR_MISALIGNED), the others their element's alignment only (aligned ones are faster).
  * Sizes up to 2^30 each.
  *   kda_linear_fwd:    y [M][N] = act(x [M][K] w [N][K]^T + bias [N]) + residual [M][N];
- *                      z [M][N] (may be NULL) receives x w^T + bias, rounded, for the backward
+ *                      z [M][N] (may be NULL) receives x w^T + bias, rounded, for the backward; past the
+ *                      type's range its largest value
  *   kda_act_grad:      dz = dy act'(z) over [rows][cols] and its column sums db [cols]; with KDA_ACT_NONE
  *                      (z may be NULL) a copy, which also brings a matrix into the alignment the
  *                      others need; dz may be NULL where the sums alone are wanted

@@ -177,12 +177,19 @@ __device__ __forceinline__ void dealloc(uint32_t taddr, uint32_t cols) {
 // byte offset of 16-byte chunk c of row r in a tile of 128-byte rows with the 128-byte swizzle
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 
+// pack_z: of a pre-activation, whose value past the type's range, finite as it may be in float32, becomes the type's
+// largest: every derivative has its limit there, and 0 times infinity at the infinity itself.  A NaN stays one.
 template <typename T> struct Pair;
 template <> struct Pair<__nv_bfloat16> {
   using type = __nv_bfloat162;
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const type v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&v);
+  }
+  static __device__ __forceinline__ uint32_t pack_z(float a, float b) {
+    uint32_t u;
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(b), "f"(a));
+    return u;
   }
   static __device__ __forceinline__ float2 unpack(uint32_t u) {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
@@ -194,8 +201,19 @@ template <> struct Pair<__half> {
     const type v = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&v);
   }
+  static __device__ __forceinline__ uint32_t pack_z(float a, float b) {
+    uint32_t u;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(b), "f"(a));
+    return u;
+  }
   static __device__ __forceinline__ float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<const type *>(&u)); }
 };
+
+template <typename T>
+__device__ __forceinline__ void store_z(T *p, float v) {
+  const unsigned short u = (unsigned short)Pair<T>::pack_z(v, 0.f);
+  *p = *reinterpret_cast<const T *>(&u);
+}
 
 // A 32 x 64 tile between global memory and a warp's staging rows where no TMA map can describe the
 // matrix (a row pitch or a base that 16 bytes do not divide): coalesced 2-byte accesses.
@@ -312,7 +330,8 @@ __device__ __forceinline__ void chunk(const Args &g, uint32_t acc, uint8_t *so, 
         const int j = 32 * h + 8 * u + lane;
         if (lane < 8 && j < cols) sums[j] = s;
       }
-      *slot = make_uint4(P::pack(v[0], v[1]), P::pack(v[2], v[3]), P::pack(v[4], v[5]), P::pack(v[6], v[7]));
+      *slot = keep ? make_uint4(P::pack_z(v[0], v[1]), P::pack_z(v[2], v[3]), P::pack_z(v[4], v[5]), P::pack_z(v[6], v[7]))
+                   : make_uint4(P::pack(v[0], v[1]), P::pack(v[2], v[3]), P::pack(v[4], v[5]), P::pack(v[6], v[7]));
     }
   }
 }
@@ -600,7 +619,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
       T *z = static_cast<T *>(g.z_ptr) + row * g.ldz + col;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (j < k) z[j] = from_f<T>(v[j]);
+        if (j < k) store_z<T>(z + j, v[j]);
     }
     float x[8];
     if (g.in_kind) {
@@ -773,7 +792,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) few_rows_kernel(const FewAr
     float v = 0.f;
     for (int i = 0; i < kw; ++i) v += red[j / (8 * NB) * kw + i][row][j % (8 * NB)];
     if (a.bias) v += to_f<T>(static_cast<const T *>(a.bias)[n]);
-    if (a.z) static_cast<T *>(a.z)[row * a.ldz + n] = from_f<T>(v);
+    if (a.z) store_z<T>(static_cast<T *>(a.z) + row * a.ldz + n, v);
     v = activate(a.act, v);
     if (a.res) v += to_f<T>(static_cast<const T *>(a.res)[row * a.ldr + n]);
     static_cast<T *>(a.y)[row * a.ldy + n] = from_f<T>(v);

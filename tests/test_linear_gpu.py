@@ -593,3 +593,34 @@ def test_far_from_zero(cuda, act, m, n):
             e = edz if name == "dx" else edz.t()
             near(got, want, e @ right.abs() + (m + n + 2) * U * (left.abs() @ right.abs()) + 1.01 * h * want.abs(), name)
         near(db, dz.sum(0), edz.sum(0) + (m + 2) * U * dz.abs().sum(0) + 1.01 * h * dz.sum(0).abs(), "db")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("act", [a for a in ACTIVATIONS if a != "none"])
+@pytest.mark.parametrize("m,k", [(3, 16), (70, 16), (70, 9008)])
+def test_pre_activations_past_the_type(cuda, dtype, act, m, k):
+    """z is finite in float32 and past the 16-bit type: the derivative is 1 or 0 as at the type's largest value, in
+    the kernel for few rows, in tiles and joined from parts.  Every value below is exact."""
+    if k > 16:
+        assert _lib.lib().kda_linear_workspace_bytes(_lib.KDA_LINEAR_FWD, m, 16, k, 0) > 0
+    dt = DT[dtype]
+    x, w = torch.zeros(m, k, dtype=dt, device=cuda), torch.zeros(16, k, dtype=dt, device=cuda)
+    if dtype == "fp16":
+        x[:, 0], w[:8, 0], w[8:, 0] = 400.0, 250.0, -250.0
+    else:  # 2^127 (2 - 2^-8): above the largest bf16, which is 2^127 (2 - 2^-7), by half a step
+        x[:, :2] = 2.0 ** 64
+        w[:8, 0], w[:8, 1] = (2 - 2.0 ** -7) * 2.0 ** 63, 2.0 ** 55
+        w[8:] = -w[:8]
+    x.requires_grad_(), w.requires_grad_()
+    b = torch.zeros(16, dtype=dt, device=cuda, requires_grad=True)
+    y = linear_act(x, w, b, act)
+    assert torch.isinf(y[:, :8]).all() and (y[:, 8:] == 0).all()
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+    assert torch.equal(dx, 8 * w[:1].detach().expand(m, k))
+    assert torch.equal(dw[:8], (m * x[:1].detach()).expand(8, k)) and (dw[8:] == 0).all()
+    assert (db[:8] == m).all() and (db[8:] == 0).all()
+    w1, w2 = w.detach()[8:].clone().requires_grad_(), torch.ones(4, 8, dtype=dt, device=cuda, requires_grad=True)
+    y = mlp(x, w1, None, w2, None, act)
+    assert (y == 0).all()
+    for t in torch.autograd.grad(y, (x, w1, w2), torch.ones_like(y)):
+        assert (t == 0).all()
