@@ -77,9 +77,8 @@ __device__ __forceinline__ float activate(int act, float z) {
     default: return z;
   }
 }
-__device__ __forceinline__ float activate_grad(int act, float z) {
+__device__ __forceinline__ float activate_grad(int act, float z) {  // not ReLU's: grad_through
   switch (act) {
-    case KDA_ACT_RELU: return z > 0.f ? 1.f : 0.f;
     case KDA_ACT_SILU: {
       const float s = logistic(z);
       return s * fmaf(z, 1.f - s, 1.f);
@@ -99,9 +98,15 @@ __device__ __forceinline__ float2 activate2(int act, float2 z) {
   if (act == KDA_ACT_GELU) return gelu2(z);
   return make_float2(activate(act, z.x), activate(act, z.y));
 }
-__device__ __forceinline__ float2 activate_grad2(int act, float2 z) {
-  if (act == KDA_ACT_GELU) return gelu_grad2(z);
-  return make_float2(activate_grad(act, z.x), activate_grad(act, z.y));
+// A gradient g at an activation's result to the one at its input z: g act'(z).  ReLU's selects, as torch's:
+// behind a dead unit an infinite or NaN g is dropped, and where z is NaN it passes.
+__device__ __forceinline__ float grad_through(int act, float g, float z) {
+  if (act == KDA_ACT_RELU) return z <= 0.f ? 0.f : g;
+  return g * activate_grad(act, z);
+}
+__device__ __forceinline__ float2 grad_through2(int act, float2 g, float2 z) {
+  if (act == KDA_ACT_RELU) return make_float2(grad_through(act, g.x, z.x), grad_through(act, g.y, z.y));
+  return mul2(g, act == KDA_ACT_GELU ? gelu_grad2(z) : make_float2(activate_grad(act, z.x), activate_grad(act, z.y)));
 }
 
 }  // namespace kda

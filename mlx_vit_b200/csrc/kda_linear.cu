@@ -256,7 +256,7 @@ __device__ __forceinline__ void finish8(float (&v)[8], uint4 *slot, bool add) {
     const uint32_t w[4] = {zi.x, zi.y, zi.z, zi.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float2 d = mul2(make_float2(v[2 * j], v[2 * j + 1]), activate_grad2(ACT, P::unpack(w[j])));
+      const float2 d = grad_through2(ACT, make_float2(v[2 * j], v[2 * j + 1]), P::unpack(w[j]));
       v[2 * j] = d.x;
       v[2 * j + 1] = d.y;
     }
@@ -629,7 +629,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Args 
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      if (g.in_kind == kInActGrad) v[j] *= activate_grad(g.act, x[j]);
+      if (g.in_kind == kInActGrad) v[j] = grad_through(g.act, v[j], x[j]);
       else v[j] = activate(g.act, v[j]) + (g.in_kind == kInAdd ? x[j] : 0.f);
       if (SUMS) sum[j] += v[j];
     }
@@ -822,9 +822,9 @@ __global__ void __launch_bounds__(256) act_grad_kernel(int64_t rows, int cols, c
     if (ACT != KDA_ACT_NONE) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float2 g = activate_grad2(ACT, make_float2(y[2 * j], y[2 * j + 1]));
-        x[2 * j] *= g.x;
-        x[2 * j + 1] *= g.y;
+        const float2 d = grad_through2(ACT, make_float2(x[2 * j], x[2 * j + 1]), make_float2(y[2 * j], y[2 * j + 1]));
+        x[2 * j] = d.x;
+        x[2 * j + 1] = d.y;
       }
     }
     if (SUMS) {

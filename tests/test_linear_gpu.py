@@ -624,3 +624,41 @@ def test_pre_activations_past_the_type(cuda, dtype, act, m, k):
     assert (y == 0).all()
     for t in torch.autograd.grad(y, (x, w1, w2), torch.ones_like(y)):
         assert (t == 0).all()
+
+
+@pytest.mark.parametrize("n", [64, 75])
+def test_relu_gradient_selects(cuda, n):
+    """Behind a dead unit an infinite or NaN gradient is dropped, and a NaN's passes, as torch's ReLU does it: in the
+    activation-gradient pass and in the epilogue of the product below, whole and joined from parts."""
+    g = gen(21)
+    m, k = 70, 64
+    x, w = rnd(g, m, k, dt=torch.bfloat16), rnd(g, n, k, dt=torch.bfloat16, scale=0.1)
+    b = torch.zeros(n, dtype=torch.bfloat16, device=cuda)
+    b[5], b[6], b[7] = -1e4, 1e4, float("nan")
+    dy = rnd(g, m, n, dt=torch.bfloat16)
+    dy[3, 5], dy[4, 5] = float("inf"), float("nan")
+    for t in (x, w, b):
+        t.requires_grad_()
+    got = torch.autograd.grad(linear_act(x, w, b, "relu"), (x, b), dy)
+    clean = dy.clone()
+    clean[:, 5] = 0
+    with torch.no_grad():
+        b[7] = 1e4
+    want = torch.autograd.grad(linear_act(x, w, b, "relu"), (x, b), clean)
+    assert all(torch.isfinite(t).all() for t in want)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for out in (40, 5000):  # 5000: the sum over out is in parts
+        if out > 40:
+            plain = -(-m // 32) * n * 4
+            assert _lib.lib().kda_linear_workspace_bytes(_lib.KDA_LINEAR_DGRAD, m, out, n, 1) > plain + m * n * 4
+        w2, dy2 = rnd(g, out, n, dt=torch.bfloat16, scale=0.1), rnd(g, m, out, dt=torch.bfloat16).abs()
+        with torch.no_grad():
+            b[7] = float("nan")
+            w2[1, 5], w2[2, 5] = float("inf"), float("nan")
+        got = torch.autograd.grad(mlp(x, w, b, w2, None, "relu"), (x, w, b), dy2)
+        with torch.no_grad():
+            b[7] = 1e4
+            w2[1, 5] = w2[2, 5] = 0
+        want = torch.autograd.grad(mlp(x, w, b, w2, None, "relu"), (x, w, b), dy2)
+        assert all(torch.isfinite(t).all() for t in want)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
