@@ -662,3 +662,15 @@ def test_relu_gradient_selects(cuda, n):
         want = torch.autograd.grad(mlp(x, w, b, w2, None, "relu"), (x, w, b), dy2)
         assert all(torch.isfinite(t).all() for t in want)
         assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("act", list(ACTIVATIONS))
+@pytest.mark.parametrize("m,k,n,out", [(200, 64, 512, 2048), (131, 40, 137, 3001)])
+def test_mlp_split_hidden_gradient(cuda, dtype, act, m, k, n, out):
+    """The gradient at the hidden activation summed in parts: the join takes the activation's derivative, with the
+    bias's sums and without."""
+    sums = -(-m // 32) * n * 4
+    assert _lib.lib().kda_linear_workspace_bytes(_lib.KDA_LINEAR_DGRAD, m, out, n, 1) >= sums + 2 * m * n * 4
+    check_mlp(m, k, n, out, dtype, act, True, True, seed=22)
+    check_mlp(m, k, n, out, dtype, act, False, False, seed=23)
