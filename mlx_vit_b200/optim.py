@@ -130,10 +130,6 @@ class AdamW(torch.optim.Optimizer):
         """The shadow average of a parameter, in its shape (float32)."""
         return self.state[p]["ema"].as_strided(p.shape, p.stride())
 
-    def _lacks_state(self, p):
-        st = self.state[p]
-        return not st or (self.ema_decay is not None and "ema" not in st)
-
     def _init_state(self, p):
         """The state of a parameter that has none, and the shadow of one whose loaded state has none."""
         st = self.state[p]
@@ -161,6 +157,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        shadow = self.ema_decay is not None
         calls = []  # (group, parameters, gradients in memory order, step number)
         for group in self.param_groups:
             live = [p for p in group["params"] if p.grad is not None]
@@ -170,7 +167,8 @@ class AdamW(torch.optim.Optimizer):
             if capturing and not self.capturable:
                 raise ValueError("AdamW: a step is captured into a graph with capturable=True only")
             for p in live:
-                if self._lacks_state(p):
+                st = self.state[p]
+                if not st or (shadow and "ema" not in st):
                     if capturing:
                         raise ValueError("AdamW: take one step before a step is captured into a graph")
                     self._init_state(p)
