@@ -17,7 +17,11 @@
 // from tensor memory through the epilogue while the next tile's products run (two accumulators).
 // Rows, columns and k past the end are TMA's zero fill and clipped stores.  Where the tiles are too few
 // to fill the GPU, k is split: each part writes its float32 tile to a workspace and a second kernel
-// adds the parts in order and runs the epilogue.  A few rows (M <= 16, <= 32 of fewer outputs) take a kernel of their own
+// adds the parts in order and runs the epilogue.  The tensor cores' operands have 16 bits, so what is computed
+// here and multiplied again (an MLP's hidden activation, the gradient at z) is rounded to them once, and z is
+// kept in them: a layer's gradients behind an activation are off by 2.4e-3 (bf16, 2-norm) where their own rounding
+// makes 1.7e-3; carrying a second operand of the remainders would double the backward's products.  Sums (accumulators,
+// parts, column sums) are float32 throughout.  A few rows (M <= 16, <= 32 of fewer outputs) take a kernel of their own
 // that streams the weights once through registers.
 //
 // Bound by the tensor cores where the tiles fill the GPU: 4096 x 2048 x 8192 in bf16 92-98 us (1400-1490
@@ -930,8 +934,7 @@ static int device_sms() {
 // four 128 x 128 tiles' 128 KB) and wins where its tiles fill the GPU (12544 x 2304 x 768 forward: 37 us,
 // 49 on 128 x 128, 88 on 128 x 64); fewer rows or columns take smaller tiles (256 x 768 x 768: 10.4,
 // 8.1 and 7.7 us), and long sums over few tiles are split (dW of 768 x 768 from 12544 rows: 61 us whole,
-// 21 in eight parts; dW of 4096 x 1024, whose tiles nearly fill the GPU: 75 and 87 us in two).  Over 16
-// shapes the choice was within 5 % of the best of all tiles and 1 to 12 parts ----
+// 21 in eight parts; dW of 4096 x 1024, whose tiles nearly fill the GPU: 75 and 87 us in two) ----
 struct Plan {
   int cg, bn, splits, per_split;
 };
