@@ -427,7 +427,8 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
   static variable_list backward(AutogradContext *ctx, variable_list dys) {
     refuse_uncapturable_leaves(dys[0].device());
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor x = saved[0].detach(), w = saved[1].detach(), z = saved[2], dy = dys[0].detach();
+    Tensor x = saved[0].detach(), w = saved[1].detach(), z = saved[2];
+    const Tensor dy = dys[0].detach();
     const int64_t n = w.size(0), k = w.size(1);
     const int act = (int)ctx->saved_data["act"].toInt();
     const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
@@ -443,6 +444,10 @@ struct LinearAct : public torch::autograd::Function<LinearAct> {
       if (need_b) g[2] = at::zeros({n}, w.options());
     } else if (need_x || need_w || need_b) {
       const c10::cuda::CUDAGuard guard(x.device());
+      // a hook on saved tensors (save_on_cpu) gives them back without their padded rows
+      x = readable(rows_of(x, k));
+      w = readable(rows_of(w, k));
+      if (z.defined()) z = rows_of(z, n);
       const Tensor dz = gradient_at_sum(act, rows_of(dy, n), z, need_b, g[2]);
       if (need_x) {
         g[0] = at::empty(sizes, x.options());
@@ -484,8 +489,8 @@ struct Mlp : public torch::autograd::Function<Mlp> {
   static variable_list backward(AutogradContext *ctx, variable_list dys) {
     refuse_uncapturable_leaves(dys[0].device());
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor x = saved[0].detach(), w1 = saved[1].detach(), w2 = saved[2].detach(), h = saved[3], z = saved[4],
-                 dy = dys[0].detach();
+    Tensor x = saved[0].detach(), w1 = saved[1].detach(), w2 = saved[2].detach(), h = saved[3], z = saved[4];
+    const Tensor dy = dys[0].detach();
     const int64_t n = w1.size(0), k = w1.size(1), out = w2.size(0);
     const int act = (int)ctx->saved_data["act"].toInt();
     const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
@@ -503,6 +508,12 @@ struct Mlp : public torch::autograd::Function<Mlp> {
       if (need_b2) g[4] = at::zeros({out}, w2.options());
     } else if (need_x || need_w1 || need_b1 || need_w2 || need_b2) {
       const c10::cuda::CUDAGuard guard(x.device());
+      // as in LinearAct
+      x = readable(rows_of(x, k));
+      w1 = readable(rows_of(w1, k));
+      w2 = readable(rows_of(w2, n));
+      h = readable(rows_of(h, n));
+      if (z.defined()) z = rows_of(z, n);
       const Tensor dy2 = gradient_at_sum(KDA_ACT_NONE, rows_of(dy, out), Tensor(), need_b2, g[4]);
       if (need_w2) g[3] = wgrad(dy2, h);
       if (need_x || need_w1 || need_b1) {

@@ -674,3 +674,23 @@ def test_mlp_split_hidden_gradient(cuda, dtype, act, m, k, n, out):
     assert _lib.lib().kda_linear_workspace_bytes(_lib.KDA_LINEAR_DGRAD, m, out, n, 1) >= sums + 2 * m * n * 4
     check_mlp(m, k, n, out, dtype, act, True, True, seed=22)
     check_mlp(m, k, n, out, dtype, act, False, False, seed=23)
+
+
+@pytest.mark.parametrize("act", ["none", "silu"])
+@pytest.mark.parametrize("k,n", [(64, 72), (75, 37), (64, 37), (75, 72)])
+def test_hooks_on_saved_tensors(cuda, k, n, act):
+    """What a hook gives back for a saved tensor has its values and not its padded rows, nor their order in memory."""
+    g = gen(24)
+    x, w, b = rnd(g, 100, k, dt=torch.bfloat16), rnd(g, n, k, dt=torch.bfloat16, scale=0.1), rnd(g, n, dt=torch.bfloat16)
+    w2, r, dy = (rnd(g, *s, dt=torch.bfloat16) for s in ((k, n), (100, n), (100, n)))
+    for t in (x, w, b, w2, r):
+        t.requires_grad_()
+    calls = [(lambda: linear_act(x, w, b, act, r), (x, w, b, r), dy), (lambda: mlp(x, w, b, w2, None, act, x), (x, w, b, w2), x)]
+    turned = torch.autograd.graph.saved_tensors_hooks(lambda t: t.t().contiguous() if t.dim() == 2 else t,
+                                                      lambda t: t.t() if t.dim() == 2 else t)
+    for call, leaves, d in calls:
+        want = torch.autograd.grad(call(), leaves, d)
+        for hook in (torch.autograd.graph.save_on_cpu(), turned):
+            with hook:
+                y = call()
+            assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, leaves, d), want))
