@@ -96,7 +96,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     _need(0 <= first_tensor < 1 << 31, "first_tensor counts from 0")
     return _lib.tensors().adamw_step(list(params), list(grads), list(exp_avgs), list(exp_avg_sqs),
                                      None if emas is None else list(emas), step, lr, betas[0], betas[1], eps, weight_decay,
-                                     bias_correction, max_grad_norm or 0.0, ema_decay or 0.0, seed & 0xFFFFFFFF, norm, first_tensor)
+                                     bias_correction, max_grad_norm or 0.0, ema_decay or 0.0, seed & 0xFFFFFFFF, norm,
+                                     first_tensor)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -106,8 +107,9 @@ class AdamW(torch.optim.Optimizer):
     step's norm is ``self.grad_norm``); ``ema_decay`` keeps a float32 shadow of every parameter
     (``ema_of``), started at the parameter's first step, or the first after states without a shadow
     were loaded.  ``capturable`` keeps the step's number and the learning rate on the device, so that
-    ``step`` can be captured into a CUDA graph after one eager step; the parameters of a group then share one step number and all need
-    gradients, and ``lr`` is the tensor ``group["lr"]`` (fill it to change it).
+    ``step`` can be captured into a CUDA graph after one eager step; the parameters of a group then
+    share one step number and all need gradients, and ``lr`` is the tensor ``group["lr"]`` (fill it
+    to change it).
     """
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *,
